@@ -1,0 +1,258 @@
+// What the products of the linear layers need around them: the gradient of the
+// activation with the bias gradient's column sums, and rows laid out for TMA.
+#include "linear_common.cuh"
+
+namespace wave {
+
+namespace {
+
+using namespace linear_detail;
+
+// PDL as in the product kernels: set-up may overlap the kernel before this one.
+template <typename Kernel, typename... Args>
+cudaError_t launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, Kernel kernel, const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ------------------------------------------------------------------- packing
+// Eight elements to a thread, neighbouring threads on neighbouring pieces of a
+// row; the source may start at any element, so it is read 2 bytes at a time
+// (a warp still reads 512 consecutive bytes) and written 16.
+__global__ void __launch_bounds__(256)
+pack_rows_kernel(const uint16_t *src, long long ld_src, long long group_src, uint16_t *dst, long long ld_dst,
+                 long long group_dst, int rows, int cols, int pieces) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const long long total = static_cast<long long>(rows) * pieces;
+  const uint16_t *s = src + blockIdx.y * group_src;
+  uint16_t *d = dst + blockIdx.y * group_dst;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long r = i / pieces;
+    const int c = static_cast<int>(i - r * pieces) * 8;
+    const uint16_t *row = s + r * ld_src + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t lo = c + 2 * e < cols ? row[2 * e] : 0u, hi = c + 2 * e + 1 < cols ? row[2 * e + 1] : 0u;
+      w[e] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4 *>(d + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// -------------------------------------------- activation gradient, column sums
+constexpr int kAgThreads = 256;
+constexpr int kAgCols = 256;                   // columns of a block, eight to a thread
+constexpr int kAgLanes = kAgThreads / (kAgCols / 8); // rows side by side
+constexpr int kAgUnroll = 4;                   // rows in flight for each thread
+
+struct Eight {
+  float v[8];
+};
+
+// Eight consecutive values of a row, zero beyond `cols`.
+__device__ __forceinline__ void load_eight(Eight &out, const void *base, long long at, int live, bool f32, bool vec,
+                                           int bf16) {
+  if (f32) {
+    const float *src = static_cast<const float *>(base) + at;
+    if (vec && live >= 8) {
+      const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+      out.v[0] = a.x, out.v[1] = a.y, out.v[2] = a.z, out.v[3] = a.w;
+      out.v[4] = b.x, out.v[5] = b.y, out.v[6] = b.z, out.v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        out.v[e] = e < live ? src[e] : 0.0f;
+    }
+    return;
+  }
+  const uint16_t *src = static_cast<const uint16_t *>(base) + at;
+  if (vec && live >= 8) {
+    const uint4 q = *reinterpret_cast<const uint4 *>(src);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_pair(w[e], bf16);
+      out.v[2 * e] = f.x;
+      out.v[2 * e + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      out.v[e] = e < live ? from_16bit(src[e], bf16) : 0.0f;
+  }
+}
+
+// One chunk of rows x 256 columns to a block.  A chunk never crosses a group's
+// end, so its column sums go to one group; which rows chunk `blockIdx.y` has
+// comes from the offsets, on the device.
+__global__ void __launch_bounds__(kAgThreads)
+act_grad_kernel(const __grid_constant__ LinearActGrad p) {
+  extern __shared__ int ag_smem[];
+  __shared__ float sums[kAgLanes][kAgCols];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int r0, r1;
+  if (p.offsets) {
+    GroupTable t{ag_smem, ag_smem + p.groups + 1};
+    build_group_table(t, p.offsets, p.groups, p.rows, p.chunk_rows);
+    const int chunk = blockIdx.y;
+    if (chunk >= t.blocks[p.groups])
+      return;
+    int lo = 0, hi = p.groups; // the group with blocks[lo] <= chunk < blocks[lo + 1]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (t.blocks[mid] <= chunk)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    r0 = t.begin[lo] + (chunk - t.blocks[lo]) * p.chunk_rows;
+    r1 = min(r0 + p.chunk_rows, t.begin[lo + 1]);
+  } else {
+    r0 = static_cast<int>(blockIdx.y) * p.chunk_rows;
+    r1 = min(r0 + p.chunk_rows, p.rows);
+  }
+  const int tc = threadIdx.x % (kAgCols / 8), tr = threadIdx.x / (kAgCols / 8);
+  const int col = static_cast<int>(blockIdx.x) * kAgCols + tc * 8;
+  const int live = p.cols - col;
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    acc[e] = 0.0f;
+  if (live > 0) {
+    for (int r = r0 + tr; r < r1; r += kAgLanes * kAgUnroll) {
+      Eight g[kAgUnroll], z[kAgUnroll];
+#pragma unroll
+      for (int u = 0; u < kAgUnroll; ++u) {
+        const int row = r + u * kAgLanes;
+        if (row < r1) {
+          load_eight(g[u], p.dY, static_cast<long long>(row) * p.ldy + col, live, p.dy_f32 != 0, p.vec_dy != 0, p.is_bf16);
+          if (p.Z)
+            load_eight(z[u], p.Z, static_cast<long long>(row) * p.ldz + col, live, false, p.vec_z != 0, p.is_bf16);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAgUnroll; ++u) {
+        const int row = r + u * kAgLanes;
+        if (row >= r1)
+          break;
+        if (p.Z) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            g[u].v[e] *= act_slope(z[u].v[e], p.act);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          acc[e] += g[u].v[e];
+        if (p.dZ) {
+          // rows of dZ are padded to whole 16-byte pieces; columns behind the last are zero
+          uint4 q;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = pack_pair(2 * e < live ? g[u].v[2 * e] : 0.0f, 2 * e + 1 < live ? g[u].v[2 * e + 1] : 0.0f, p.is_bf16);
+          q = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dZ) + static_cast<long long>(row) * p.lddz + col) = q;
+        }
+      }
+    }
+  }
+  if (!p.partial)
+    return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    sums[tr][tc * 8 + e] = acc[e];
+  __syncthreads();
+  const int c = static_cast<int>(blockIdx.x) * kAgCols + threadIdx.x;
+  if (c < p.cols) {
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kAgLanes; ++r)
+      s += sums[r][threadIdx.x];
+    p.partial[static_cast<long long>(blockIdx.y) * p.cols + c] = s;
+  }
+}
+
+// The chunks' sums of each group added up: 32 columns x 8 strands of chunks to a
+// block, strands joined in order.
+__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ LinearActGrad p) {
+  extern __shared__ int ag_smem[];
+  __shared__ float sums[8][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int c0 = 0, c1 = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
+  if (p.offsets) {
+    GroupTable t{ag_smem, ag_smem + p.groups + 1};
+    build_group_table(t, p.offsets, p.groups, p.rows, p.chunk_rows);
+    c0 = t.blocks[blockIdx.y];
+    c1 = t.blocks[blockIdx.y + 1];
+  }
+  const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
+  const int col = static_cast<int>(blockIdx.x) * 32 + lane;
+  float s = 0.0f;
+  if (col < p.cols) {
+#pragma unroll 4
+    for (int c = c0 + strand; c < c1; c += 8)
+      s += p.partial[static_cast<long long>(c) * p.cols + col];
+  }
+  sums[strand][lane] = s;
+  __syncthreads();
+  if (strand == 0 && col < p.cols) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      total += sums[i][lane];
+    const long long at = static_cast<long long>(blockIdx.y) * p.cols + col;
+    if (p.dbias_type == 0)
+      static_cast<float *>(p.dbias)[at] = total;
+    else
+      static_cast<uint16_t *>(p.dbias)[at] = to_16bit(total, p.dbias_type == 2);
+  }
+}
+
+} // namespace
+
+cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
+                             long long group_dst, int rows, int cols, int groups, cudaStream_t stream) {
+  const int pieces = (cols + 7) / 8;
+  const long long blocks = (static_cast<long long>(rows) * pieces + 255) / 256;
+  if (blocks == 0 || groups == 0)
+    return cudaSuccess;
+  // enough blocks to fill the machine; the rest in the kernel's loop
+  const unsigned grid = static_cast<unsigned>(blocks < 4096 ? blocks : 4096);
+  return launch(dim3(grid, static_cast<unsigned>(groups)), 256, 0, stream, pack_rows_kernel,
+                static_cast<const uint16_t *>(src), ld_src, group_src, static_cast<uint16_t *>(dst), ld_dst, group_dst, rows,
+                cols, pieces);
+}
+
+int linear_act_grad_chunks(int rows, int groups, int chunk_rows) {
+  const int whole = (rows + chunk_rows - 1) / chunk_rows;
+  return groups > 0 ? rows / chunk_rows + (groups < rows ? groups : rows) : whole;
+}
+
+cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
+  const int chunks = linear_act_grad_chunks(p.rows, p.offsets ? p.groups : 0, p.chunk_rows);
+  const size_t table = p.offsets ? 2 * sizeof(int) * (static_cast<size_t>(p.groups) + 1) : 0;
+  cudaError_t err = cudaSuccess;
+  if (chunks > 0)
+    err = launch(dim3(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks)), kAgThreads,
+                 table, stream, act_grad_kernel, p);
+  if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
+    return err;
+  return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(p.offsets ? p.groups : 1)), 256, table,
+                stream, column_sum_kernel, p);
+}
+
+} // namespace wave

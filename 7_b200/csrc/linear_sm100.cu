@@ -1,0 +1,588 @@
+// Products of the linear layers on one CTA: D = act(A * B^T + bias) + residual,
+// dense or grouped by expert, and the two products of the backward pass.
+//
+// One 128 x TN tile at a time: TMA fills a ring of 64-deep stages (128-byte
+// swizzled rows), one thread issues tcgen05.mma into one of two accumulators in
+// tensor memory, four or eight warps take the finished one through the epilogue
+// while the next tile accumulates.  What the operands look like is in the
+// descriptors alone:
+//   forward            A, B stored with the contraction last (K-major)
+//   input gradient     dx = dz W: W is stored [contraction][columns], MN-major
+//   weight gradient    dW = dz^T x: both MN-major, contraction = token rows
+// With few tokens the operands change sides (kSwap): the weights fill the 128
+// rows of the tensor core's tile and the tokens its 16..128 columns, so that no
+// row of the machine multiplies padding and the weights are read once.
+//
+// Long contractions with few tiles are split over the CTAs of a cluster: each
+// leaves its partial tile in its own shared memory, and each sums a share of the
+// columns over the cluster in rank order (fixed, so results do not vary), with
+// no workspace, no counters and nothing to clear.
+//
+// Experts: the row ranges are read on the device (no host sync).  A row block
+// ends at its expert's last row by not storing the rows behind it; a weight
+// gradient's last 64 rows are cut to the expert's by zeroing what TMA brought in
+// of the next one's in shared memory (in both operands: 0 * NaN would stay).
+//
+// f32 results: the tensor core adds to its f32 accumulator by truncation, an
+// error that grows with the length of the sum (measured relative to the norm:
+// 4.7e-7 at K = 512, 9e-6 at 8192, 3.8e-5 at 32768).  Behind a 16-bit rounding
+// (4e-3 / 5e-4) that is nothing; f32 results are summed in registers, rounded to
+// nearest, from accumulators of kSegment * 64 = 512 products each.
+#include "launch_cache.h"
+#include "linear_common.cuh"
+
+namespace wave {
+
+__device__ int g_linear_status[4]; // [0] code, [1] linear block, [2] role, [3] detail
+
+namespace {
+
+using namespace linear_detail;
+
+constexpr int kTileP = 128;
+constexpr int kBK = 64;
+constexpr int kChunkBytes = 64 * 128; // 64 rows of 128 bytes: a 64-element MN chunk of a stage
+constexpr int kABytes = kTileP * kBK * 2;
+constexpr int kMaxStages = 12;
+constexpr int kSegment = 8; // stages of an accumulator that is summed in registers
+constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
+constexpr int kSmemLimit = 227 * 1024;
+
+struct Shared {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Shared) <= 1024, "Shared outgrew its slot");
+
+template <int TN, bool kF32> struct Cfg {
+  static constexpr int kEpiWarps = TN >= 128 ? 8 : 4;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kBBytes = TN * kBK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kSlots = kEpiWarps * slot_bytes<kF32>();
+  static constexpr int kFit = (kSmemLimit - 1024 - 1024 - kTableBytes - kSlots) / kStageBytes;
+  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  static constexpr int kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
+  static constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots; // + the group table
+  static_assert(kStages >= 4, "ring too short");
+  static_assert(TN * kTileP * 4 <= kStages * kStageBytes, "a partial tile must fit the ring");
+};
+
+__device__ __noinline__ void report(int code, int role, int detail) {
+  if (atomicCAS(&g_linear_status[0], 0, code) == 0) {
+    g_linear_status[1] = static_cast<int>(blockIdx.x);
+    g_linear_status[2] = role;
+    g_linear_status[3] = detail;
+  }
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int W> __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[W]) {
+  static_assert(W == 16 || W == 32, "16 or 32 columns");
+  uint32_t r[W];
+  if constexpr (W == 32)
+    tmem_ld_32x32b_x32(addr, r);
+  else
+    tmem_ld_32x32b_x16(addr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    v[i] = __uint_as_float(r[i]);
+}
+
+template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
+__global__ void __launch_bounds__(Cfg<TN, kF32>::kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+              const __grid_constant__ LinearParams p) {
+  using C = Cfg<TN, kF32>;
+  constexpr int kStages = C::kStages;
+  constexpr bool kCut = kAMn && kBMn; // the weight gradient: stages may have to be cut at the last row
+  constexpr int kColGroups = C::kEpiWarps / 4;
+  constexpr int kMyCols = TN / kColGroups; // columns of an epilogue warp
+  constexpr int W = kMyCols < 32 ? kMyCols : 32;
+  static_assert(!kF32 || kMyCols <= 64, "running sums stay in registers");
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Shared *sh = reinterpret_cast<Shared *>(tiles + kStages * C::kStageBytes);
+  uint8_t *slots = tiles + kStages * C::kStageBytes + 1024;
+  GroupTable table;
+  table.begin = reinterpret_cast<int *>(slots + C::kSlots);
+  table.blocks = table.begin + p.groups + 1;
+  volatile int *abort_flag = &sh->abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int splits = p.splits;
+  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first_tile = splits > 1 ? static_cast<int>(blockIdx.x) / splits : static_cast<int>(blockIdx.x);
+  const int tile_step = splits > 1 ? 0x3FFFFFFF : static_cast<int>(gridDim.x); // a cluster has one tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&sh->tfull[a], 1);
+      mbar_init(&sh->tempty[a], C::kEpiWarps);
+    }
+    sh->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = sh->tmem_base;
+  // Up to here only this CTA's own state was touched: it may run while the kernel
+  // before this one on the stream is finishing.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.ragged != kRaggedNone)
+    build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : (kSwap ? p.Q : p.P),
+                      kSwap ? p.tile_q : kTileP);
+
+  // This CTA's share of a tile's stages.
+  auto k_blocks = [&](const Tile &w, int &kb0, int &kb1) {
+    const int total = (w.k_len + kBK - 1) / kBK;
+    kb0 = splits > 1 ? static_cast<int>(static_cast<long long>(total) * rank / splits) : 0;
+    kb1 = splits > 1 ? static_cast<int>(static_cast<long long>(total) * (rank + 1) / splits) : total;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- loads
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_a);
+      tma_prefetch_desc(&tm_b);
+      TileWalk<kSwap> walk(p, table, kTileP);
+      Tile w;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t tx = kABytes + static_cast<uint32_t>(p.tile_q) * kBK * 2;
+      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+        int kb0, kb1;
+        k_blocks(w, kb0, kb1);
+        const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag)) {
+            report(kStatusWaitTimeout, 0, stage);
+            ok = false;
+            break;
+          }
+          uint8_t *a_dst = tiles + stage * C::kStageBytes;
+          uint8_t *b_dst = a_dst + kABytes;
+          uint64_t *bar = &sh->full[stage];
+          const int k = w.k_begin + kb * kBK;
+          mbar_arrive_expect_tx(bar, tx);
+          if constexpr (kAMn) {
+            for (int c = 0; c < kTileP / 64; ++c)
+              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, w.p0 + c * 64, k, za);
+          } else {
+            tma_load_3d(a_dst, &tm_a, bar, k, w.p0, za);
+          }
+          if constexpr (kBMn) {
+            for (int c = 0; c < p.tile_q / 64; ++c)
+              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, w.q0 + c * 64, k, zb);
+          } else {
+            tma_load_3d(b_dst, &tm_b, bar, k, w.q0, zb);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok)
+        bounded_delay(1 << 21); // let copies in flight land before teardown
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- UMMA issue
+    if (kCut || lane == 0) {
+      const uint32_t idesc = umma_idesc_f16(kTileP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
+      constexpr uint32_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
+      TileWalk<kSwap> walk(p, table, kTileP);
+      Tile w;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      // (a warp that works together gives up together)
+      auto wait = [&](uint64_t *bar, uint32_t parity) {
+        const bool got = mbar_wait(bar, parity, abort_flag);
+        if constexpr (kCut)
+          return __all_sync(0xffffffffu, got) != 0;
+        return got;
+      };
+      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+        int kb0, kb1;
+        k_blocks(w, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const bool first = kF32 ? (kb - kb0) % kSegment == 0 : kb == kb0;
+          const bool last = kb + 1 == kb1 || (kF32 && (kb - kb0) % kSegment == kSegment - 1);
+          if (first) {
+            ok = wait(&sh->tempty[acc], acc_phase ^ 1);
+            if (!ok) {
+              report(kStatusWaitTimeout, 1, 100 + acc);
+              break;
+            }
+          }
+          ok = wait(&sh->full[stage], phase);
+          if (!ok) {
+            report(kStatusWaitTimeout, 1, stage);
+            break;
+          }
+          uint8_t *a_tile = tiles + stage * C::kStageBytes;
+          const int live = min(kBK, w.k_len - kb * kBK); // contraction indices of this stage
+          const int steps = (live + 15) / 16;
+          if constexpr (kCut) {
+            if (p.ragged == kRaggedK && live < steps * 16) {
+              // rows [live, steps * 16) belong to the next expert or to nobody
+              const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
+              const int chunks = kTileP / 64 + p.tile_q / 64;
+              for (int i = lane; i < chunks * vecs; i += 32) {
+                uint8_t *dst = a_tile + (i / vecs) * kChunkBytes + live * 128 + (i % vecs) * 16;
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
+          }
+          tc_fence_after_sync();
+          if (lane == 0) {
+            const uint32_t a_addr = smem_u32(a_tile), b_addr = a_addr + kABytes;
+            const uint64_t da = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
+            const uint64_t db = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
+            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TN);
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k)
+              if (k < steps)
+                umma_ss(d, da + static_cast<uint64_t>(k * kStepA), db + static_cast<uint64_t>(k * kStepB), idesc,
+                        (!first || k > 0) ? 1u : 0u);
+            umma_commit(&sh->empty[stage]);
+            if (last)
+              umma_commit(&sh->tfull[acc]);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (last && ++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue
+    const int quarter = warp & 3; // tensor-memory lanes this warp may read
+    const int col0 = ((warp - 2) >> 2) * kMyCols;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint8_t *slot = slots + (warp - 2) * slot_bytes<kF32>();
+    TileWalk<kSwap> walk(p, table, kTileP);
+    Tile w;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    auto wait_acc = [&]() {
+      if (!mbar_wait(&sh->tfull[acc], acc_phase, abort_flag)) {
+        if (lane == 0)
+          report(kStatusWaitTimeout, 2, 200 + acc);
+        return false;
+      }
+      tc_fence_after_sync();
+      return true;
+    };
+    auto release_acc = [&]() {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&sh->tempty[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    };
+    for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+      int kb0, kb1;
+      k_blocks(w, kb0, kb1);
+      EpiTile t;
+      t.group = w.group;
+      t.lane0 = w.p0 + quarter * 32;
+      t.lane_end = w.p_end;
+      t.q_end = min(w.q_end, w.q0 + p.tile_q);
+      const float bias = kSwap && splits == 1 ? column_bias(p, t, lane) : 0.0f;
+      // columns of this warp that exist, in chunks of W
+      const int my_cols = min(kMyCols, p.tile_q - col0);
+      float *part = reinterpret_cast<float *>(tiles) + quarter * 32 + lane; // split: column c of the lane's row at c * 128
+      auto chunk = [&](int c, float (&v)[W], const uint4 (&res)[W / 8]) {
+        if (splits > 1) {
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            part[(c + j) * kTileP] = v[j];
+        } else if constexpr (kSwap) {
+          epilogue_columns<kF32, W>(p, t, w.q0 + c, 1, v, bias, lane);
+        } else {
+          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, res, slot, lane);
+        }
+      };
+      if constexpr (kF32) {
+        float run[kMyCols];
+#pragma unroll
+        for (int j = 0; j < kMyCols; ++j)
+          run[j] = 0.0f;
+        for (int kb = kb0; kb < kb1 && ok; kb += kSegment) {
+          ok = wait_acc();
+          if (!ok)
+            break;
+#pragma unroll
+          for (int c = 0; c < kMyCols; c += W) {
+            if (c >= my_cols)
+              break;
+            float v[W];
+            tmem_load<W>(lane_addr + static_cast<uint32_t>(acc * TN + col0 + c), v);
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+              run[c + j] += v[j];
+          }
+          release_acc();
+        }
+        if (!ok)
+          break;
+#pragma unroll
+        for (int c = 0; c < kMyCols; c += W) {
+          if (c >= my_cols)
+            break;
+          uint4 res[W / 8];
+          if (!kSwap && p.R && splits == 1)
+            fetch_residual<W>(res, p, t, w.q0 + col0 + c, lane);
+          float v[W];
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            v[j] = run[c + j];
+          chunk(col0 + c, v, res);
+        }
+      } else {
+        const bool empty = kb0 == kb1; // nothing to multiply: the epilogue of zero
+        uint4 res[W / 8];
+        const bool want_res = !kSwap && p.R && splits == 1;
+        if (want_res && my_cols > 0)
+          fetch_residual<W>(res, p, t, w.q0 + col0, lane);
+        if (!empty && !wait_acc()) {
+          ok = false;
+          break;
+        }
+#pragma unroll 1
+        for (int c = 0; c < my_cols; c += W) {
+          float v[W];
+          if (empty) {
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+              v[j] = 0.0f;
+          } else {
+            tmem_load<W>(lane_addr + static_cast<uint32_t>(acc * TN + col0 + c), v);
+          }
+          uint4 now[W / 8];
+#pragma unroll
+          for (int j = 0; j < W / 8; ++j)
+            now[j] = res[j];
+          if (want_res && c + W < my_cols)
+            fetch_residual<W>(res, p, t, w.q0 + col0 + c + W, lane);
+          chunk(col0 + c, v, now);
+        }
+        if (!empty)
+          release_acc();
+      }
+    }
+    if (p.zero_rest && p.ragged == kRaggedRows) {
+      // the rows in front of the first and behind the last group
+      const int rows = kSwap ? p.Q : p.P, cols = kSwap ? p.P : p.Q;
+      const int wid = static_cast<int>(blockIdx.x) * C::kEpiWarps + warp - 2, warps = static_cast<int>(gridDim.x) * C::kEpiWarps;
+      zero_rows(p.D, kF32 ? 4 : 2, p.ldd, 0, table.begin[0], cols, wid, warps, lane);
+      zero_rows(p.D, kF32 ? 4 : 2, p.ldd, table.begin[p.groups], rows, cols, wid, warps, lane);
+      if (p.Z) {
+        zero_rows(p.Z, 2, p.ldz, 0, table.begin[0], cols, wid, warps, lane);
+        zero_rows(p.Z, 2, p.ldz, table.begin[p.groups], rows, cols, wid, warps, lane);
+      }
+    }
+  }
+
+  if (splits > 1) {
+    // The partial tiles of the cluster: each CTA takes columns of all 128 rows
+    // and adds the parts in rank order.  Every CTA of the cluster passes both
+    // barriers whatever happened above.
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2 && *abort_flag == 0) {
+      const int quarter = warp & 3, half = (warp - 2) >> 2;
+      uint8_t *slot = slots + (warp - 2) * slot_bytes<kF32>();
+      TileWalk<kSwap> walk(p, table, kTileP);
+      Tile w;
+      if (walk.get(first_tile, w)) {
+        EpiTile t;
+        t.group = w.group;
+        t.lane0 = w.p0 + quarter * 32;
+        t.lane_end = w.p_end;
+        t.q_end = min(w.q_end, w.q0 + p.tile_q);
+        uint32_t peer[kLinearMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kLinearMaxSplits; ++s)
+          peer[s] = s < splits ? map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 4 : 0u;
+        if constexpr (kSwap) {
+          constexpr int B = 4; // tokens at a time: rank, rank + splits, ...
+          const float bias = column_bias(p, t, lane);
+          const int live = t.q_end - w.q0;
+          for (int j0 = rank + half * B * splits; j0 < live; j0 += kColGroups * B * splits) {
+            float v[B];
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+              v[j] = 0.0f;
+              const int col = j0 + j * splits;
+              if (col < live) {
+                float part[kLinearMaxSplits];
+#pragma unroll
+                for (int s = 0; s < kLinearMaxSplits; ++s)
+                  part[s] = s < splits ? ld_cluster_f32(peer[s] + col * (kTileP * 4)) : 0.0f;
+#pragma unroll
+                for (int s = 0; s < kLinearMaxSplits; ++s)
+                  v[j] += part[s];
+              }
+            }
+            epilogue_columns<kF32, B>(p, t, w.q0 + j0, splits, v, bias, lane);
+          }
+        } else {
+          constexpr int V = 16; // columns at a time
+          for (int i = rank + half * splits; i * V < p.tile_q; i += kColGroups * splits) {
+            const int q0 = w.q0 + i * V;
+            uint4 res[V / 8];
+            if (p.R)
+              fetch_residual<V>(res, p, t, q0, lane);
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              v[j] = 0.0f;
+#pragma unroll 1
+            for (int s = 0; s < splits; ++s) {
+              const uint32_t from = map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 4;
+#pragma unroll
+              for (int j = 0; j < V; ++j)
+                v[j] += ld_cluster_f32(from + (i * V + j) * (kTileP * 4));
+            }
+            epilogue_rows<kF32, V>(p, t, q0, v, res, slot, lane);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_arrive(); // nobody leaves while its part may still be read
+    cluster_wait();
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, C::kTmemCols);
+  }
+}
+
+template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
+cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                       cudaStream_t stream) {
+  using C = Cfg<TN, kF32>;
+  auto kernel = linear_kernel<TN, kAMn, kBMn, kSwap, kF32>;
+  cudaError_t err = prepare_kernel(kernel, C::kSmemFixed + kTableBytes, nullptr);
+  if (err != cudaSuccess)
+    return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (p.splits > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+}
+
+template <bool kAMn, bool kBMn, bool kSwap, bool kF32>
+cudaError_t launch_tile(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                        cudaStream_t stream) {
+  if constexpr (kSwap) {
+    switch (l.tile_n) {
+    case 16:
+      return launch_one<16, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+    case 32:
+      return launch_one<32, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+    }
+  }
+  switch (l.tile_n) {
+  case 64:
+    return launch_one<64, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+  case 128:
+    return launch_one<128, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+  }
+  if constexpr (!kSwap && !kF32) {
+    if (l.tile_n == 256)
+      return launch_one<256, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+template <bool kF32>
+cudaError_t launch_layout(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                          cudaStream_t stream) {
+  if (!l.a_mn && !l.b_mn)
+    return l.swap ? launch_tile<false, false, true, kF32>(ta, tb, p, l, stream)
+                  : launch_tile<false, false, false, kF32>(ta, tb, p, l, stream);
+  if (l.swap)
+    return cudaErrorInvalidValue;
+  if (!l.a_mn && l.b_mn) {
+    if constexpr (!kF32) // the input gradient has the operands' type
+      return launch_tile<false, true, false, kF32>(ta, tb, p, l, stream);
+  }
+  if (l.a_mn && l.b_mn)
+    return launch_tile<true, true, false, kF32>(ta, tb, p, l, stream);
+  return cudaErrorInvalidValue;
+}
+
+} // namespace
+
+cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                          cudaStream_t stream) {
+  return l.out_f32 ? launch_layout<true>(ta, tb, p, l, stream) : launch_layout<false>(ta, tb, p, l, stream);
+}
+
+cudaError_t linear_read_status(int out[4], bool clear) {
+  cudaError_t err = cudaMemcpyFromSymbol(out, g_linear_status, sizeof(int) * 4);
+  if (err == cudaSuccess && clear) {
+    int zero[4] = {0, 0, 0, 0};
+    err = cudaMemcpyToSymbol(g_linear_status, zero, sizeof(zero));
+  }
+  return err;
+}
+
+} // namespace wave

@@ -1,0 +1,95 @@
+// Internal interface between the C-ABI backend and the sm_100a kernels of the
+// linear layers: matrix products with bias, activation and residual in their
+// epilogue, dense or grouped by expert, and the products of their backward pass.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace wave {
+
+enum LinearAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+
+// Which extent of a product follows the experts' offsets.
+enum LinearRagged : int {
+  kRaggedNone = 0,
+  kRaggedRows = 1, // the token rows of the output (forward, input gradient)
+  kRaggedK = 2,    // the contraction (weight gradient): one output matrix for each expert
+};
+
+constexpr int kLinearMaxGroups = 1024; // two ints of shared memory for each
+constexpr int kLinearMaxSplits = 8;    // CTAs of a cluster that share one tile's contraction
+
+// Kernel-space product D[P x Q] = A[P x K] * B[Q x K]^T.  The P side takes the
+// 128 rows of the tensor core's tile, the Q side its 16..256 columns.  With
+// `swap` the features are on the P side and the tokens on the Q side (few
+// tokens), otherwise tokens are rows; the weight gradient has out-features on P
+// and in-features on Q.  D's element (token m, feature n) is at m * ldd + n
+// either way.
+struct LinearParams {
+  int P, Q, K;       // extents; the ragged one is its upper bound (all tokens)
+  int ragged, groups;
+  const int *offsets; // [groups + 1], on the device; null when not ragged
+  int group_a, group_b; // the operand has one matrix for each group (third coordinate of its tensor map)
+  int tile_q;        // columns of a tile: a multiple of 16 (of 64 where B is stored [K][Q]) <= the kernel's tile
+  int p_blocks, q_blocks; // tiles along each side (ragged side: unused)
+  int raster;        // row blocks that are walked down before the next column block
+  int splits;        // CTAs of a cluster that share a tile's contraction; then one tile for each cluster
+  int is_bf16;       // operands, z, residual and 16-bit outputs: bf16 or f16
+  int act;
+  // D
+  void *D;
+  long long ldd, group_d;
+  void *Z;           // pre-activation, 16-bit, or null
+  long long ldz;
+  const void *R;     // residual, 16-bit, or null
+  long long ldr;
+  const void *bias;  // or null
+  int bias_f32;
+  long long group_bias;
+  int vec_d, vec_z, vec_r; // 16-byte accesses are aligned in D / Z / R
+  int zero_rest;     // rows of D and Z that belong to no group are set to zero
+};
+
+struct LinearLaunch {
+  int a_mn, b_mn; // operand stored with the contraction as its slow direction
+  int swap;
+  int tile_n;     // kernel instantiation: 16, 32, 64, 128 or 256 columns
+  int out_f32;
+  int grid;       // CTAs (a multiple of splits)
+  int pair;       // CTA-pair kernel
+};
+
+int linear_stage_box_rows();
+cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                          cudaStream_t stream);
+cudaError_t linear_read_status(int out[4], bool clear);
+
+// ---- helpers around the products (linear_aux_sm100.cu)
+// 16-bit rows with any stride into rows of `ld_dst` elements: what a TMA load
+// needs (16-byte strides) of an operand that does not have it.
+cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
+                             long long group_dst, int rows, int cols, int groups, cudaStream_t stream);
+
+// dz = dy * act'(z), rounded to the operands' type, and the column sums of the
+// unrounded dz (dbias) of each group in two steps of fixed order.
+struct LinearActGrad {
+  int rows, cols, groups;
+  const int *offsets; // null: one group of all rows
+  int act, is_bf16, dy_f32;
+  const void *dY;
+  long long ldy;
+  const void *Z; // null when act is none
+  long long ldz;
+  void *dZ; // null: column sums only
+  long long lddz;
+  float *partial; // [chunks][cols], null: no column sums
+  int chunk_rows;
+  void *dbias; // [groups][cols]
+  int dbias_type; // 0 f32, 1 f16, 2 bf16
+  int vec_dy, vec_z;
+};
+int linear_act_grad_chunks(int rows, int groups, int chunk_rows); // upper bound, sizes `partial`
+cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream);
+
+} // namespace wave

@@ -10,6 +10,7 @@
 #include "backend_env.h"
 #include "fa_sm100.h"
 #include "gemm_sm100.h"
+#include "linear_sm100.h"
 
 #include <cmath>
 #include <cstdarg>
@@ -99,6 +100,16 @@ EnvKnobs read_env() {
     const int cycles = atoi(v);
     e.fa_stagger = cycles < 0 ? 0 : (cycles > 100000 ? 100000 : cycles); // a bounded spin, whatever is asked
   }
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_TILE")) {
+    const int n = atoi(v);
+    e.linear_tile = (n == 16 || n == 32 || n == 64 || n == 128 || n == 256) ? n : 0;
+  }
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_SPLITS")) {
+    const int n = atoi(v);
+    e.linear_splits = (n >= 1 && n <= 8) ? n : 0;
+  }
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_SWAP"))
+    e.linear_swap = !strcmp(v, "0") ? 0 : !strcmp(v, "1") ? 1 : -1;
   return e;
 }
 } // namespace
@@ -1323,13 +1334,16 @@ int wave_cuda_check_device_status(int *out4) {
   }
   if ((err = wave::fa_read_status(f, true)) != cudaSuccess)
     return cuda_fail(err, "read attention status");
-  const int *bad = g[0] ? g : (f[0] ? f : nullptr);
+  int l[4] = {0, 0, 0, 0};
+  if ((err = wave::linear_read_status(l, true)) != cudaSuccess)
+    return cuda_fail(err, "read linear layer status");
+  const int *bad = g[0] ? g : (f[0] ? f : (l[0] ? l : nullptr));
   if (out4)
     for (int i = 0; i < 4; ++i)
       out4[i] = bad ? bad[i] : 0;
   if (bad)
     return fail(WAVE_E_DEVICE_STATUS, "%s kernel reported status %d (block %d, role %d, detail %d)",
-                bad == g ? "GEMM" : "attention", bad[0], bad[1], bad[2], bad[3]);
+                bad == g ? "GEMM" : bad == f ? "attention" : "linear layer", bad[0], bad[1], bad[2], bad[3]);
   return WAVE_OK;
 }
 

@@ -1,0 +1,549 @@
+// Host side of the linear layers (include/wave_cuda.h, "linear layers"): checks,
+// workspace, tensor maps and the choice of tiles for the products with an
+// epilogue, dense and grouped by expert, forward and backward.
+#include "../../include/wave_cuda.h"
+#include "backend_env.h"
+#include "fa_sm100.h" // make_tensor_map_16bit
+#include "linear_sm100.h"
+
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <exception>
+
+namespace wave {
+void set_last_error(const char *message); // wave_cuda_backend.cu
+}
+
+namespace {
+
+using wave::LinearLaunch;
+using wave::LinearParams;
+
+int fail(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  wave::set_last_error(buf);
+  return code;
+}
+int cuda_fail(cudaError_t err, const char *what) {
+  return fail(WAVE_E_CUDA, "%s: %s", what, cudaGetErrorString(err));
+}
+
+// No C++ exception leaves a C entry (std::bad_alloc of the small host objects).
+template <typename F> int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception &e) {
+    return fail(WAVE_E_CUDA, "host side failed: %s", e.what());
+  } catch (...) {
+    return fail(WAVE_E_CUDA, "host side failed");
+  }
+}
+
+int sm_count(int *out) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess)
+    return cuda_fail(err, "cudaGetDevice");
+  err = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev);
+  return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "cudaDeviceGetAttribute");
+}
+
+long long round_up(long long v, long long a) { return (v + a - 1) / a * a; }
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ---------------------------------------------------------------- descriptor
+// The descriptor with its zeros replaced by what they stand for.
+struct Shape {
+  wave_linear_desc d;
+  bool grouped;
+  int matrices; // weight matrices
+};
+
+Shape resolve(const wave_linear_desc &in) {
+  Shape s;
+  s.d = in;
+  wave_linear_desc &d = s.d;
+  s.grouped = d.experts > 0;
+  s.matrices = s.grouped ? d.experts : 1;
+  auto rows = [](long long &ld, int rows, long long cols) {
+    // a single row has no stride: take one that every access likes
+    if (ld == 0)
+      ld = cols;
+    if (rows <= 1)
+      ld = round_up(cols, 8);
+  };
+  rows(d.ldx, d.tokens, d.in_features);
+  rows(d.ldy, d.tokens, d.out_features);
+  rows(d.ldr, d.tokens, d.out_features);
+  rows(d.ldz, d.tokens, d.out_features);
+  rows(d.lddx, d.tokens, d.in_features);
+  rows(d.ldw, d.out_features, d.in_features);
+  rows(d.lddw, d.out_features, d.in_features);
+  // (one row to a matrix: the matrices follow one another without the padding
+  // that `rows` assumed)
+  if (d.expert_stride_w == 0)
+    d.expert_stride_w = (in.ldw ? in.ldw : d.in_features) * static_cast<long long>(d.out_features);
+  if (d.expert_stride_dw == 0)
+    d.expert_stride_dw = (in.lddw ? in.lddw : d.in_features) * static_cast<long long>(d.out_features);
+  return s;
+}
+
+int validate(const wave_linear_desc *d) {
+  if (!d)
+    return fail(WAVE_E_INVALID, "descriptor is null");
+  if (d->tokens < 0)
+    return fail(WAVE_E_INVALID, "tokens must be >= 0; got %d", d->tokens);
+  if (d->out_features < 1 || d->in_features < 1)
+    return fail(WAVE_E_INVALID, "out_features and in_features must be >= 1; got %d and %d", d->out_features,
+                d->in_features);
+  if (d->experts < 0 || d->experts > wave::kLinearMaxGroups)
+    return fail(WAVE_E_INVALID, "experts must be between 0 (one weight matrix) and %d; got %d", wave::kLinearMaxGroups,
+                d->experts);
+  if (d->io_type != WAVE_BF16 && d->io_type != WAVE_F16)
+    return fail(WAVE_E_UNSUPPORTED, "io_type must be bf16 or f16; got %d", d->io_type);
+  const int types[4] = {d->y_type, d->bias_type, d->dweight_type, d->dbias_type};
+  const char *names[4] = {"y_type", "bias_type", "dweight_type", "dbias_type"};
+  for (int i = 0; i < 4; ++i)
+    if (types[i] != d->io_type && types[i] != WAVE_F32)
+      return fail(WAVE_E_UNSUPPORTED, "%s must be io_type or f32; got %d", names[i], types[i]);
+  if (d->activation < WAVE_ACT_NONE || d->activation > WAVE_ACT_SILU)
+    return fail(WAVE_E_INVALID, "activation must be one of none, relu, gelu, gelu_tanh, silu; got %d", d->activation);
+  const long long lds[7] = {d->ldx, d->ldw, d->ldy, d->ldr, d->ldz, d->lddx, d->lddw};
+  const char *ld_names[7] = {"ldx", "ldw", "ldy", "ldr", "ldz", "lddx", "lddw"};
+  const int cols[7] = {d->in_features, d->in_features,  d->out_features, d->out_features,
+                       d->out_features, d->in_features, d->in_features};
+  for (int i = 0; i < 7; ++i)
+    if (lds[i] != 0 && (lds[i] < cols[i] || lds[i] > (1ll << 36)))
+      return fail(WAVE_E_INVALID, "%s must be 0 or between %d and 2^36 elements; got %lld", ld_names[i], cols[i], lds[i]);
+  const Shape s = resolve(*d);
+  if (s.grouped) {
+    const long long strides[2] = {s.d.expert_stride_w, s.d.expert_stride_dw};
+    const long long lds2[2] = {d->ldw ? d->ldw : d->in_features, d->lddw ? d->lddw : d->in_features};
+    for (int i = 0; i < 2; ++i)
+      if (strides[i] < lds2[i] * (d->out_features - 1) + d->in_features || strides[i] > (1ll << 38))
+        return fail(WAVE_E_INVALID, "%s must be 0 or hold a whole matrix (at most 2^38 elements); got %lld",
+                    i == 0 ? "expert_stride_w" : "expert_stride_dw", strides[i]);
+  }
+  // Tile counts stay far inside 32 bits: 16-token tiles of 128 features, 128 x 64 tiles of each gradient.
+  const long long token_tiles = (static_cast<long long>(d->tokens) + 15) / 16 + s.matrices;
+  const long long f_tiles = ((d->out_features > d->in_features ? d->out_features : d->in_features) + 63) / 64;
+  const long long w_tiles = ((d->out_features + 127ll) / 128) * ((d->in_features + 63ll) / 64) * s.matrices;
+  if (token_tiles * f_tiles > (1ll << 29) || w_tiles > (1ll << 29))
+    return fail(WAVE_E_INVALID, "too many output tiles");
+  return WAVE_OK;
+}
+
+// ------------------------------------------------------------------ products
+enum class Product { kForward, kInputGrad, kWeightGrad };
+
+// One 16-bit operand as the tensor maps see it: `rows` x `cols` of each matrix,
+// cols contiguous.
+struct Operand {
+  const void *ptr;
+  long long ld, group;
+  int rows, cols, matrices;
+  bool packed() const { return ld % 8 != 0 || (matrices > 1 && group % 8 != 0); }
+  long long packed_ld() const { return round_up(cols, 8); }
+  size_t packed_bytes() const {
+    return packed() ? static_cast<size_t>(round_up(packed_ld() * 2 * rows * static_cast<long long>(matrices), 256)) : 0;
+  }
+};
+
+// Lays the operand out in `to` if its strides are not multiples of 16 bytes.
+int pack(Operand *o, char **to, cudaStream_t stream) {
+  if (!o->packed())
+    return WAVE_OK;
+  const long long ld = o->packed_ld(), group = ld * o->rows;
+  const size_t bytes = o->packed_bytes();
+  cudaError_t err =
+      wave::launch_pack_rows(o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices, stream);
+  if (err != cudaSuccess)
+    return cuda_fail(err, "linear: laying out an operand");
+  o->ptr = *to;
+  o->ld = ld;
+  o->group = group;
+  *to += bytes;
+  return WAVE_OK;
+}
+
+int operand_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_cols, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(o.cols), static_cast<uint64_t>(o.rows), static_cast<uint64_t>(o.matrices)};
+  const long long group = o.matrices > 1 ? o.group : o.ld * o.rows; // (read by nobody where there is one matrix)
+  const uint64_t strides[2] = {static_cast<uint64_t>(o.ld) * 2, static_cast<uint64_t>(group) * 2};
+  const uint32_t box[3] = {static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), 1};
+  return wave::make_tensor_map_16bit(map, is_bf16, o.ptr, 3, dims, strides, box);
+}
+
+// Tile choice of one product.  `tokens` rows over `matrices` experts (grouped)
+// or all with one matrix; P x Q and the contraction as in LinearParams.
+struct Plan {
+  LinearLaunch launch;
+  int tile_q, p_blocks, q_blocks, raster, splits;
+};
+
+int tile_for(int want) {
+  for (int t : {16, 32, 64, 128})
+    if (want <= t)
+      return t;
+  return 128;
+}
+
+Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
+  const wave::EnvKnobs env = wave::env_knobs();
+  const wave_linear_desc &d = s.d;
+  Plan pl{};
+  LinearLaunch &l = pl.launch;
+  l.a_mn = kind == Product::kWeightGrad;
+  l.b_mn = kind != Product::kForward;
+  l.out_f32 = out_f32;
+  const long long M = d.tokens;
+  const int N = d.out_features, K = d.in_features;
+  const long long per_expert = (M + s.matrices - 1) / s.matrices;
+  // Few tokens: the weights on the 128 rows of the tile, the tokens on its columns.
+  l.swap = kind == Product::kForward && per_expert <= (s.grouped ? 64 : 128);
+  if (env.linear_swap >= 0 && kind == Product::kForward)
+    l.swap = env.linear_swap;
+  long long p_ext, q_ext, k_ext;
+  if (kind == Product::kForward) {
+    p_ext = l.swap ? N : M;
+    q_ext = l.swap ? M : N;
+    k_ext = K;
+  } else if (kind == Product::kInputGrad) {
+    p_ext = M;
+    q_ext = K;
+    k_ext = N;
+  } else {
+    p_ext = N;
+    q_ext = K;
+    k_ext = s.grouped ? per_expert : M;
+  }
+  const long long k_iters = (k_ext + 63) / 64;
+  auto blocks = [&](int tile_q, long long *pb, long long *qb) -> long long {
+    *pb = (p_ext + 127) / 128;
+    *qb = (q_ext + tile_q - 1) / tile_q;
+    long long tiles;
+    if (kind == Product::kWeightGrad)
+      tiles = *pb * *qb * s.matrices;
+    else if (!s.grouped)
+      tiles = *pb * *qb;
+    else if (l.swap) // an upper bound: every expert may add a ragged block
+      tiles = *pb * (M / tile_q + (s.matrices < M ? s.matrices : M));
+    else
+      tiles = *qb * (M / 128 + (s.matrices < M ? s.matrices : M));
+    return tiles;
+  };
+  long long pb = 0, qb = 0, tiles = 0;
+  if (l.swap) {
+    const long long want = s.grouped ? 2 * per_expert : M;
+    l.tile_n = tile_for(static_cast<int>(want < 128 ? (want < M ? want : M) : 128));
+    if (env.linear_tile && env.linear_tile <= 128)
+      l.tile_n = env.linear_tile;
+    pl.tile_q = l.tile_n;
+    if (!s.grouped) // no columns of padding beyond the multiple of 16
+      pl.tile_q = static_cast<int>(round_up((M + (M + l.tile_n - 1) / l.tile_n - 1) / ((M + l.tile_n - 1) / l.tile_n), 16));
+    tiles = blocks(pl.tile_q, &pb, &qb);
+  } else {
+    l.tile_n = 64;
+    for (int t : {256, 128}) {
+      if (t == 256 && out_f32)
+        continue;
+      if (blocks(t, &pb, &qb) >= sms * (t == 256 ? 1 : 1) && q_ext > t / 2) {
+        l.tile_n = t;
+        break;
+      }
+    }
+    if (l.tile_n == 64 && q_ext > 64)
+      l.tile_n = 128;
+    if (env.linear_tile && env.linear_tile >= 64 && !(out_f32 && env.linear_tile == 256))
+      l.tile_n = env.linear_tile;
+    pl.tile_q = l.tile_n;
+    tiles = blocks(pl.tile_q, &pb, &qb);
+  }
+  // Few tiles: a cluster of CTAs shares a tile's contraction.
+  pl.splits = 1;
+  if (tiles > 0)
+    for (int c : {8, 4, 2})
+      if (tiles * c <= sms && k_iters / c >= 2 && (l.swap || pl.tile_q / 16 >= c)) {
+        pl.splits = c;
+        break;
+      }
+  if (env.linear_splits > 0 && tiles * env.linear_splits <= 65535)
+    pl.splits = env.linear_splits;
+  pl.p_blocks = static_cast<int>(pb);
+  pl.q_blocks = static_cast<int>(qb);
+  pl.raster = 16;
+  l.grid = static_cast<int>(pl.splits > 1 ? tiles * pl.splits : (tiles < sms ? tiles : sms));
+  if (l.grid < 1)
+    l.grid = 1;
+  return pl;
+}
+
+struct Outputs {
+  void *D;
+  long long ldd, group_d;
+  int elem; // bytes
+  void *Z;
+  const void *R, *bias;
+};
+
+int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operand &b_op, const int *offsets, const Outputs &o,
+                bool out_f32, int zero_rest, int sms, cudaStream_t stream) {
+  const wave_linear_desc &d = s.d;
+  const Plan pl = plan_product(kind, s, out_f32, sms);
+  const LinearLaunch &l = pl.launch;
+  LinearParams p{};
+  const int is_bf16 = d.io_type == WAVE_BF16;
+  // forward: (x, W) or, swapped, (W, x); input gradient: (dz, W); weight gradient: (dz, x)
+  const Operand &a = l.swap ? b_op : a_tok;
+  const Operand &b = l.swap ? a_tok : b_op;
+  const bool weights_a = l.swap, weights_b = kind != Product::kWeightGrad && !l.swap;
+  p.group_a = s.grouped && weights_a;
+  p.group_b = s.grouped && weights_b;
+  if (kind == Product::kForward) {
+    p.P = l.swap ? d.out_features : d.tokens;
+    p.Q = l.swap ? d.tokens : d.out_features;
+    p.K = d.in_features;
+  } else if (kind == Product::kInputGrad) {
+    p.P = d.tokens;
+    p.Q = d.in_features;
+    p.K = d.out_features;
+  } else {
+    p.P = d.out_features;
+    p.Q = d.in_features;
+    p.K = d.tokens;
+  }
+  p.ragged = !s.grouped ? wave::kRaggedNone : kind == Product::kWeightGrad ? wave::kRaggedK : wave::kRaggedRows;
+  p.groups = s.matrices;
+  p.offsets = s.grouped ? offsets : nullptr;
+  p.tile_q = pl.tile_q;
+  p.p_blocks = pl.p_blocks;
+  p.q_blocks = pl.q_blocks;
+  p.raster = pl.raster;
+  p.splits = pl.splits;
+  p.is_bf16 = is_bf16;
+  p.act = kind == Product::kForward ? d.activation : WAVE_ACT_NONE;
+  p.D = o.D;
+  p.ldd = o.ldd;
+  p.group_d = o.group_d;
+  p.Z = o.Z;
+  p.ldz = d.ldz;
+  p.R = o.R;
+  p.ldr = d.ldr;
+  p.bias = o.bias;
+  p.bias_f32 = d.bias_type == WAVE_F32;
+  p.group_bias = s.grouped ? d.out_features : 0;
+  p.vec_d = aligned16(o.D) && (o.ldd * o.elem) % 16 == 0 && (o.group_d * o.elem) % 16 == 0;
+  p.vec_z = aligned16(o.Z) && d.ldz % 8 == 0;
+  p.vec_r = aligned16(o.R) && d.ldr % 8 == 0;
+  p.zero_rest = zero_rest;
+  CUtensorMap ta, tb;
+  int rc = operand_map(&ta, a, is_bf16, 64, l.a_mn ? 64 : 128);
+  if (rc != WAVE_OK)
+    return rc;
+  rc = operand_map(&tb, b, is_bf16, 64, l.b_mn ? 64 : pl.tile_q);
+  if (rc != WAVE_OK)
+    return rc;
+  cudaError_t err = wave::launch_linear(ta, tb, p, l, stream);
+  return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear launch");
+}
+
+Operand tokens_by_in(const Shape &s, const void *ptr) {
+  return Operand{ptr, s.d.ldx, 0, s.d.tokens, s.d.in_features, 1};
+}
+Operand weights(const Shape &s, const void *ptr) {
+  return Operand{ptr, s.d.ldw, s.d.expert_stride_w, s.d.out_features, s.d.in_features, s.matrices};
+}
+
+// Rows of a chunk of the activation gradient: enough chunks for two blocks to an
+// SM where the rows allow it, long ones otherwise (fewer partial sums).
+int chunk_rows(const Shape &s, int sms) {
+  const long long col_blocks = (s.d.out_features + 255) / 256;
+  int rows = 128;
+  while (rows > 16 && (s.d.tokens / rows) * col_blocks < 2ll * sms)
+    rows /= 2;
+  while (s.d.tokens / rows + s.matrices > 32768)
+    rows *= 2;
+  return rows;
+}
+
+struct BackwardLayout {
+  bool make_dz;   // dz has to be written: an activation, an f32 dy, or rows that TMA cannot load
+  long long lddz;
+  int chunk;
+  size_t dz_bytes, partial_bytes, x_bytes, w_bytes;
+};
+BackwardLayout backward_layout(const Shape &s, int sms) {
+  BackwardLayout b{};
+  const wave_linear_desc &d = s.d;
+  b.make_dz = d.activation != WAVE_ACT_NONE || d.y_type == WAVE_F32 || d.ldy % 8 != 0;
+  b.lddz = round_up(d.out_features, 8);
+  b.chunk = chunk_rows(s, sms);
+  b.dz_bytes = b.make_dz ? static_cast<size_t>(round_up(b.lddz * 2 * d.tokens, 256)) : 0;
+  const long long chunks = wave::linear_act_grad_chunks(d.tokens, s.grouped ? s.matrices : 0, b.chunk);
+  b.partial_bytes = static_cast<size_t>(round_up(chunks * d.out_features * 4ll, 256));
+  b.x_bytes = tokens_by_in(s, nullptr).packed_bytes();
+  b.w_bytes = weights(s, nullptr).packed_bytes();
+  return b;
+}
+
+} // namespace
+
+extern "C" {
+
+void wave_cuda_linear_desc_init(wave_linear_desc *d, int tokens, int out_features, int in_features) {
+  memset(d, 0, sizeof *d);
+  d->tokens = tokens;
+  d->out_features = out_features;
+  d->in_features = in_features;
+  d->io_type = d->y_type = d->bias_type = d->dweight_type = WAVE_BF16;
+  d->dbias_type = WAVE_F32;
+}
+
+int wave_cuda_linear_validate(const wave_linear_desc *d) { return validate(d); }
+
+int wave_cuda_linear_workspace_bytes(const wave_linear_desc *d, int backward, size_t *bytes) {
+  int rc = validate(d);
+  if (rc != WAVE_OK)
+    return rc;
+  if (!bytes)
+    return fail(WAVE_E_INVALID, "the result pointer is null");
+  const Shape s = resolve(*d);
+  if (!backward) {
+    *bytes = tokens_by_in(s, nullptr).packed_bytes() + weights(s, nullptr).packed_bytes();
+    return WAVE_OK;
+  }
+  int sms = 0;
+  if ((rc = sm_count(&sms)) != WAVE_OK)
+    return rc;
+  const BackwardLayout b = backward_layout(s, sms);
+  *bytes = b.dz_bytes + b.partial_bytes + b.x_bytes + b.w_bytes;
+  return WAVE_OK;
+}
+
+int wave_cuda_linear_fwd(const wave_linear_desc *d, const void *X, const void *W, const void *bias, const void *residual,
+                         const int *offsets, void *Y, void *Z, void *workspace, void *stream) {
+  return guarded([&] {
+    int rc = validate(d);
+    if (rc != WAVE_OK)
+      return rc;
+    const Shape s = resolve(*d);
+    if (s.grouped && !offsets)
+      return fail(WAVE_E_INVALID, "grouped layers need the experts' offsets");
+    if (s.grouped && residual)
+      return fail(WAVE_E_UNSUPPORTED, "a residual goes with one weight matrix, not with experts");
+    if (d->tokens == 0)
+      return WAVE_OK;
+    if (!X || !W || !Y)
+      return fail(WAVE_E_INVALID, "X, W and Y must be non-null device pointers");
+    if (!aligned16(X) || !aligned16(W))
+      return fail(WAVE_E_INVALID, "X and W must be 16-byte aligned");
+    int sms = 0;
+    if ((rc = sm_count(&sms)) != WAVE_OK)
+      return rc;
+    Operand x = tokens_by_in(s, X), w = weights(s, W);
+    if (x.packed_bytes() + w.packed_bytes() > 0 && (!workspace || !aligned16(workspace)))
+      return fail(WAVE_E_INVALID, "rows of X or W that are no multiple of 16 bytes apart need a 16-byte aligned workspace of %zu bytes",
+                  x.packed_bytes() + w.packed_bytes());
+    char *ws = static_cast<char *>(workspace);
+    cudaStream_t q = static_cast<cudaStream_t>(stream);
+    if ((rc = pack(&x, &ws, q)) != WAVE_OK || (rc = pack(&w, &ws, q)) != WAVE_OK)
+      return rc;
+    const bool f32 = s.d.y_type == WAVE_F32;
+    const Outputs o{Y, s.d.ldy, 0, f32 ? 4 : 2, Z, residual, bias};
+    return run_product(Product::kForward, s, x, w, offsets, o, f32, d->zero_rest, sms, q);
+  });
+}
+
+int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *X, const void *W, const void *Z,
+                         const int *offsets, void *dX, void *dW, void *dbias, void *workspace, void *stream) {
+  return guarded([&] {
+    int rc = validate(d);
+    if (rc != WAVE_OK)
+      return rc;
+    const Shape s = resolve(*d);
+    if (s.grouped && !offsets)
+      return fail(WAVE_E_INVALID, "grouped layers need the experts' offsets");
+    if (d->tokens > 0) {
+      if (!dY || (dW && !X) || (dX && !W))
+        return fail(WAVE_E_INVALID, "dY, the X that dW needs and the W that dX needs must be non-null device pointers");
+      if (d->activation != WAVE_ACT_NONE && !Z)
+        return fail(WAVE_E_INVALID, "the gradient of an activation needs the pre-activation Z");
+      if (!aligned16(dY) || (dW && !aligned16(X)) || (dX && !aligned16(W)))
+        return fail(WAVE_E_INVALID, "dY, X and W must be 16-byte aligned");
+    }
+    int sms = 0;
+    if ((rc = sm_count(&sms)) != WAVE_OK)
+      return rc;
+    const BackwardLayout b = backward_layout(s, sms);
+    const size_t need = b.dz_bytes + b.partial_bytes + b.x_bytes + b.w_bytes;
+    if (need > 0 && (!workspace || !aligned16(workspace)))
+      return fail(WAVE_E_INVALID, "the backward pass needs a 16-byte aligned workspace of %zu bytes", need);
+    cudaStream_t q = static_cast<cudaStream_t>(stream);
+    char *ws = static_cast<char *>(workspace);
+    const int is_bf16 = d->io_type == WAVE_BF16;
+    Operand dz{dY, s.d.ldy, 0, s.d.tokens, s.d.out_features, 1};
+    const bool dz_wanted = b.make_dz && (dX || dW);
+    if (dz_wanted || dbias) {
+      wave::LinearActGrad g{};
+      g.rows = s.d.tokens;
+      g.cols = s.d.out_features;
+      g.groups = s.matrices;
+      g.offsets = s.grouped ? offsets : nullptr;
+      g.act = s.d.activation;
+      g.is_bf16 = is_bf16;
+      g.dy_f32 = s.d.y_type == WAVE_F32;
+      g.dY = dY;
+      g.ldy = s.d.ldy;
+      g.Z = s.d.activation != WAVE_ACT_NONE ? Z : nullptr;
+      g.ldz = s.d.ldz;
+      g.dZ = dz_wanted ? ws : nullptr;
+      g.lddz = b.lddz;
+      g.partial = dbias ? reinterpret_cast<float *>(ws + b.dz_bytes) : nullptr;
+      g.chunk_rows = b.chunk;
+      g.dbias = dbias;
+      g.dbias_type = s.d.dbias_type == WAVE_F32 ? 0 : is_bf16 ? 2 : 1;
+      g.vec_dy = aligned16(dY) && (s.d.ldy * (g.dy_f32 ? 4 : 2)) % 16 == 0;
+      g.vec_z = aligned16(g.Z) && s.d.ldz % 8 == 0;
+      cudaError_t err = wave::launch_act_grad(g, q);
+      if (err != cudaSuccess)
+        return cuda_fail(err, "linear: gradient of the activation");
+    }
+    if (b.make_dz) {
+      dz.ptr = ws;
+      dz.ld = b.lddz;
+    }
+    ws += b.dz_bytes + b.partial_bytes;
+    if (dX && s.d.tokens > 0) {
+      Operand w = weights(s, W);
+      if ((rc = pack(&w, &ws, q)) != WAVE_OK)
+        return rc;
+      const Outputs o{dX, s.d.lddx, 0, 2, nullptr, nullptr, nullptr};
+      if ((rc = run_product(Product::kInputGrad, s, dz, w, offsets, o, false, d->zero_rest, sms, q)) != WAVE_OK)
+        return rc;
+    }
+    if (dW) {
+      const bool f32 = s.d.dweight_type == WAVE_F32;
+      const Outputs o{dW, s.d.lddw, s.grouped ? s.d.expert_stride_dw : 0, f32 ? 4 : 2, nullptr, nullptr, nullptr};
+      if (s.d.tokens == 0) { // no rows: the sums are empty
+        cudaError_t err = cudaSuccess;
+        const size_t row = static_cast<size_t>(s.d.in_features) * o.elem;
+        for (int g = 0; g < s.matrices && err == cudaSuccess; ++g)
+          err = cudaMemset2DAsync(static_cast<char *>(dW) + static_cast<size_t>(g) * o.group_d * o.elem,
+                                  static_cast<size_t>(s.d.lddw) * o.elem, 0, row, static_cast<size_t>(s.d.out_features), q);
+        return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear: clearing the weight gradient");
+      }
+      Operand x = tokens_by_in(s, X);
+      if ((rc = pack(&x, &ws, q)) != WAVE_OK)
+        return rc;
+      return run_product(Product::kWeightGrad, s, dz, x, offsets, o, f32, 0, sms, q);
+    }
+    return WAVE_OK;
+  });
+}
+
+} // extern "C"

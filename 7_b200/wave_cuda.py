@@ -42,6 +42,13 @@ class FaDesc(C.Structure):
                 ("out_f32", C.c_int), ("qk_max_abs", C.c_float)]
 
 
+class LinearDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in (
+        "tokens", "out_features", "in_features", "experts", "io_type", "y_type", "bias_type", "dweight_type", "dbias_type",
+        "activation", "zero_rest", "reserved")] + [(n, C.c_longlong) for n in (
+            "ldx", "ldw", "ldy", "ldr", "ldz", "lddx", "lddw", "expert_stride_w", "expert_stride_dw")]
+
+
 EXPORTS = [
     "wave_cuda_last_error", "wave_cuda_version", "wave_cuda_reload_env",
     "_mlir_ciface_wave_memref_to_ptr_global_i32", "_mlir_ciface_wave_memref_to_ptr_global_i8",
@@ -52,7 +59,8 @@ EXPORTS = [
     "wave_cuda_gemm_host", "wave_cuda_gemm_host_a_resident", "wave_cuda_gemm_multi_output", "wave_cuda_gemm_multicast_output",
     "wave_cuda_gemm_plan", "wave_cuda_gemm_plan_for_sms", "wave_cuda_gemm_streamk_static", "wave_cuda_fa_validate", "wave_cuda_flash_attention_fwd",
     "wave_cuda_flash_attention_fwd_multi_output", "wave_cuda_flash_attention_fwd_multicast_output",
-    "wave_cuda_flash_attention_fwd_host", "wave_cuda_module_get_function", "wave_cuda_launch",
+    "wave_cuda_flash_attention_fwd_host", "wave_cuda_linear_desc_init", "wave_cuda_linear_validate",
+    "wave_cuda_linear_workspace_bytes", "wave_cuda_linear_fwd", "wave_cuda_linear_bwd", "wave_cuda_module_get_function", "wave_cuda_launch",
     "wave_cuda_function_release", "wave_cuda_check_device_status",
     # include/wave_mgpu.h: the wrappers a host module lowered by gpu-to-llvm calls
     "wave_cuda_module_blob_bytes", "wave_cuda_module_blob_write", "wave_cuda_mgpu_status", "wave_cuda_memref_region",
@@ -102,6 +110,12 @@ def lib() -> C.CDLL:
     L.wave_cuda_flash_attention_fwd_host.argtypes = [C.POINTER(FaDesc), vp, vp, vp, vp, vp]
     L.wave_cuda_flash_attention_fwd_multi_output.argtypes = [C.POINTER(FaDesc), vp, vp, vp, C.POINTER(vp), C.c_int, vp, vp]
     L.wave_cuda_flash_attention_fwd_multicast_output.argtypes = [C.POINTER(FaDesc), vp, vp, vp, vp, vp, vp, vp]
+    L.wave_cuda_linear_desc_init.argtypes = [C.POINTER(LinearDesc), C.c_int, C.c_int, C.c_int]
+    L.wave_cuda_linear_desc_init.restype = None
+    L.wave_cuda_linear_validate.argtypes = [C.POINTER(LinearDesc)]
+    L.wave_cuda_linear_workspace_bytes.argtypes = [C.POINTER(LinearDesc), C.c_int, C.POINTER(C.c_size_t)]
+    L.wave_cuda_linear_fwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 9
+    L.wave_cuda_linear_bwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 10
     L.wave_cuda_module_get_function.argtypes = [C.c_char_p, vp, C.POINTER(vp)]
     L.wave_cuda_launch.argtypes = [vp, C.POINTER(vp), vp]
     L.wave_cuda_function_release.argtypes = [vp]
@@ -259,6 +273,16 @@ def flash_attention_fwd_multicast_output(desc: FaDesc, q_ptr: int, k_ptr: int, v
 
 def flash_attention_fwd_host(desc: FaDesc, q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, stream: int = 0) -> None:
     check(lib().wave_cuda_flash_attention_fwd_host(C.byref(desc), q_ptr, k_ptr, v_ptr, o_ptr, stream or None))
+
+
+def linear_validate(desc: LinearDesc) -> None:
+    check(lib().wave_cuda_linear_validate(C.byref(desc)))
+
+
+def linear_workspace_bytes(desc: LinearDesc, backward: bool) -> int:
+    n = C.c_size_t(0)
+    check(lib().wave_cuda_linear_workspace_bytes(C.byref(desc), int(backward), C.byref(n)))
+    return n.value
 
 
 def check_device_status() -> None:

@@ -288,6 +288,75 @@ int wave_cuda_flash_attention_fwd_multicast_output(const wave_fa_desc *desc, con
 int wave_cuda_flash_attention_fwd_host(const wave_fa_desc *desc, const void *Q_host, const void *K_host,
                                        const void *V_host, void *O_host, void *stream);
 
+/* ---- linear layers ------------------------------------------------------- *
+ * No counterpart in the reference, whose GEMM ends at its accumulator.  The
+ * layers of a transformer around the attention above, with everything that
+ * follows the product in its epilogue, and their backward pass:
+ *   z = x W^T + b             x [tokens][in], W [out][in] (as the GEMM's B), b [out] or NULL
+ *   y = act(z) + r            r [tokens][out] or NULL
+ *   dz = dy * act'(z);  dx = dz W;  dW = dz^T x;  db = sum of dz over the tokens  (r's gradient is dy)
+ * With experts > 0 there are that many weight matrices and biases, rows of x
+ * and y are sorted by expert, and offsets[experts + 1] (int32, on the device;
+ * nothing is copied to the host) says where each expert's rows begin and end.
+ * Offsets are cut to [0, tokens] and read with a running maximum, so that bad
+ * ones give empty experts.  An expert without rows reads nothing and has
+ * dW = 0, db = 0.  Rows in front of the first and behind the last expert's are
+ * left as they are in y, z and dx, or set to zero with `zero_rest`; what x, dy and
+ * z hold there is never used.
+ *
+ * Any sizes from one token and one feature on; tokens = 0 writes nothing but
+ * zero gradients.  Products accumulate in f32; z is rounded to io_type only
+ * where it is stored (act is taken of the unrounded value), y once; f32 results
+ * are summed in pieces of 512 products, rounded to nearest.  dz is rounded to
+ * io_type on its way into the two products (they are 16-bit matrix products),
+ * db is summed in f32 from the unrounded one.  Sums are in fixed order: the same
+ * call gives the same bits.  relu keeps a NaN and has slope 0 at 0.
+ * y may be r itself (in place); otherwise outputs overlap nothing.
+ *
+ * Rows may be any stride apart.  x, W and dy must be 16-byte aligned; where
+ * their rows (or matrices) are not a multiple of 8 elements apart the call first
+ * lays them out in the workspace.  Every other buffer needs its elements'
+ * alignment only.  A workspace is used by one call at a time, nothing in it
+ * needs clearing, and nothing is kept in it between calls.
+ * WAVE_CUDA_LINEAR_TILE=<columns>, WAVE_CUDA_LINEAR_SPLITS=<CTAs to a tile> and
+ * WAVE_CUDA_LINEAR_SWAP=0|1 override the choice of tiles (measurement knobs;
+ * sums are then taken in another order).                                     */
+#define WAVE_ACT_NONE 0
+#define WAVE_ACT_RELU 1
+#define WAVE_ACT_GELU 2      /* x Phi(x), with erf */
+#define WAVE_ACT_GELU_TANH 3 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+#define WAVE_ACT_SILU 4      /* x / (1 + e^-x) */
+
+typedef struct wave_linear_desc {
+  int tokens, out_features, in_features;
+  int experts;      /* 0: one weight matrix; else 1 .. 1024 */
+  int io_type;      /* WAVE_BF16 | WAVE_F16: x, W, r, z, dx */
+  int y_type;       /* io_type | WAVE_F32: y and dy */
+  int bias_type;    /* io_type | WAVE_F32 */
+  int dweight_type; /* io_type | WAVE_F32 */
+  int dbias_type;   /* io_type | WAVE_F32 */
+  int activation;   /* WAVE_ACT_* */
+  int zero_rest;    /* experts: non-zero sets the rows that belong to none to zero (y, z, dx) */
+  int reserved;     /* 0 */
+  long long ldx, ldw, ldy, ldr, ldz, lddx, lddw; /* elements from row to row of x, W, y / dy, r, z, dx, dW; 0 = rows without gaps */
+  long long expert_stride_w, expert_stride_dw;   /* elements from matrix to matrix; 0 = without gaps */
+} wave_linear_desc;
+
+/* bf16 everywhere (dbias f32), one weight matrix, no activation, no gaps. */
+void wave_cuda_linear_desc_init(wave_linear_desc *desc, int tokens, int out_features, int in_features);
+int wave_cuda_linear_validate(const wave_linear_desc *desc); /* needs no GPU */
+/* Device workspace of a call (16-byte aligned; may be NULL when 0).  The forward
+ * pass needs one only for operands that have to be laid out. */
+int wave_cuda_linear_workspace_bytes(const wave_linear_desc *desc, int backward, size_t *bytes);
+/* bias, residual and Z (the pre-activation, io_type) may be NULL; offsets is
+ * read only with experts; experts take no residual. */
+int wave_cuda_linear_fwd(const wave_linear_desc *desc, const void *X, const void *W, const void *bias,
+                         const void *residual, const int *offsets, void *Y, void *Z, void *workspace, void *stream);
+/* Any of dX, dW and dbias may be NULL: it is not computed, and what only it needs
+ * (W for dX, X for dW) may be NULL too.  Z may be NULL without an activation. */
+int wave_cuda_linear_bwd(const wave_linear_desc *desc, const void *dY, const void *X, const void *W, const void *Z,
+                         const int *offsets, void *dX, void *dW, void *dbias, void *workspace, void *stream);
+
 /* ---- name-based launch facade ------------------------------------------ *
  * Keeps the runners' call shape (hipModuleGetFunction by kernel name, then a
  * launch with a void* args[] block of pointers-to-values): names
