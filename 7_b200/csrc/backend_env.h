@@ -22,6 +22,8 @@ struct EnvKnobs {
   int linear_tile = 0;           // WAVE_CUDA_LINEAR_TILE: columns of a linear layer's tile (16, 32, 64, 128, 256), 0 = chosen
   int linear_splits = 0;         // WAVE_CUDA_LINEAR_SPLITS: CTAs that share a tile's contraction (1..8), 0 = chosen
   int linear_swap = -1;          // WAVE_CUDA_LINEAR_SWAP: 1 tokens on the tile's columns, 0 on its rows, -1 = chosen
+  int linear_pair = -1;          // WAVE_CUDA_LINEAR_PAIR: 1 CTA pairs wherever they can, 0 never, -1 = chosen
+  bool linear_pdl = true;        // WAVE_CUDA_LINEAR_PDL=0: linear layers' launches without programmatic dependent launch
 };
 
 EnvKnobs env_knobs();

@@ -10,7 +10,7 @@ using namespace linear_detail;
 
 // PDL as in the product kernels: set-up may overlap the kernel before this one.
 template <typename Kernel, typename... Args>
-cudaError_t launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, Kernel kernel, const Args &...args) {
+cudaError_t launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, int pdl, Kernel kernel, const Args &...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -20,7 +20,7 @@ cudaError_t launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, Ker
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -97,6 +97,10 @@ __device__ __forceinline__ void load_eight(Eight &out, const void *base, long lo
 // One chunk of rows x 256 columns to a block.  A chunk never crosses a group's
 // end, so its column sums go to one group; which rows chunk `blockIdx.y` has
 // comes from the offsets, on the device.
+// kAct < 0: dz = dy (column sums alone, or a copy in another layout or type).
+// The activation is a template argument: chosen for each value at run time it
+// costs more than the arithmetic (8192 x 8192 bf16, gelu_tanh: 243 us).
+template <int kAct>
 __global__ void __launch_bounds__(kAgThreads)
 act_grad_kernel(const __grid_constant__ LinearActGrad p) {
   extern __shared__ int ag_smem[];
@@ -139,7 +143,7 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
         const int row = r + u * kAgLanes;
         if (row < r1) {
           load_eight(g[u], p.dY, static_cast<long long>(row) * p.ldy + col, live, p.dy_f32 != 0, p.vec_dy != 0, p.is_bf16);
-          if (p.Z)
+          if constexpr (kAct >= 0)
             load_eight(z[u], p.Z, static_cast<long long>(row) * p.ldz + col, live, false, p.vec_z != 0, p.is_bf16);
         }
       }
@@ -148,10 +152,10 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
         const int row = r + u * kAgLanes;
         if (row >= r1)
           break;
-        if (p.Z) {
+        if constexpr (kAct >= 0) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            g[u].v[e] *= act_slope(z[u].v[e], p.act);
+            g[u].v[e] *= act_slope(z[u].v[e], kAct);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -225,14 +229,14 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 } // namespace
 
 cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
-                             long long group_dst, int rows, int cols, int groups, cudaStream_t stream) {
+                             long long group_dst, int rows, int cols, int groups, int pdl, cudaStream_t stream) {
   const int pieces = (cols + 7) / 8;
   const long long blocks = (static_cast<long long>(rows) * pieces + 255) / 256;
   if (blocks == 0 || groups == 0)
     return cudaSuccess;
   // enough blocks to fill the machine; the rest in the kernel's loop
   const unsigned grid = static_cast<unsigned>(blocks < 4096 ? blocks : 4096);
-  return launch(dim3(grid, static_cast<unsigned>(groups)), 256, 0, stream, pack_rows_kernel,
+  return launch(dim3(grid, static_cast<unsigned>(groups)), 256, 0, stream, pdl, pack_rows_kernel,
                 static_cast<const uint16_t *>(src), ld_src, group_src, static_cast<uint16_t *>(dst), ld_dst, group_dst, rows,
                 cols, pieces);
 }
@@ -246,13 +250,21 @@ cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
   const int chunks = linear_act_grad_chunks(p.rows, p.offsets ? p.groups : 0, p.chunk_rows);
   const size_t table = p.offsets ? 2 * sizeof(int) * (static_cast<size_t>(p.groups) + 1) : 0;
   cudaError_t err = cudaSuccess;
-  if (chunks > 0)
-    err = launch(dim3(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks)), kAgThreads,
-                 table, stream, act_grad_kernel, p);
+  if (chunks > 0) {
+    const dim3 grid(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks));
+    auto go = [&](auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); };
+    switch (p.Z ? p.act : kActNone) {
+    case kActRelu: go(act_grad_kernel<kActRelu>); break;
+    case kActGelu: go(act_grad_kernel<kActGelu>); break;
+    case kActGeluTanh: go(act_grad_kernel<kActGeluTanh>); break;
+    case kActSilu: go(act_grad_kernel<kActSilu>); break;
+    default: go(act_grad_kernel<-1>); break;
+    }
+  }
   if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
     return err;
   return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(p.offsets ? p.groups : 1)), 256, table,
-                stream, column_sum_kernel, p);
+                stream, p.pdl, column_sum_kernel, p);
 }
 
 } // namespace wave

@@ -1,0 +1,428 @@
+// Products of the linear layers on CTA pairs, for problems with many tiles: two
+// CTAs of a cluster compute one 256 x (up to 256) tile with tcgen05.mma
+// cta_group::2.  Each loads its own 128 rows of A and its own half of the tile's
+// B (no multicast) and receives its 128 accumulator rows in its own tensor
+// memory, so a step of 64 moves 32 KB to a CTA where the one-CTA kernel moves 48
+// for the same outputs: a deeper ring and a third less shared-memory traffic.
+// Operand layouts, experts and the epilogue are those of linear_sm100.cu.
+//
+// Barriers across the pair:
+//   full[s]    in the leader, armed by its loader with the bytes of both CTAs'
+//              loads (an arrival of the other CTA's loader for each stage was
+//              tried: a remote arrival with release costs that thread so long that
+//              8192^3 took 1500 us)
+//   landed[s]  one per CTA: the last stage of an expert's weight gradient lands
+//              here, and the CTA's own warp 1 zeroes the rows behind the expert's
+//              last (several such stages may be in the ring, so each has a barrier)
+//   cut[s]     in the leader: the other CTA has done so; the leader then completes
+//              full[s] itself
+//   empty[s], tfull[a]  one per CTA; the leader's tcgen05.commit arrives on both
+//   tempty[a]  in the leader; the epilogue warps of both CTAs arrive
+#include "launch_cache.h"
+#include "linear_common.cuh"
+
+namespace wave {
+
+__device__ int g_linear_pair_status[4]; // [0] code, [1] linear block, [2] role, [3] detail
+
+namespace {
+
+using namespace linear_detail;
+
+constexpr int kRows = 128; // rows of A, and of the accumulator, in each CTA
+constexpr int kPairP = 256;
+constexpr int kTN = 256;
+constexpr int kBK = 64;
+constexpr int kChunkBytes = 64 * 128;
+constexpr int kABytes = kRows * kBK * 2;
+constexpr int kBBytes = kTN / 2 * kBK * 2;
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kMyCols = kTN / 2; // columns of an epilogue warp
+constexpr int kW = 32;
+constexpr int kSlots = kEpiWarps * slot_bytes<false>();
+constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
+constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots;
+static_assert(kSmemFixed + kTableBytes <= 227 * 1024, "does not fit the shared memory of an SM");
+
+struct PairShared {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t landed[kStages];
+  uint64_t cut[kStages];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __noinline__ void pair_report(int code, int role, int detail) {
+  if (atomicCAS(&g_linear_pair_status[0], 0, code) == 0) {
+    g_linear_pair_status[1] = static_cast<int>(blockIdx.x);
+    g_linear_pair_status[2] = role;
+    g_linear_pair_status[3] = detail;
+  }
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+               " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar) & kPeerBitMask), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
+// Orders what this thread does next behind what the other CTA's threads wrote
+// before they arrived on a barrier that this thread has seen complete.
+__device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+template <bool kAMn, bool kBMn>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                   const __grid_constant__ LinearParams p) {
+  constexpr bool kCut = kAMn && kBMn;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  PairShared *sh = reinterpret_cast<PairShared *>(tiles + kStages * kStageBytes);
+  uint8_t *slots = tiles + kStages * kStageBytes + 1024;
+  GroupTable table;
+  table.begin = reinterpret_cast<int *>(slots + kSlots);
+  table.blocks = table.begin + p.groups + 1;
+  volatile int *abort_flag = &sh->abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int first_tile = static_cast<int>(blockIdx.x >> 1), tile_step = static_cast<int>(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+      mbar_init(&sh->landed[s], 1);
+      mbar_init(&sh->cut[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&sh->tfull[a], 1);
+      mbar_init(&sh->tempty[a], 2 * kEpiWarps);
+    }
+    sh->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&sh->tmem_base, 2 * kTN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_arrive(); // the peer's barriers must be there before anything signals them
+  cluster_wait();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = sh->tmem_base;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.ragged != kRaggedNone)
+    build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : p.P, kPairP);
+
+  // Contraction indices of stage kb, and whether rows behind them have to be cut away.
+  auto live_of = [](const Tile &w, int kb) { return min(kBK, w.k_len - kb * kBK); };
+  auto is_cut = [&](int live) { return kCut && p.ragged == kRaggedK && live < kBK; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- loads
+    if (lane == 0) {
+      TileWalk<false> walk(p, table, kPairP);
+      Tile w;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const int half_q = p.tile_q / 2;
+      const uint32_t tx = kABytes + static_cast<uint32_t>(half_q) * kBK * 2; // one CTA's bytes
+      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+        const int kbs = (w.k_len + kBK - 1) / kBK;
+        const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
+        const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * half_q;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag)) {
+            pair_report(kStatusWaitTimeout, 0, stage);
+            ok = false;
+            break;
+          }
+          uint8_t *a_dst = tiles + stage * kStageBytes;
+          uint8_t *b_dst = a_dst + kABytes;
+          const int k = w.k_begin + kb * kBK;
+          if (is_cut(live_of(w, kb))) {
+            // this CTA's bytes on its own barrier: warp 1 cuts them
+            uint64_t *bar = &sh->landed[stage];
+            mbar_arrive_expect_tx(bar, tx);
+            for (int c = 0; c < kRows / 64; ++c)
+              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+            for (int c = 0; c < half_q / 64; ++c)
+              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
+          } else {
+            uint64_t *bar = &sh->full[stage];
+            if (leader)
+              mbar_arrive_expect_tx(bar, 2 * tx);
+            if constexpr (kAMn) {
+              for (int c = 0; c < kRows / 64; ++c)
+                tma_load_3d_pair(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+            } else {
+              tma_load_3d_pair(a_dst, &tm_a, bar, k, pa, za);
+            }
+            if constexpr (kBMn) {
+              for (int c = 0; c < half_q / 64; ++c)
+                tma_load_3d_pair(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
+            } else {
+              tma_load_3d_pair(b_dst, &tm_b, bar, k, qb, zb);
+            }
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok)
+        bounded_delay(1 << 21);
+    }
+  } else if (warp == 1) {
+    // ---------------------- UMMA issue (leader), cutting of last stages (both)
+    // The loop over whole stages is kept as bare as in linear_sm100.cu.
+    if (kCut || (leader && lane == 0)) {
+      const uint32_t idesc = umma_idesc_f16(kPairP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
+      constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
+      constexpr uint64_t kStep = kStageBytes >> 4;
+      const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
+      const uint64_t da0 = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
+      const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
+      TileWalk<false> walk(p, table, kPairP);
+      Tile w;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0, cut_phases = 0; // of landed and cut: a bit to a stage
+      bool ok = true;
+      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+        const int kbs = (w.k_len + kBK - 1) / kBK;
+        if (kbs <= 0)
+          continue;
+        const int live = live_of(w, kbs - 1);
+        const bool cut = is_cut(live);
+        const int whole = kbs - (cut ? 1 : 0);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTN);
+        uint32_t more = 0; // the accumulator holds something
+        if (leader && lane == 0) {
+          ok = mbar_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag);
+          if (!ok)
+            pair_report(kStatusWaitTimeout, 1, 100 + acc);
+          tc_fence_after_sync();
+          int st = stage;
+          uint32_t ph = phase;
+          for (int i = 0; ok && i < whole; ++i) {
+            if (!mbar_wait(&sh->full[st], ph, abort_flag)) {
+              pair_report(kStatusWaitTimeout, 1, st);
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint64_t da = da0 + static_cast<uint64_t>(st) * kStep, db = db0 + static_cast<uint64_t>(st) * kStep;
+            umma_ss_pair(d, da, db, idesc, more);
+#pragma unroll
+            for (int k = 1; k < kBK / 16; ++k)
+              umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+            more = 1;
+            umma_commit_pair(&sh->empty[st], 3); // frees the stage in both CTAs
+            if (++st == kStages) {
+              st = 0;
+              ph ^= 1;
+            }
+          }
+        }
+        {
+          const int at = stage + whole; // every lane, in both CTAs, keeps count
+          phase ^= static_cast<uint32_t>(at / kStages) & 1u;
+          stage = at % kStages;
+        }
+        if constexpr (kCut) {
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (ok && cut) {
+            const uint32_t parity = (cut_phases >> stage) & 1u;
+            cut_phases ^= 1u << stage;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh->landed[stage], parity, abort_flag)) != 0;
+            if (!ok) {
+              pair_report(kStatusWaitTimeout, 1, 50 + stage);
+              break;
+            }
+            uint8_t *a_tile = tiles + stage * kStageBytes;
+            const int steps = (live + 15) / 16;
+            const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
+            const int chunks = kRows / 64 + p.tile_q / 128;
+            for (int i = lane; i < chunks * vecs; i += 32) {
+              uint8_t *dst = a_tile + (i / vecs) * kChunkBytes + live * 128 + (i % vecs) * 16;
+              *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (leader) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&sh->cut[stage], parity, abort_flag)) != 0;
+              if (!ok) {
+                pair_report(kStatusWaitTimeout, 1, 70 + stage);
+                break;
+              }
+              fence_acquire_cluster();
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&sh->full[stage]); // the stage's turn of this barrier
+                tc_fence_after_sync();
+                const uint64_t da = da0 + static_cast<uint64_t>(stage) * kStep, db = db0 + static_cast<uint64_t>(stage) * kStep;
+                for (int k = 0; k < steps; ++k, more = 1)
+                  umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, more);
+                umma_commit_pair(&sh->empty[stage], 3);
+              }
+            } else if (lane == 0) {
+              mbar_arrive_cluster(map_to_cta(&sh->cut[stage], 0));
+            }
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        if (ok && leader && lane == 0)
+          umma_commit_pair(&sh->tfull[acc], 3);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue
+    const int quarter = warp & 3;
+    const int col0 = ((warp - 2) >> 2) * kMyCols;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint8_t *slot = slots + (warp - 2) * slot_bytes<false>();
+    const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
+    TileWalk<false> walk(p, table, kPairP);
+    Tile w;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int id = first_tile; walk.get(id, w); id += tile_step) {
+      const bool empty = w.k_len <= 0; // nothing to multiply: the epilogue of zero
+      EpiTile t;
+      t.group = w.group;
+      t.lane0 = w.p0 + rank * kRows + quarter * 32;
+      t.lane_end = w.p_end;
+      t.q_end = min(w.q_end, w.q0 + p.tile_q);
+      const int my_cols = min(kMyCols, p.tile_q - col0);
+      uint4 res[kW / 8];
+      if (p.R && my_cols > 0)
+        fetch_residual<kW>(res, p, t, w.q0 + col0, lane);
+      if (!empty) {
+        if (!mbar_wait(&sh->tfull[acc], acc_phase, abort_flag)) {
+          if (lane == 0)
+            pair_report(kStatusWaitTimeout, 2, 200 + acc);
+          break;
+        }
+        tc_fence_after_sync();
+      }
+#pragma unroll 1
+      for (int c = 0; c < my_cols; c += kW) {
+        float v[kW];
+        if (empty) {
+#pragma unroll
+          for (int j = 0; j < kW; ++j)
+            v[j] = 0.0f;
+        } else {
+          uint32_t r[kW];
+          tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTN + col0 + c), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < kW; ++j)
+            v[j] = __uint_as_float(r[j]);
+        }
+        uint4 now[kW / 8];
+#pragma unroll
+        for (int j = 0; j < kW / 8; ++j)
+          now[j] = res[j];
+        if (p.R && c + kW < my_cols)
+          fetch_residual<kW>(res, p, t, w.q0 + col0 + c + kW, lane);
+        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, now, slot, lane);
+      }
+      if (!empty) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive_cluster(tempty_leader[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+    }
+    if (p.zero_rest && p.ragged == kRaggedRows) {
+      const int wid = static_cast<int>(blockIdx.x) * kEpiWarps + warp - 2, warps = static_cast<int>(gridDim.x) * kEpiWarps;
+      zero_rows(p.D, 2, p.ldd, 0, table.begin[0], p.Q, wid, warps, lane);
+      zero_rows(p.D, 2, p.ldd, table.begin[p.groups], p.P, p.Q, wid, warps, lane);
+      if (p.Z) {
+        zero_rows(p.Z, 2, p.ldz, 0, table.begin[0], p.Q, wid, warps, lane);
+        zero_rows(p.Z, 2, p.ldz, table.begin[p.groups], p.P, p.Q, wid, warps, lane);
+      }
+    }
+  }
+
+  // Neither CTA may leave, or free tensor memory, while its partner can still
+  // read its shared memory, signal its barriers or write its accumulator.
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 2 * kTN);
+  }
+}
+
+template <bool kAMn, bool kBMn>
+cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                       cudaStream_t stream) {
+  auto kernel = linear_pair_kernel<kAMn, kBMn>;
+  cudaError_t err = prepare_kernel(kernel, kSmemFixed + kTableBytes, nullptr);
+  if (err != cudaSuccess)
+    return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(kSmemFixed) + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = l.pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+}
+
+} // namespace
+
+cudaError_t launch_linear_pair(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                               cudaStream_t stream) {
+  if (!l.a_mn)
+    return l.b_mn ? launch_one<false, true>(ta, tb, p, l, stream) : launch_one<false, false>(ta, tb, p, l, stream);
+  return l.b_mn ? launch_one<true, true>(ta, tb, p, l, stream) : cudaErrorInvalidValue;
+}
+
+cudaError_t linear_pair_read_status(int out[4], bool clear) {
+  cudaError_t err = cudaMemcpyFromSymbol(out, g_linear_pair_status, sizeof(int) * 4);
+  if (err == cudaSuccess && clear) {
+    int zero[4] = {0, 0, 0, 0};
+    err = cudaMemcpyToSymbol(g_linear_pair_status, zero, sizeof(zero));
+  }
+  return err;
+}
+
+} // namespace wave

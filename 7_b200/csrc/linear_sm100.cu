@@ -67,9 +67,9 @@ template <int TN, bool kF32> struct Cfg {
   static constexpr int kFit = (kSmemLimit - 1024 - 1024 - kTableBytes - kSlots) / kStageBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr int kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
-  static constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots; // + the group table
+  static constexpr int kSmemFixed = 1024 + 1024 + kSlots; // + the stages, the group table
   static_assert(kStages >= 4, "ring too short");
-  static_assert(TN * kTileP * 4 <= kStages * kStageBytes, "a partial tile must fit the ring");
+  static_assert(TN * kTileP * 4 <= 4 * kStageBytes, "a partial tile must fit the shortest ring");
 };
 
 __device__ __noinline__ void report(int code, int role, int detail) {
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(Cfg<TN, kF32>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ LinearParams p) {
   using C = Cfg<TN, kF32>;
-  constexpr int kStages = C::kStages;
+  const int num_stages = p.stages;
   constexpr bool kCut = kAMn && kBMn; // the weight gradient: stages may have to be cut at the last row
   constexpr int kColGroups = C::kEpiWarps / 4;
   constexpr int kMyCols = TN / kColGroups; // columns of an epilogue warp
@@ -113,8 +113,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Shared *sh = reinterpret_cast<Shared *>(tiles + kStages * C::kStageBytes);
-  uint8_t *slots = tiles + kStages * C::kStageBytes + 1024;
+  Shared *sh = reinterpret_cast<Shared *>(tiles + num_stages * C::kStageBytes);
+  uint8_t *slots = tiles + num_stages * C::kStageBytes + 1024;
   GroupTable table;
   table.begin = reinterpret_cast<int *>(slots + C::kSlots);
   table.blocks = table.begin + p.groups + 1;
@@ -128,7 +128,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const int tile_step = splits > 1 ? 0x3FFFFFFF : static_cast<int>(gridDim.x); // a cluster has one tile
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+    for (int s = 0; s < num_stages; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
     }
@@ -155,6 +157,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : (kSwap ? p.Q : p.P),
                       kSwap ? p.tile_q : kTileP);
 
+  float col_bias = 0.0f; // tokens as columns: the bias of the lane's feature, fetched while the tile accumulates
+
   // This CTA's share of a tile's stages.
   auto k_blocks = [&](const Tile &w, int &kb0, int &kb1) {
     const int total = (w.k_len + kBK - 1) / kBK;
@@ -165,8 +169,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
     if (lane == 0) {
-      tma_prefetch_desc(&tm_a);
-      tma_prefetch_desc(&tm_b);
       TileWalk<kSwap> walk(p, table, kTileP);
       Tile w;
       int stage = 0;
@@ -200,7 +202,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           } else {
             tma_load_3d(b_dst, &tm_b, bar, k, w.q0, zb);
           }
-          if (++stage == kStages) {
+          if (++stage == num_stages) {
             stage = 0;
             phase ^= 1;
           }
@@ -211,45 +213,78 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
   } else if (warp == 1) {
     // -------------------------------------------------------- UMMA issue
+    // One thread issues; the loop over whole stages holds nothing but a wait, four
+    // products and a commit (descriptors are one addition away from those of stage
+    // 0: built anew for each stage, with the number of steps looked at, 8192^3 took
+    // 14 % longer).  The weight gradient's warp stays together for the last stage
+    // of an expert, which all its lanes cut.
     if (kCut || lane == 0) {
       const uint32_t idesc = umma_idesc_f16(kTileP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
-      constexpr uint32_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
+      constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
+      constexpr uint64_t kStep = C::kStageBytes >> 4;
+      const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
+      const uint64_t da0 = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
+      const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
       TileWalk<kSwap> walk(p, table, kTileP);
       Tile w;
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      // (a warp that works together gives up together)
-      auto wait = [&](uint64_t *bar, uint32_t parity) {
-        const bool got = mbar_wait(bar, parity, abort_flag);
-        if constexpr (kCut)
-          return __all_sync(0xffffffffu, got) != 0;
-        return got;
-      };
       for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
         int kb0, kb1;
         k_blocks(w, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const bool first = kF32 ? (kb - kb0) % kSegment == 0 : kb == kb0;
-          const bool last = kb + 1 == kb1 || (kF32 && (kb - kb0) % kSegment == kSegment - 1);
-          if (first) {
-            ok = wait(&sh->tempty[acc], acc_phase ^ 1);
-            if (!ok) {
+        // the stage with an expert's last rows, if it is one of this CTA's
+        const int live = w.k_len & (kBK - 1);
+        const bool cut = kCut && p.ragged == kRaggedK && live != 0 && kb1 > kb0 && kb1 * kBK > w.k_len;
+        for (int kb = kb0; ok && kb < kb1;) {
+          const int end = kF32 ? min(kb + kSegment, kb1) : kb1;
+          const bool cut_here = cut && end == kb1;
+          const int whole = end - kb - (cut_here ? 1 : 0);
+          const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TN);
+          uint32_t more = 0; // the accumulator holds something
+          if (lane == 0) {
+            ok = mbar_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag);
+            if (!ok)
               report(kStatusWaitTimeout, 1, 100 + acc);
-              break;
+            tc_fence_after_sync();
+            int st = stage;
+            uint32_t ph = phase;
+            for (int i = 0; ok && i < whole; ++i) {
+              if (!mbar_wait(&sh->full[st], ph, abort_flag)) {
+                report(kStatusWaitTimeout, 1, st);
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+              const uint64_t da = da0 + static_cast<uint64_t>(st) * kStep, db = db0 + static_cast<uint64_t>(st) * kStep;
+              umma_ss(d, da, db, idesc, more);
+#pragma unroll
+              for (int k = 1; k < kBK / 16; ++k)
+                umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+              more = 1;
+              umma_commit(&sh->empty[st]);
+              if (++st == num_stages) {
+                st = 0;
+                ph ^= 1;
+              }
             }
           }
-          ok = wait(&sh->full[stage], phase);
-          if (!ok) {
-            report(kStatusWaitTimeout, 1, stage);
-            break;
+          {
+            const int at = stage + whole; // every lane keeps count
+            phase ^= static_cast<uint32_t>(at / num_stages) & 1u;
+            stage = at % num_stages;
           }
-          uint8_t *a_tile = tiles + stage * C::kStageBytes;
-          const int live = min(kBK, w.k_len - kb * kBK); // contraction indices of this stage
-          const int steps = (live + 15) / 16;
           if constexpr (kCut) {
-            if (p.ragged == kRaggedK && live < steps * 16) {
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (ok && cut_here) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag)) != 0;
+              if (!ok) {
+                report(kStatusWaitTimeout, 1, stage);
+                break;
+              }
               // rows [live, steps * 16) belong to the next expert or to nobody
+              uint8_t *a_tile = tiles + stage * C::kStageBytes;
+              const int steps = (live + 15) / 16;
               const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
               const int chunks = kTileP / 64 + p.tile_q / 64;
               for (int i = lane; i < chunks * vecs; i += 32) {
@@ -257,32 +292,27 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
               }
               fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tc_fence_after_sync();
+                const uint64_t da = da0 + static_cast<uint64_t>(stage) * kStep, db = db0 + static_cast<uint64_t>(stage) * kStep;
+                for (int k = 0; k < steps; ++k, more = 1)
+                  umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, more);
+                umma_commit(&sh->empty[stage]);
+              }
+              if (++stage == num_stages) {
+                stage = 0;
+                phase ^= 1;
+              }
             }
-            __syncwarp();
           }
-          tc_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t a_addr = smem_u32(a_tile), b_addr = a_addr + kABytes;
-            const uint64_t da = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
-            const uint64_t db = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
-            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TN);
-#pragma unroll
-            for (int k = 0; k < kBK / 16; ++k)
-              if (k < steps)
-                umma_ss(d, da + static_cast<uint64_t>(k * kStepA), db + static_cast<uint64_t>(k * kStepB), idesc,
-                        (!first || k > 0) ? 1u : 0u);
-            umma_commit(&sh->empty[stage]);
-            if (last)
-              umma_commit(&sh->tfull[acc]);
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (last && ++acc == 2) {
+          if (ok && lane == 0)
+            umma_commit(&sh->tfull[acc]);
+          if (++acc == 2) {
             acc = 0;
             acc_phase ^= 1;
           }
+          kb = end;
         }
       }
     }
@@ -324,7 +354,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       t.lane0 = w.p0 + quarter * 32;
       t.lane_end = w.p_end;
       t.q_end = min(w.q_end, w.q0 + p.tile_q);
-      const float bias = kSwap && splits == 1 ? column_bias(p, t, lane) : 0.0f;
+      if constexpr (kSwap)
+        col_bias = column_bias(p, t, lane);
       // columns of this warp that exist, in chunks of W
       const int my_cols = min(kMyCols, p.tile_q - col0);
       float *part = reinterpret_cast<float *>(tiles) + quarter * 32 + lane; // split: column c of the lane's row at c * 128
@@ -334,7 +365,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int j = 0; j < W; ++j)
             part[(c + j) * kTileP] = v[j];
         } else if constexpr (kSwap) {
-          epilogue_columns<kF32, W>(p, t, w.q0 + c, 1, v, bias, lane);
+          epilogue_columns<kF32, W>(p, t, w.q0 + c, 1, v, col_bias, lane);
         } else {
           epilogue_rows<kF32, W>(p, t, w.q0 + c, v, res, slot, lane);
         }
@@ -444,7 +475,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           peer[s] = s < splits ? map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 4 : 0u;
         if constexpr (kSwap) {
           constexpr int B = 4; // tokens at a time: rank, rank + splits, ...
-          const float bias = column_bias(p, t, lane);
           const int live = t.q_end - w.q0;
           for (int j0 = rank + half * B * splits; j0 < live; j0 += kColGroups * B * splits) {
             float v[B];
@@ -462,7 +492,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
                   v[j] += part[s];
               }
             }
-            epilogue_columns<kF32, B>(p, t, w.q0 + j0, splits, v, bias, lane);
+            epilogue_columns<kF32, B>(p, t, w.q0 + j0, splits, v, col_bias, lane);
           }
         } else {
           constexpr int V = 16; // columns at a time
@@ -506,23 +536,25 @@ cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const Linea
                        cudaStream_t stream) {
   using C = Cfg<TN, kF32>;
   auto kernel = linear_kernel<TN, kAMn, kBMn, kSwap, kF32>;
-  cudaError_t err = prepare_kernel(kernel, C::kSmemFixed + kTableBytes, nullptr);
+  cudaError_t err = prepare_kernel(kernel, C::kSmemFixed + C::kStages * C::kStageBytes + kTableBytes, nullptr);
   if (err != cudaSuccess)
     return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
   cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
+  cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + static_cast<size_t>(p.stages) * C::kStageBytes + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 0;
+  if (l.pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
   if (p.splits > 1) {
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(p.splits);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
   }
   cfg.attrs = attr;
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
@@ -571,8 +603,20 @@ cudaError_t launch_layout(const CUtensorMap &ta, const CUtensorMap &tb, const Li
 
 } // namespace
 
+int linear_max_stages(int tile_n, int out_f32) {
+  switch (tile_n) {
+  case 16: return out_f32 ? Cfg<16, true>::kStages : Cfg<16, false>::kStages;
+  case 32: return out_f32 ? Cfg<32, true>::kStages : Cfg<32, false>::kStages;
+  case 64: return out_f32 ? Cfg<64, true>::kStages : Cfg<64, false>::kStages;
+  case 128: return out_f32 ? Cfg<128, true>::kStages : Cfg<128, false>::kStages;
+  }
+  return Cfg<256, false>::kStages;
+}
+
 cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
                           cudaStream_t stream) {
+  if (l.pair)
+    return launch_linear_pair(ta, tb, p, l, stream);
   return l.out_f32 ? launch_layout<true>(ta, tb, p, l, stream) : launch_layout<false>(ta, tb, p, l, stream);
 }
 

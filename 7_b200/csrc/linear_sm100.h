@@ -34,6 +34,7 @@ struct LinearParams {
   int tile_q;        // columns of a tile: a multiple of 16 (of 64 where B is stored [K][Q]) <= the kernel's tile
   int p_blocks, q_blocks; // tiles along each side (ragged side: unused)
   int raster;        // row blocks that are walked down before the next column block
+  int stages;        // ring depth of this launch (at most the kernel's)
   int splits;        // CTAs of a cluster that share a tile's contraction; then one tile for each cluster
   int is_bf16;       // operands, z, residual and 16-bit outputs: bf16 or f16
   int act;
@@ -57,19 +58,25 @@ struct LinearLaunch {
   int tile_n;     // kernel instantiation: 16, 32, 64, 128 or 256 columns
   int out_f32;
   int grid;       // CTAs (a multiple of splits)
-  int pair;       // CTA-pair kernel
+  int pair;       // CTA-pair kernel: 256 x tile_q tiles, 16-bit results, tokens as rows
+  int pdl;        // launch with programmatic stream serialization
 };
 
-int linear_stage_box_rows();
+// Ring depth the kernel has room for; a launch may take fewer stages, at least 4.
+int linear_max_stages(int tile_n, int out_f32);
 cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
                           cudaStream_t stream);
 cudaError_t linear_read_status(int out[4], bool clear);
+// tile_q a multiple of 32 (of 128 where B is stored [K][Q]) up to 256; grid even.
+cudaError_t launch_linear_pair(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+                               cudaStream_t stream);
+cudaError_t linear_pair_read_status(int out[4], bool clear);
 
 // ---- helpers around the products (linear_aux_sm100.cu)
 // 16-bit rows with any stride into rows of `ld_dst` elements: what a TMA load
 // needs (16-byte strides) of an operand that does not have it.
 cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
-                             long long group_dst, int rows, int cols, int groups, cudaStream_t stream);
+                             long long group_dst, int rows, int cols, int groups, int pdl, cudaStream_t stream);
 
 // dz = dy * act'(z), rounded to the operands' type, and the column sums of the
 // unrounded dz (dbias) of each group in two steps of fixed order.
@@ -88,6 +95,7 @@ struct LinearActGrad {
   void *dbias; // [groups][cols]
   int dbias_type; // 0 f32, 1 f16, 2 bf16
   int vec_dy, vec_z;
+  int pdl;
 };
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows); // upper bound, sizes `partial`
 cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream);

@@ -110,6 +110,10 @@ EnvKnobs read_env() {
   }
   if (const char *v = getenv("WAVE_CUDA_LINEAR_SWAP"))
     e.linear_swap = !strcmp(v, "0") ? 0 : !strcmp(v, "1") ? 1 : -1;
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_PAIR"))
+    e.linear_pair = !strcmp(v, "0") ? 0 : !strcmp(v, "1") ? 1 : -1;
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_PDL"))
+    e.linear_pdl = strcmp(v, "0") != 0;
   return e;
 }
 } // namespace
@@ -1337,6 +1341,14 @@ int wave_cuda_check_device_status(int *out4) {
   int l[4] = {0, 0, 0, 0};
   if ((err = wave::linear_read_status(l, true)) != cudaSuccess)
     return cuda_fail(err, "read linear layer status");
+  int l2[4] = {0, 0, 0, 0};
+  if ((err = wave::linear_pair_read_status(l2, true)) != cudaSuccess)
+    return cuda_fail(err, "read linear layer (CTA pair) status");
+  if (!l[0] && l2[0]) {
+    for (int i = 0; i < 4; ++i)
+      l[i] = l2[i];
+    l[2] += 10; // roles 10.. : CTA-pair kernel
+  }
   const int *bad = g[0] ? g : (f[0] ? f : (l[0] ? l : nullptr));
   if (out4)
     for (int i = 0; i < 4; ++i)

@@ -161,7 +161,8 @@ int pack(Operand *o, char **to, cudaStream_t stream) {
   const long long ld = o->packed_ld(), group = ld * o->rows;
   const size_t bytes = o->packed_bytes();
   cudaError_t err =
-      wave::launch_pack_rows(o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices, stream);
+      wave::launch_pack_rows(o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices,
+                             wave::env_knobs().linear_pdl, stream);
   if (err != cudaSuccess)
     return cuda_fail(err, "linear: laying out an operand");
   o->ptr = *to;
@@ -183,7 +184,7 @@ int operand_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_cols, i
 // or all with one matrix; P x Q and the contraction as in LinearParams.
 struct Plan {
   LinearLaunch launch;
-  int tile_q, p_blocks, q_blocks, raster, splits;
+  int tile_q, p_blocks, q_blocks, raster, splits, stages;
 };
 
 int tile_for(int want) {
@@ -201,6 +202,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   l.a_mn = kind == Product::kWeightGrad;
   l.b_mn = kind != Product::kForward;
   l.out_f32 = out_f32;
+  l.pdl = env.linear_pdl;
   const long long M = d.tokens;
   const int N = d.out_features, K = d.in_features;
   const long long per_expert = (M + s.matrices - 1) / s.matrices;
@@ -264,6 +266,25 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
     pl.tile_q = l.tile_n;
     tiles = blocks(pl.tile_q, &pb, &qb);
   }
+  if (!l.swap && !out_f32 && env.linear_pair != 0 && !env.linear_splits) {
+    const long long pairs = sms / 2;
+    const long long p_pair = (p_ext + 255) / 256, q_pair = (q_ext + 255) / 256;
+    const long long pair_tiles = kind == Product::kWeightGrad ? p_pair * q_pair * s.matrices
+                                 : s.grouped ? q_pair * (M / 256 + (s.matrices < M ? s.matrices : M)) : p_pair * q_pair;
+    if ((pair_tiles >= pairs && per_expert >= 256) || env.linear_pair == 1) {
+      l.pair = 1;
+      l.tile_n = pl.tile_q = 256;
+      pb = p_pair;
+      qb = q_pair;
+      tiles = pair_tiles;
+      pl.raster = 8;
+      pl.splits = 1;
+      pl.p_blocks = static_cast<int>(pb);
+      pl.q_blocks = static_cast<int>(qb);
+      l.grid = static_cast<int>(2 * (tiles < pairs ? (tiles > 0 ? tiles : 1) : pairs));
+      return pl;
+    }
+  }
   // Few tiles: a cluster of CTAs shares a tile's contraction.
   pl.splits = 1;
   if (tiles > 0)
@@ -280,6 +301,14 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   l.grid = static_cast<int>(pl.splits > 1 ? tiles * pl.splits : (tiles < sms ? tiles : sms));
   if (l.grid < 1)
     l.grid = 1;
+  // A CTA with one tile takes no more stages than that has: what it leaves of the
+  // SM lets the next kernel of the stream set itself up meanwhile.
+  pl.stages = wave::linear_max_stages(l.tile_n, l.out_f32);
+  if (kind != Product::kWeightGrad || !s.grouped) {
+    const long long need = (k_iters + pl.splits - 1) / pl.splits;
+    if ((pl.splits > 1 || tiles <= sms) && need < pl.stages)
+      pl.stages = need < 4 ? 4 : static_cast<int>(need);
+  }
   return pl;
 }
 
@@ -325,6 +354,7 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   p.q_blocks = pl.q_blocks;
   p.raster = pl.raster;
   p.splits = pl.splits;
+  p.stages = pl.stages;
   p.is_bf16 = is_bf16;
   p.act = kind == Product::kForward ? d.activation : WAVE_ACT_NONE;
   p.D = o.D;
@@ -345,7 +375,7 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   int rc = operand_map(&ta, a, is_bf16, 64, l.a_mn ? 64 : 128);
   if (rc != WAVE_OK)
     return rc;
-  rc = operand_map(&tb, b, is_bf16, 64, l.b_mn ? 64 : pl.tile_q);
+  rc = operand_map(&tb, b, is_bf16, 64, l.b_mn ? 64 : l.pair ? pl.tile_q / 2 : pl.tile_q);
   if (rc != WAVE_OK)
     return rc;
   cudaError_t err = wave::launch_linear(ta, tb, p, l, stream);
@@ -509,6 +539,7 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
       g.dbias_type = s.d.dbias_type == WAVE_F32 ? 0 : is_bf16 ? 2 : 1;
       g.vec_dy = aligned16(dY) && (s.d.ldy * (g.dy_f32 ? 4 : 2)) % 16 == 0;
       g.vec_z = aligned16(g.Z) && s.d.ldz % 8 == 0;
+      g.pdl = wave::env_knobs().linear_pdl;
       cudaError_t err = wave::launch_act_grad(g, q);
       if (err != cudaSuccess)
         return cuda_fail(err, "linear: gradient of the activation");

@@ -319,8 +319,10 @@ int wave_cuda_flash_attention_fwd_host(const wave_fa_desc *desc, const void *Q_h
  * alignment only.  A workspace is used by one call at a time, nothing in it
  * needs clearing, and nothing is kept in it between calls.
  * WAVE_CUDA_LINEAR_TILE=<columns>, WAVE_CUDA_LINEAR_SPLITS=<CTAs to a tile> and
- * WAVE_CUDA_LINEAR_SWAP=0|1 override the choice of tiles (measurement knobs;
- * sums are then taken in another order).                                     */
+ * WAVE_CUDA_LINEAR_SWAP=0|1 and
+ * WAVE_CUDA_LINEAR_PAIR=0|1 override the choice of tiles, WAVE_CUDA_LINEAR_PDL=0
+ * launches without programmatic dependent launch (measurement knobs; with other
+ * tiles sums are taken in another order).                                    */
 #define WAVE_ACT_NONE 0
 #define WAVE_ACT_RELU 1
 #define WAVE_ACT_GELU 2      /* x Phi(x), with erf */

@@ -128,31 +128,43 @@ def test_forward_strided_rows(cuda, wc, wl, m, n, k, gap):
 @pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
 def test_every_tile_and_split(cuda, wc, wl, tile, splits, swap):
-    """Forward and backward in each variant of the kernels, sizes that divide by nothing."""
-    torch, gen = cuda, make_gen(cuda, tile * 10 + splits)
+    """Forward and backward in each variant of the one-CTA kernel, sizes that divide by nothing."""
+    gen = make_gen(cuda, tile * 10 + splits)
     with env_knobs(wc, WAVE_CUDA_LINEAR_TILE=tile, WAVE_CUDA_LINEAR_SPLITS=splits, WAVE_CUDA_LINEAR_SWAP=swap):
-        for m, n, k in ((45, 300, 712), (261, 136, 330)):
-            x, w, dy = (quarters(torch, gen, *s, io="bf16") for s in ((m, k), (n, k), (m, n)))
-            b, r = quarters(torch, gen, n, io="bf16"), quarters(torch, gen, m, n, io="bf16")
-            z, y = forward_want(torch, x, w, b, r, "relu")
-            for out in (torch.bfloat16, torch.float32):
-                got, got_z = wl.linear(x, w, b, r, activation="relu", out_dtype=out, save_pre_activation=True)
-                same(torch, got, y, "y")
-                same(torch, got_z, z, "z")
-                dx, dw, db = wl.linear_backward(dy, x, w, dweight_dtype=out)
-                same(torch, dx, dy.double() @ w.double(), "dx")
-                same(torch, dw, dy.double().t() @ x.double(), "dw")
-                same(torch, db, dy.double().sum(0), "db")
-            sizes = [0, 17, 0, 1, m - 20, 0]
-            off = offsets_of(torch, sizes, 1)
-            wg = quarters(torch, gen, len(sizes), n, k, io="bf16")
-            want_y, want_dx, want_dw, want_db = grouped_want(torch, x, wg, off, None, "none", dy)
-            for out in (torch.bfloat16, torch.float32):
-                same(torch, wl.grouped_linear(x, wg, off, out_dtype=out), want_y, "grouped y")
-                dx, dw, db = wl.grouped_linear_backward(dy, x, wg, off, dweight_dtype=out)
-                same(torch, dx, want_dx, "grouped dx")
-                same(torch, dw, want_dw, "grouped dw")
-                same(torch, db, want_db, "grouped db")
+        check_all(cuda, wc, wl, gen, ((45, 300, 712), (261, 136, 330)))
+
+
+def test_pairs(cuda, wc, wl):
+    """The same on CTA pairs: one tile and less, ragged edges, several tiles, experts with a handful of rows."""
+    with env_knobs(wc, WAVE_CUDA_LINEAR_SWAP=0, WAVE_CUDA_LINEAR_PAIR=1):
+        check_all(cuda, wc, wl, make_gen(cuda, 3), ((45, 300, 712), (261, 136, 330), (1000, 520, 1032), (513, 1001, 777)))
+        # more tiles than pairs, several cut stages of one expert after the other in the ring
+        check_all(cuda, wc, wl, make_gen(cuda, 4), ((300, 2504, 2568),), [3, 17, 0, 5, 33, 1, 2, 64, 80, 15, 16, 40])
+
+
+def check_all(torch, wc, wl, gen, shapes, rows=None):
+    for m, n, k in shapes:
+        x, w, dy = (quarters(torch, gen, *s, io="bf16") for s in ((m, k), (n, k), (m, n)))
+        b, r = quarters(torch, gen, n, io="bf16"), quarters(torch, gen, m, n, io="bf16")
+        z, y = forward_want(torch, x, w, b, r, "relu")
+        for out in (torch.bfloat16, torch.float32):
+            got, got_z = wl.linear(x, w, b, r, activation="relu", out_dtype=out, save_pre_activation=True)
+            same(torch, got, y, "y")
+            same(torch, got_z, z, "z")
+            dx, dw, db = wl.linear_backward(dy, x, w, dweight_dtype=out)
+            same(torch, dx, dy.double() @ w.double(), "dx")
+            same(torch, dw, dy.double().t() @ x.double(), "dw")
+            same(torch, db, dy.double().sum(0), "db")
+        sizes = rows or [0, 17, 0, 1, m - 20, 0]
+        off = offsets_of(torch, sizes, 1)
+        wg = quarters(torch, gen, len(sizes), n, k, io="bf16")
+        want_y, want_dx, want_dw, want_db = grouped_want(torch, x, wg, off, None, "none", dy)
+        for out in (torch.bfloat16, torch.float32):
+            same(torch, wl.grouped_linear(x, wg, off, out_dtype=out), want_y, "grouped y")
+            dx, dw, db = wl.grouped_linear_backward(dy, x, wg, off, dweight_dtype=out)
+            same(torch, dx, want_dx, "grouped dx")
+            same(torch, dw, want_dw, "grouped dw")
+            same(torch, db, want_db, "grouped db")
     wc.check_device_status()
 
 
