@@ -2,6 +2,8 @@
 // activation with the bias gradient's column sums, and rows laid out for TMA.
 #include "linear_common.cuh"
 
+#include <type_traits>
+
 namespace wave {
 
 namespace {
@@ -61,37 +63,58 @@ struct Eight {
   float v[8];
 };
 
-// Eight consecutive values of a row, zero beyond `cols`.
-__device__ __forceinline__ void load_eight(Eight &out, const void *base, long long at, int live, bool f32, bool vec,
-                                           int bf16) {
-  if (f32) {
-    const float *src = static_cast<const float *>(base) + at;
-    if (vec && live >= 8) {
-      const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-      out.v[0] = a.x, out.v[1] = a.y, out.v[2] = a.z, out.v[3] = a.w;
-      out.v[4] = b.x, out.v[5] = b.y, out.v[6] = b.z, out.v[7] = b.w;
+// Eight consecutive values of a row as they lie in memory: 16 bytes, or 32 in f32.
+template <bool kF32> struct Raw {
+  uint4 w[kF32 ? 2 : 1];
+};
+
+// kVec: all eight exist and are aligned; else `live` of them exist and the others are zero.
+template <bool kF32, bool kVec>
+__device__ __forceinline__ void load_raw(Raw<kF32> &out, const void *base, long long at, int live) {
+  if constexpr (kF32) {
+    const uint32_t *src = static_cast<const uint32_t *>(base) + at;
+    if constexpr (kVec) {
+      out.w[0] = *reinterpret_cast<const uint4 *>(src);
+      out.w[1] = *reinterpret_cast<const uint4 *>(src + 4);
     } else {
+      uint32_t t[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        out.v[e] = e < live ? src[e] : 0.0f;
+        t[e] = e < live ? src[e] : 0u;
+      out.w[0] = make_uint4(t[0], t[1], t[2], t[3]);
+      out.w[1] = make_uint4(t[4], t[5], t[6], t[7]);
     }
-    return;
+  } else {
+    const uint16_t *src = static_cast<const uint16_t *>(base) + at;
+    if constexpr (kVec) {
+      out.w[0] = *reinterpret_cast<const uint4 *>(src);
+    } else {
+      uint32_t t[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < live)
+          t[e >> 1] |= static_cast<uint32_t>(src[e]) << ((e & 1) * 16);
+      out.w[0] = make_uint4(t[0], t[1], t[2], t[3]);
+    }
   }
-  const uint16_t *src = static_cast<const uint16_t *>(base) + at;
-  if (vec && live >= 8) {
-    const uint4 q = *reinterpret_cast<const uint4 *>(src);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+}
+template <bool kF32> __device__ __forceinline__ Eight values(const Raw<kF32> &r, int bf16) {
+  Eight out;
+  if constexpr (kF32) {
+    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      out.v[e] = __uint_as_float(w[e]);
+  } else {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 f = unpack_pair(w[e], bf16);
       out.v[2 * e] = f.x;
       out.v[2 * e + 1] = f.y;
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      out.v[e] = e < live ? from_16bit(src[e], bf16) : 0.0f;
   }
+  return out;
 }
 
 // One chunk of rows x 256 columns to a block.  A chunk never crosses a group's
@@ -100,8 +123,11 @@ __device__ __forceinline__ void load_eight(Eight &out, const void *base, long lo
 // kAct < 0: dz = dy (column sums alone, or a copy in another layout or type).
 // The activation is a template argument: chosen for each value at run time it
 // costs more than the arithmetic (8192 x 8192 bf16, gelu_tanh: 243 us).
-template <int kAct>
-__global__ void __launch_bounds__(kAgThreads)
+// Bound by memory: what counts is bytes in flight, so rows wait in registers as
+// they lie in memory (widened on arrival they took 98 registers and left two
+// blocks to an SM: 177 us).
+template <int kAct, bool kDyF32, bool kVec>
+__global__ void __launch_bounds__(kAgThreads, kVec && !kDyF32 ? 4 : 2)
 act_grad_kernel(const __grid_constant__ LinearActGrad p) {
   extern __shared__ int ag_smem[];
   __shared__ float sums[kAgLanes][kAgCols];
@@ -137,14 +163,15 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
     acc[e] = 0.0f;
   if (live > 0) {
     for (int r = r0 + tr; r < r1; r += kAgLanes * kAgUnroll) {
-      Eight g[kAgUnroll], z[kAgUnroll];
+      Raw<kDyF32> dy_raw[kAgUnroll];
+      Raw<false> z_raw[kAgUnroll];
 #pragma unroll
       for (int u = 0; u < kAgUnroll; ++u) {
         const int row = r + u * kAgLanes;
         if (row < r1) {
-          load_eight(g[u], p.dY, static_cast<long long>(row) * p.ldy + col, live, p.dy_f32 != 0, p.vec_dy != 0, p.is_bf16);
+          load_raw<kDyF32, kVec>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
           if constexpr (kAct >= 0)
-            load_eight(z[u], p.Z, static_cast<long long>(row) * p.ldz + col, live, false, p.vec_z != 0, p.is_bf16);
+            load_raw<false, kVec>(z_raw[u], p.Z, static_cast<long long>(row) * p.ldz + col, live);
         }
       }
 #pragma unroll
@@ -152,21 +179,29 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
         const int row = r + u * kAgLanes;
         if (row >= r1)
           break;
+        Eight g = values<kDyF32>(dy_raw[u], p.is_bf16);
         if constexpr (kAct >= 0) {
+          const Eight z = values<false>(z_raw[u], p.is_bf16);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            g[u].v[e] *= act_slope(z[u].v[e], kAct);
+          for (int e = 0; e < 8; e += 2) {
+            const float2 d = __fmul2_rn(make_float2(g.v[e], g.v[e + 1]), slope_pair<kAct>(make_float2(z.v[e], z.v[e + 1])));
+            g.v[e] = d.x;
+            g.v[e + 1] = d.y;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          acc[e] += g[u].v[e];
+        for (int e = 0; e < 8; e += 2) {
+          const float2 sum = __fadd2_rn(make_float2(acc[e], acc[e + 1]), make_float2(g.v[e], g.v[e + 1]));
+          acc[e] = sum.x;
+          acc[e + 1] = sum.y;
+        }
         if (p.dZ) {
           // rows of dZ are padded to whole 16-byte pieces; columns behind the last are zero
           uint4 q;
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            w[e] = pack_pair(2 * e < live ? g[u].v[2 * e] : 0.0f, 2 * e + 1 < live ? g[u].v[2 * e + 1] : 0.0f, p.is_bf16);
+            w[e] = pack_pair(g.v[2 * e], g.v[2 * e + 1], p.is_bf16); // (zeros behind the last column: 0 * slope(0))
           q = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dZ) + static_cast<long long>(row) * p.lddz + col) = q;
         }
@@ -253,13 +288,21 @@ cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
   if (chunks > 0) {
     const dim3 grid(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks));
     auto go = [&](auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); };
-    switch (p.Z ? p.act : kActNone) {
-    case kActRelu: go(act_grad_kernel<kActRelu>); break;
-    case kActGelu: go(act_grad_kernel<kActGelu>); break;
-    case kActGeluTanh: go(act_grad_kernel<kActGeluTanh>); break;
-    case kActSilu: go(act_grad_kernel<kActSilu>); break;
-    default: go(act_grad_kernel<-1>); break;
-    }
+    auto pick = [&](auto f32, auto vec) {
+      constexpr bool kF32 = decltype(f32)::value, kVec = decltype(vec)::value;
+      switch (p.Z ? p.act : kActNone) {
+      case kActRelu: go(act_grad_kernel<kActRelu, kF32, kVec>); break;
+      case kActGelu: go(act_grad_kernel<kActGelu, kF32, kVec>); break;
+      case kActGeluTanh: go(act_grad_kernel<kActGeluTanh, kF32, kVec>); break;
+      case kActSilu: go(act_grad_kernel<kActSilu, kF32, kVec>); break;
+      default: go(act_grad_kernel<-1, kF32, kVec>); break;
+      }
+    };
+    const bool vec = p.vec_dy && (!p.Z || p.vec_z) && p.cols % 8 == 0;
+    if (p.dy_f32)
+      vec ? pick(std::true_type{}, std::true_type{}) : pick(std::true_type{}, std::false_type{});
+    else
+      vec ? pick(std::false_type{}, std::true_type{}) : pick(std::false_type{}, std::false_type{});
   }
   if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
     return err;

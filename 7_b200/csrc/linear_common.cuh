@@ -141,73 +141,113 @@ template <bool kSwap> struct TileWalk {
 };
 
 // ------------------------------------------------------------- activations
-// All in f32 on the unrounded pre-activation.  sigmoid(x) = 1 / (1 + e^-x); the
-// exponential is 2^(x log2 e) on the special-function unit (2^-22 relative for
-// |x| < 4, 2^-20 at 20: far below a 16-bit rounding and below 2e-6 in f32).
-__device__ __forceinline__ float exp_fast(float x) {
+// All in f32 on the unrounded pre-activation, two values at a time (one issue
+// slot for both).  The epilogue shares its issue slots with nobody, but it has
+// to finish a tile while the tensor core works on the next: with erff and one
+// value at a time, 8192 x 8192 x 2048 with gelu took 27 us longer than without.
+__device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGeluC = 0.7978845608028654f; // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-__device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-  case kActRelu:
-    return z < 0.0f ? 0.0f : z; // a NaN stays one
-  case kActGelu:
-    return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
-  case kActGeluTanh: // 0.5 z (1 + tanh u) = z sigmoid(2 u)
-    return __fdividef(z, 1.0f + exp_fast(-2.0f * kGeluC * (z + kGeluA * z * z * z)));
-  case kActSilu:
-    return __fdividef(z, 1.0f + exp_fast(-z));
-  }
-  return z;
+// 1 / (1 + 2^x) of both
+__device__ __forceinline__ float2 sigmoid_of_minus(float2 x) {
+  const float2 e = __fadd2_rn(make_float2(ex2(x.x), ex2(x.y)), both(1.0f));
+  return make_float2(rcp(e.x), rcp(e.y));
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-  case kActRelu:
-    return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-  case kActGelu:
-    return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) + z * 0.3989422804014327f * exp_fast(-0.5f * z * z);
-  case kActGeluTanh: {
-    const float s = __fdividef(1.0f, 1.0f + exp_fast(-2.0f * kGeluC * (z + kGeluA * z * z * z)));
-    return s + z * s * (1.0f - s) * (2.0f * kGeluC) * (1.0f + 3.0f * kGeluA * z * z);
+// Half the complementary error function of |z| / sqrt(2), the normal
+// distribution's tail behind |z|, and e^(-z^2 / 2): Abramowitz and Stegun's
+// rational approximation 7.1.26 (erfc(x) = t P(t) e^(-x^2), t = 1 / (1 + p x),
+// absolute error 1.5e-7).  `a` is |z|, cut at 20 where the tail is 0 in f32.
+__device__ __forceinline__ void normal_tail(float2 a, float2 &tail, float2 &gauss) {
+  const float2 d = __ffma2_rn(a, both(0.3275911f * 0.7071067811865476f), both(1.0f));
+  const float2 t = make_float2(rcp(d.x), rcp(d.y));
+  float2 q = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  q = __ffma2_rn(q, t, both(0.5f * 1.421413741f));
+  q = __ffma2_rn(q, t, both(0.5f * -0.284496736f));
+  q = __ffma2_rn(q, t, both(0.5f * 0.254829592f));
+  const float2 x = __fmul2_rn(__fmul2_rn(a, a), both(-0.5f * kLog2e));
+  gauss = make_float2(ex2(x.x), ex2(x.y));
+  tail = __fmul2_rn(__fmul2_rn(q, t), gauss);
+}
+
+template <int kAct> __device__ __forceinline__ float2 act_pair(float2 z) {
+  if constexpr (kAct == kActRelu) {
+    return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y); // a NaN stays one
+  } else if constexpr (kAct == kActGelu) {
+    // z Phi(z) = max(z, 0) - |z| tail
+    const float2 a = make_float2(fminf(fabsf(z.x), 20.0f), fminf(fabsf(z.y), 20.0f));
+    float2 tail, gauss;
+    normal_tail(a, tail, gauss);
+    const float2 top = make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    return __ffma2_rn(make_float2(-a.x, -a.y), tail, top);
+  } else if constexpr (kAct == kActGeluTanh) {
+    // 0.5 z (1 + tanh u) = z sigmoid(2 u)
+    const float2 k = __ffma2_rn(__fmul2_rn(z, z), both(-2.0f * kLog2e * kGeluC * kGeluA), both(-2.0f * kLog2e * kGeluC));
+    return __fmul2_rn(z, sigmoid_of_minus(__fmul2_rn(z, k)));
+  } else if constexpr (kAct == kActSilu) {
+    return __fmul2_rn(z, sigmoid_of_minus(__fmul2_rn(z, both(-kLog2e))));
+  } else {
+    return z;
   }
-  case kActSilu: {
-    const float s = __fdividef(1.0f, 1.0f + exp_fast(-z));
-    return s * (1.0f + z * (1.0f - s));
+}
+
+template <int kAct> __device__ __forceinline__ float2 slope_pair(float2 z) {
+  if constexpr (kAct == kActRelu) {
+    return make_float2(z.x > 0.0f ? 1.0f : (z.x <= 0.0f ? 0.0f : z.x), z.y > 0.0f ? 1.0f : (z.y <= 0.0f ? 0.0f : z.y));
+  } else if constexpr (kAct == kActGelu) {
+    // Phi(z) + z phi(z)
+    const float2 a = make_float2(fminf(fabsf(z.x), 20.0f), fminf(fabsf(z.y), 20.0f));
+    float2 tail, gauss;
+    normal_tail(a, tail, gauss);
+    const float2 phi = make_float2(z.x < 0.0f ? tail.x : 1.0f - tail.x, z.y < 0.0f ? tail.y : 1.0f - tail.y);
+    const float2 zc = make_float2(z.x < 0.0f ? -a.x : (z.x >= 0.0f ? a.x : z.x), z.y < 0.0f ? -a.y : (z.y >= 0.0f ? a.y : z.y));
+    return __ffma2_rn(__fmul2_rn(zc, both(0.3989422804014327f)), gauss, phi);
+  } else if constexpr (kAct == kActGeluTanh || kAct == kActSilu) {
+    // z s with s = sigmoid(r z), r = 1 or 2c (1 + a z^2): s + z s (1 - s) (r z)' = s (1 + (1 - s) z (r z)')
+    float2 s, w;
+    if constexpr (kAct == kActSilu) {
+      s = sigmoid_of_minus(__fmul2_rn(z, both(-kLog2e)));
+      w = z;
+    } else {
+      const float2 z2 = __fmul2_rn(z, z);
+      s = sigmoid_of_minus(__fmul2_rn(z, __ffma2_rn(z2, both(-2.0f * kLog2e * kGeluC * kGeluA), both(-2.0f * kLog2e * kGeluC))));
+      w = __fmul2_rn(z, __ffma2_rn(z2, both(6.0f * kGeluC * kGeluA), both(2.0f * kGeluC)));
+    }
+    const float2 rest = __ffma2_rn(s, both(-1.0f), both(1.0f));
+    return __fmul2_rn(s, __ffma2_rn(rest, w, both(1.0f)));
+  } else {
+    return both(1.0f);
   }
-  }
-  return 1.0f;
 }
 
 // The switch outside the loop over the values.
+template <int kAct, int W> __device__ __forceinline__ void apply_one(float (&v)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; i += 2) {
+    const float2 y = act_pair<kAct>(make_float2(v[i], v[i + 1]));
+    v[i] = y.x;
+    v[i + 1] = y.y;
+  }
+}
 template <int W> __device__ __forceinline__ void apply_act(float (&v)[W], int act) {
   switch (act) {
-  case kActRelu:
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      v[i] = act_value(v[i], kActRelu);
-    break;
-  case kActGelu:
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      v[i] = act_value(v[i], kActGelu);
-    break;
-  case kActGeluTanh:
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      v[i] = act_value(v[i], kActGeluTanh);
-    break;
-  case kActSilu:
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      v[i] = act_value(v[i], kActSilu);
-    break;
+  case kActRelu: apply_one<kActRelu, W>(v); break;
+  case kActGelu: apply_one<kActGelu, W>(v); break;
+  case kActGeluTanh: apply_one<kActGeluTanh, W>(v); break;
+  case kActSilu: apply_one<kActSilu, W>(v); break;
   }
 }
 
@@ -242,35 +282,51 @@ __device__ __forceinline__ float from_16bit(uint16_t w, int bf16) {
 // -------------------------------------------------------------- the epilogue
 // A warp holds W consecutive columns of 32 rows, one row to a lane, as they come
 // out of tensor memory.  Rows of memory are longer than that, so values change
-// places through a slot of shared memory that belongs to the warp: 16 bytes to a
-// lane, a row's pieces in neighbouring lanes, whole 32-byte sectors on the way
-// out.  The pitch (an odd number of 16-byte units) keeps both directions free of
-// bank conflicts.
-template <int kElem> __host__ __device__ constexpr int slot_pitch(int cols) { return cols * kElem + 16; }
+// places through a slot of shared memory that belongs to the warp: 16-byte
+// pieces, a row's in neighbouring lanes, whole 32-byte sectors on the way out.
+// Piece `c` of row `r` lies at a place that is turned by the row's number, so
+// that eight lanes that go down a column of pieces and eight that go along the
+// rows both meet all 32 banks.
+template <int kElem, int W> struct Slot {
+  static constexpr int kPieces = W * kElem / 16; // of a row: 2, 4 or 8
+  static constexpr int kVals = 16 / kElem;
+  static constexpr int kRowsPerLine = 8 / kPieces; // rows in 128 bytes
+  static constexpr int kBytes = 32 * kPieces * 16;
+  static_assert(kPieces == 2 || kPieces == 4 || kPieces == 8, "16 or 32 columns of 2 or 4 bytes");
+  static __device__ __forceinline__ int at(int r, int c) {
+    return (r * kPieces + (c ^ ((r / kRowsPerLine) & (kPieces - 1)))) * 16;
+  }
+};
 
-// Rows [0, rows) x columns [0, cols) of the slot to memory.
+// Rows [0, rows) x columns [0, cols) of the slot to memory; `base` is the
+// element of row 0, column 0.
 template <int kElem, int W>
 __device__ __forceinline__ void slot_to_global(const uint8_t *slot, void *base, long long ld, int rows, int cols,
                                                bool vec, int lane) {
-  constexpr int kPieces = W * kElem / 16; // of a row
-  constexpr int kVals = 16 / kElem;
+  using S = Slot<kElem, W>;
+  constexpr int kRowStep = 32 / S::kPieces;
+  const int r0 = lane / S::kPieces, piece = lane % S::kPieces;
+  uint8_t *dst = static_cast<uint8_t *>(base) + static_cast<long long>(r0) * ld * kElem + piece * 16;
+  const long long step = ld * (kRowStep * kElem);
+  if (vec && rows == 32 && cols == W) { // the same for the whole warp
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int idx = i * 32 + lane;
-    const int r = idx / kPieces, piece = idx % kPieces;
-    const int col = piece * kVals;
-    if (r >= rows || col >= cols)
+    for (int i = 0; i < S::kPieces; ++i, dst += step)
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(slot + S::at(r0 + i * kRowStep, piece));
+    return;
+  }
+  const int live = cols - piece * S::kVals; // columns of the piece that exist
+#pragma unroll
+  for (int i = 0; i < S::kPieces; ++i, dst += step) {
+    if (r0 + i * kRowStep >= rows || live <= 0)
       continue;
-    const uint8_t *src = slot + r * slot_pitch<kElem>(W) + piece * 16;
-    uint8_t *dst = static_cast<uint8_t *>(base) + (static_cast<long long>(r) * ld + col) * kElem;
-    const uint4 v = *reinterpret_cast<const uint4 *>(src);
-    if (vec && col + kVals <= cols) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(slot + S::at(r0 + i * kRowStep, piece));
+    if (vec && live >= S::kVals) {
       *reinterpret_cast<uint4 *>(dst) = v;
     } else {
       const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < kVals; ++e)
-        if (col + e < cols) {
+      for (int e = 0; e < S::kVals; ++e)
+        if (e < live) {
           if constexpr (kElem == 4)
             *reinterpret_cast<uint32_t *>(dst + e * 4) = words[e];
           else
@@ -285,22 +341,29 @@ __device__ __forceinline__ void slot_to_global(const uint8_t *slot, void *base, 
 template <int W>
 __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *base, long long ld, int rows, int cols,
                                                bool vec, int lane) {
-  constexpr int kPieces = W / 8;
+  using S = Slot<2, W>;
+  constexpr int kRowStep = 32 / S::kPieces;
+  const int r0 = lane / S::kPieces, piece = lane % S::kPieces;
+  const uint16_t *src = static_cast<const uint16_t *>(base) + static_cast<long long>(r0) * ld + piece * 8;
+  const long long step = ld * kRowStep;
+  if (vec && rows == 32 && cols == W) {
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int idx = i * 32 + lane;
-    const int r = idx / kPieces, piece = idx % kPieces;
-    const int col = piece * 8;
+    for (int i = 0; i < S::kPieces; ++i, src += step)
+      out[i] = *reinterpret_cast<const uint4 *>(src);
+    return;
+  }
+  const int live = cols - piece * 8;
+#pragma unroll
+  for (int i = 0; i < S::kPieces; ++i, src += step) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows && col < cols) {
-      const uint16_t *src = static_cast<const uint16_t *>(base) + static_cast<long long>(r) * ld + col;
-      if (vec && col + 8 <= cols) {
+    if (r0 + i * kRowStep < rows && live > 0) {
+      if (vec && live >= 8) {
         v = *reinterpret_cast<const uint4 *>(src);
       } else {
         uint32_t words[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (col + e < cols)
+          if (e < live)
             words[e >> 1] |= static_cast<uint32_t>(src[e]) << ((e & 1) * 16);
         v = make_uint4(words[0], words[1], words[2], words[3]);
       }
@@ -308,21 +371,13 @@ __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *
     out[i] = v;
   }
 }
-template <int W> __device__ __forceinline__ void regs_to_slot(uint8_t *slot, const uint4 (&v)[W / 8], int lane) {
-  constexpr int kPieces = W / 8;
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int idx = i * 32 + lane;
-    *reinterpret_cast<uint4 *>(slot + (idx / kPieces) * slot_pitch<2>(W) + (idx % kPieces) * 16) = v[i];
-  }
-}
 
 template <int W> __device__ __forceinline__ void row_to_slot_16bit(uint8_t *slot, const float (&v)[W], int bf16, int lane) {
-  uint4 *dst = reinterpret_cast<uint4 *>(slot + lane * slot_pitch<2>(W));
 #pragma unroll
   for (int k = 0; k < W / 8; ++k)
-    dst[k] = make_uint4(pack_pair(v[8 * k], v[8 * k + 1], bf16), pack_pair(v[8 * k + 2], v[8 * k + 3], bf16),
-                        pack_pair(v[8 * k + 4], v[8 * k + 5], bf16), pack_pair(v[8 * k + 6], v[8 * k + 7], bf16));
+    *reinterpret_cast<uint4 *>(slot + Slot<2, W>::at(lane, k)) =
+        make_uint4(pack_pair(v[8 * k], v[8 * k + 1], bf16), pack_pair(v[8 * k + 2], v[8 * k + 3], bf16),
+                   pack_pair(v[8 * k + 4], v[8 * k + 5], bf16), pack_pair(v[8 * k + 6], v[8 * k + 7], bf16));
 }
 
 // What a warp's epilogue needs to know of its tile.
@@ -334,44 +389,49 @@ struct EpiTile {
 };
 
 // Bytes of a warp's slot.
-template <bool kF32> __host__ __device__ constexpr int slot_bytes() {
-  return 32 * (kF32 ? slot_pitch<4>(32) : slot_pitch<2>(32));
-}
+template <bool kF32> __host__ __device__ constexpr int slot_bytes() { return kF32 ? Slot<4, 32>::kBytes : Slot<2, 32>::kBytes; }
 
-// The residual of a chunk, fetched ahead of the accumulator (tokens as rows).
+// What a chunk's epilogue reads from memory, fetched while the chunk before it
+// is worked on (tokens as rows): the residual in the order of slot_to_global,
+// and the bias, one value to a lane.
+template <int W> struct Ahead {
+  uint4 res[W / 8];
+  float bias;
+};
 template <int W>
-__device__ __forceinline__ void fetch_residual(uint4 (&res)[W / 8], const LinearParams &p, const EpiTile &t, int q0,
-                                               int lane) {
+__device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, const EpiTile &t, int q0, int lane) {
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
-  global_to_regs<W>(res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(t.lane0) * p.ldr + q0, p.ldr, rows,
-                    cols, p.vec_r != 0, lane);
+  if (p.R)
+    global_to_regs<W>(f.res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(t.lane0) * p.ldr + q0, p.ldr, rows,
+                      cols, p.vec_r != 0, lane);
+  f.bias = 0.0f;
+  if (p.bias && lane < cols) {
+    const long long at = t.group * p.group_bias + q0 + lane;
+    f.bias = p.bias_f32 ? static_cast<const float *>(p.bias)[at]
+                        : from_16bit(static_cast<const uint16_t *>(p.bias)[at], p.is_bf16);
+  }
 }
 
 // Tokens as rows: v holds columns q0 .. q0 + W of the lane's row.
 template <bool kF32, int W>
 __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
-                                              const uint4 (&res)[W / 8], uint8_t *slot, int lane) {
+                                              const Ahead<W> &f, uint8_t *slot, int lane) {
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
   if (rows <= 0 || cols <= 0)
     return; // the same for the whole warp
-  if (p.bias) {
-    // one value to a lane, handed round through the slot
-    float b = 0.0f;
-    if (lane < cols) {
-      const long long at = t.group * p.group_bias + q0 + lane;
-      b = p.bias_f32 ? static_cast<const float *>(p.bias)[at]
-                     : from_16bit(static_cast<const uint16_t *>(p.bias)[at], p.is_bf16);
-    }
+  if (p.bias) { // handed round through the slot
     if (lane < W)
-      reinterpret_cast<float *>(slot)[lane] = b;
+      reinterpret_cast<float *>(slot)[lane] = f.bias;
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
-      const float4 f = reinterpret_cast<const float4 *>(slot)[k];
-      v[4 * k] += f.x;
-      v[4 * k + 1] += f.y;
-      v[4 * k + 2] += f.z;
-      v[4 * k + 3] += f.w;
+      const float4 b = reinterpret_cast<const float4 *>(slot)[k];
+      const float2 lo = __fadd2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(b.x, b.y));
+      const float2 hi = __fadd2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(b.z, b.w));
+      v[4 * k] = lo.x;
+      v[4 * k + 1] = lo.y;
+      v[4 * k + 2] = hi.x;
+      v[4 * k + 3] = hi.y;
     }
     __syncwarp();
   }
@@ -384,28 +444,32 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
   }
   apply_act<W>(v, p.act);
   if (p.R) {
-    regs_to_slot<W>(slot, res, lane);
+    using S = Slot<2, W>;
+    constexpr int kRowStep = 32 / S::kPieces;
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i)
+      *reinterpret_cast<uint4 *>(slot + S::at(lane / S::kPieces + i * kRowStep, lane % S::kPieces)) = f.res[i];
     __syncwarp();
-    const uint4 *mine = reinterpret_cast<const uint4 *>(slot + lane * slot_pitch<2>(W));
 #pragma unroll
     for (int k = 0; k < W / 8; ++k) {
-      const uint4 w = mine[k];
+      const uint4 w = *reinterpret_cast<const uint4 *>(slot + S::at(lane, k));
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack_pair(words[e], p.is_bf16);
-        v[8 * k + 2 * e] += f.x;
-        v[8 * k + 2 * e + 1] += f.y;
+        const int j = 8 * k + 2 * e;
+        const float2 sum = __fadd2_rn(make_float2(v[j], v[j + 1]), unpack_pair(words[e], p.is_bf16));
+        v[j] = sum.x;
+        v[j + 1] = sum.y;
       }
     }
     __syncwarp(); // f32 rows are longer: the slot may be rewritten once every lane has its residual
   }
   const long long at = t.group * p.group_d + static_cast<long long>(t.lane0) * p.ldd + q0;
   if constexpr (kF32) {
-    float4 *dst = reinterpret_cast<float4 *>(slot + lane * slot_pitch<4>(W));
 #pragma unroll
     for (int k = 0; k < W / 4; ++k)
-      dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+      *reinterpret_cast<float4 *>(slot + Slot<4, W>::at(lane, k)) =
+          make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
     __syncwarp();
     slot_to_global<4, W>(slot, static_cast<float *>(p.D) + at, p.ldd, rows, cols, p.vec_d != 0, lane);
   } else {

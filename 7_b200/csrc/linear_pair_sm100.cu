@@ -318,9 +318,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       t.lane_end = w.p_end;
       t.q_end = min(w.q_end, w.q0 + p.tile_q);
       const int my_cols = min(kMyCols, p.tile_q - col0);
-      uint4 res[kW / 8];
-      if (p.R && my_cols > 0)
-        fetch_residual<kW>(res, p, t, w.q0 + col0, lane);
+      Ahead<kW> next;
+      if (my_cols > 0)
+        fetch_ahead<kW>(next, p, t, w.q0 + col0, lane);
       if (!empty) {
         if (!mbar_wait(&sh->tfull[acc], acc_phase, abort_flag)) {
           if (lane == 0)
@@ -344,12 +344,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           for (int j = 0; j < kW; ++j)
             v[j] = __uint_as_float(r[j]);
         }
-        uint4 now[kW / 8];
-#pragma unroll
-        for (int j = 0; j < kW / 8; ++j)
-          now[j] = res[j];
-        if (p.R && c + kW < my_cols)
-          fetch_residual<kW>(res, p, t, w.q0 + col0 + c + kW, lane);
+        const Ahead<kW> now = next;
+        if (c + kW < my_cols)
+          fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + kW, lane);
         epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, now, slot, lane);
       }
       if (!empty) {

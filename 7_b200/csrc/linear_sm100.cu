@@ -80,9 +80,12 @@ __device__ __noinline__ void report(int code, int role, int detail) {
   }
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -358,16 +361,17 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         col_bias = column_bias(p, t, lane);
       // columns of this warp that exist, in chunks of W
       const int my_cols = min(kMyCols, p.tile_q - col0);
-      float *part = reinterpret_cast<float *>(tiles) + quarter * 32 + lane; // split: column c of the lane's row at c * 128
-      auto chunk = [&](int c, float (&v)[W], const uint4 (&res)[W / 8]) {
+      // split: four columns c .. c + 3 of a row side by side, 128 rows of them one after the other
+      float4 *part = reinterpret_cast<float4 *>(tiles) + quarter * 32 + lane;
+      auto chunk = [&](int c, float (&v)[W], const Ahead<W> &f) {
         if (splits > 1) {
 #pragma unroll
-          for (int j = 0; j < W; ++j)
-            part[(c + j) * kTileP] = v[j];
+          for (int j = 0; j < W; j += 4)
+            part[(c + j) / 4 * kTileP] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else if constexpr (kSwap) {
           epilogue_columns<kF32, W>(p, t, w.q0 + c, 1, v, col_bias, lane);
         } else {
-          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, res, slot, lane);
+          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, f, slot, lane);
         }
       };
       if constexpr (kF32) {
@@ -397,21 +401,20 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         for (int c = 0; c < kMyCols; c += W) {
           if (c >= my_cols)
             break;
-          uint4 res[W / 8];
-          if (!kSwap && p.R && splits == 1)
-            fetch_residual<W>(res, p, t, w.q0 + col0 + c, lane);
+          Ahead<W> f;
+          if (!kSwap && splits == 1)
+            fetch_ahead<W>(f, p, t, w.q0 + col0 + c, lane);
           float v[W];
 #pragma unroll
           for (int j = 0; j < W; ++j)
             v[j] = run[c + j];
-          chunk(col0 + c, v, res);
+          chunk(col0 + c, v, f);
         }
       } else {
         const bool empty = kb0 == kb1; // nothing to multiply: the epilogue of zero
-        uint4 res[W / 8];
-        const bool want_res = !kSwap && p.R && splits == 1;
-        if (want_res && my_cols > 0)
-          fetch_residual<W>(res, p, t, w.q0 + col0, lane);
+        Ahead<W> next;
+        if (!kSwap && splits == 1 && my_cols > 0)
+          fetch_ahead<W>(next, p, t, w.q0 + col0, lane);
         if (!empty && !wait_acc()) {
           ok = false;
           break;
@@ -426,12 +429,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           } else {
             tmem_load<W>(lane_addr + static_cast<uint32_t>(acc * TN + col0 + c), v);
           }
-          uint4 now[W / 8];
-#pragma unroll
-          for (int j = 0; j < W / 8; ++j)
-            now[j] = res[j];
-          if (want_res && c + W < my_cols)
-            fetch_residual<W>(res, p, t, w.q0 + col0 + c + W, lane);
+          const Ahead<W> now = next;
+          if (!kSwap && splits == 1 && c + W < my_cols)
+            fetch_ahead<W>(next, p, t, w.q0 + col0 + c + W, lane);
           chunk(col0 + c, v, now);
         }
         if (!empty)
@@ -472,47 +472,49 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         uint32_t peer[kLinearMaxSplits];
 #pragma unroll
         for (int s = 0; s < kLinearMaxSplits; ++s)
-          peer[s] = s < splits ? map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 4 : 0u;
-        if constexpr (kSwap) {
-          constexpr int B = 4; // tokens at a time: rank, rank + splits, ...
-          const int live = t.q_end - w.q0;
-          for (int j0 = rank + half * B * splits; j0 < live; j0 += kColGroups * B * splits) {
-            float v[B];
+          peer[s] = s < splits ? map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 16 : 0u;
+        // four columns from all parts, in flight together, added in rank order
+        auto four = [&](int col) {
+          float4 part[kLinearMaxSplits];
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-              v[j] = 0.0f;
-              const int col = j0 + j * splits;
-              if (col < live) {
-                float part[kLinearMaxSplits];
+          for (int s = 0; s < kLinearMaxSplits; ++s)
+            if (s < splits)
+              part[s] = ld_cluster_f32x4(peer[s] + col / 4 * (kTileP * 16));
+          float4 sum = part[0];
 #pragma unroll
-                for (int s = 0; s < kLinearMaxSplits; ++s)
-                  part[s] = s < splits ? ld_cluster_f32(peer[s] + col * (kTileP * 4)) : 0.0f;
-#pragma unroll
-                for (int s = 0; s < kLinearMaxSplits; ++s)
-                  v[j] += part[s];
-              }
+          for (int s = 1; s < kLinearMaxSplits; ++s)
+            if (s < splits) {
+              sum.x += part[s].x;
+              sum.y += part[s].y;
+              sum.z += part[s].z;
+              sum.w += part[s].w;
             }
-            epilogue_columns<kF32, B>(p, t, w.q0 + j0, splits, v, col_bias, lane);
+          return sum;
+        };
+        if constexpr (kSwap) {
+          // four tokens at a time
+          const int live = t.q_end - w.q0;
+          for (int i = rank + half * splits; i * 4 < live; i += kColGroups * splits) {
+            const float4 f = four(i * 4);
+            float v[4] = {f.x, f.y, f.z, f.w};
+            epilogue_columns<kF32, 4>(p, t, w.q0 + i * 4, 1, v, col_bias, lane);
           }
         } else {
           constexpr int V = 16; // columns at a time
           for (int i = rank + half * splits; i * V < p.tile_q; i += kColGroups * splits) {
             const int q0 = w.q0 + i * V;
-            uint4 res[V / 8];
-            if (p.R)
-              fetch_residual<V>(res, p, t, q0, lane);
+            Ahead<V> f;
+            fetch_ahead<V>(f, p, t, q0, lane);
             float v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-              v[j] = 0.0f;
-#pragma unroll 1
-            for (int s = 0; s < splits; ++s) {
-              const uint32_t from = map_to_cta(tiles, static_cast<uint32_t>(s)) + (quarter * 32 + lane) * 4;
-#pragma unroll
-              for (int j = 0; j < V; ++j)
-                v[j] += ld_cluster_f32(from + (i * V + j) * (kTileP * 4));
+            for (int j = 0; j < V; j += 4) {
+              const float4 q = four(i * V + j);
+              v[j] = q.x;
+              v[j + 1] = q.y;
+              v[j + 2] = q.z;
+              v[j + 3] = q.w;
             }
-            epilogue_rows<kF32, V>(p, t, q0, v, res, slot, lane);
+            epilogue_rows<kF32, V>(p, t, q0, v, f, slot, lane);
           }
         }
       }
