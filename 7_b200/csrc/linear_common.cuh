@@ -62,11 +62,16 @@ __device__ __forceinline__ void build_group_table(const GroupTable &t, const int
 }
 
 // ---------------------------------------------------------------- tile walk
+// A value that is the same in the whole warp, said so that the compiler keeps it
+// in a uniform register: the instructions that start TMA copies and products
+// take their operands from there.
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 struct Tile {
-  int group;
-  int p0, p_end;     // first row on the P side, end of the live rows
-  int q0, q_end;     // first column on the Q side, end of the live columns
-  int k_begin, k_len; // contraction: first index (rows of the group when ragged) and length
+  int group = 0;
+  int p0 = 0, p_end = 0; // first row on the P side, end of the live rows
+  int q0 = 0, q_end = 0; // first column on the Q side, end of the live columns
+  int k_begin = 0, k_len = 0; // contraction: first index (rows of the group when ragged) and length
 };
 
 // Local tile id -> (row block, column block): `raster` row blocks are walked
@@ -89,6 +94,16 @@ template <bool kSwap> struct TileWalk {
   int tile_p;
   __device__ TileWalk(const LinearParams &params, const GroupTable &table, int rows_of_tile)
       : p(params), t(table), g(0), tile_p(rows_of_tile) {}
+  // get() by a whole warp, the answer in uniform registers.
+  __device__ bool get_uniform(int id, Tile &w) {
+    const bool got = get(id, w);
+    w.group = warp_uniform(w.group);
+    w.p0 = warp_uniform(w.p0);
+    w.q0 = warp_uniform(w.q0);
+    w.k_begin = warp_uniform(w.k_begin);
+    w.k_len = warp_uniform(w.k_len);
+    return __all_sync(0xffffffffu, got) != 0;
+  }
   // Tiles are asked for in increasing order.  False: there is no such tile.
   __device__ bool get(int id, Tile &w) {
     if (p.ragged == kRaggedRows) {
@@ -139,6 +154,30 @@ template <bool kSwap> struct TileWalk {
     return true;
   }
 };
+
+// ------------------------------------------------------------- the stage ring
+// Position in the ring of stages: index, and the parity of its turn.
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+// A wait by a whole warp, which gives up together.  `seen`: the barrier was
+// already found complete (looked at while the stage before was being issued: the
+// look takes as long as the issue of a stage's products).
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, bool seen) {
+  if (seen)
+    return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+}
+__device__ __forceinline__ bool warp_peek(uint64_t *bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)) != 0;
+}
 
 // ------------------------------------------------------------- activations
 // All in f32 on the unrounded pre-activation, two values at a time (one issue

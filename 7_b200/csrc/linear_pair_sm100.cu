@@ -91,7 +91,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   table.blocks = table.begin + p.groups + 1;
   volatile int *abort_flag = &sh->abort_flag;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const bool leader = rank == 0;
@@ -134,128 +134,135 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
-    if (lane == 0) {
-      TileWalk<false> walk(p, table, kPairP);
-      Tile w;
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const int half_q = p.tile_q / 2;
-      const uint32_t tx = kABytes + static_cast<uint32_t>(half_q) * kBK * 2; // one CTA's bytes
-      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
-        const int kbs = (w.k_len + kBK - 1) / kBK;
-        const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
-        const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * half_q;
-        for (int kb = 0; kb < kbs; ++kb) {
-          if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag)) {
-            pair_report(kStatusWaitTimeout, 0, stage);
-            ok = false;
-            break;
-          }
-          uint8_t *a_dst = tiles + stage * kStageBytes;
-          uint8_t *b_dst = a_dst + kABytes;
-          const int k = w.k_begin + kb * kBK;
-          if (is_cut(live_of(w, kb))) {
+    TileWalk<false> walk(p, table, kPairP);
+    Tile w;
+    Ring ring;
+    bool ok = true;
+    const bool chosen = elect_one();
+    const int half_q = p.tile_q / 2;
+    const uint32_t tx = kABytes + static_cast<uint32_t>(half_q) * kBK * 2; // one CTA's bytes
+    for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
+      const int kbs = (w.k_len + kBK - 1) / kBK;
+      const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
+      const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * half_q;
+      bool seen = false;
+      for (int kb = 0; kb < kbs; ++kb) {
+        ok = warp_wait(&sh->empty[ring.stage], ring.phase ^ 1, abort_flag, seen);
+        if (!ok) {
+          pair_report(kStatusWaitTimeout, 0, ring.stage);
+          break;
+        }
+        uint8_t *a_dst = tiles + ring.stage * kStageBytes;
+        uint8_t *b_dst = a_dst + kABytes;
+        uint64_t *bar = &sh->full[ring.stage];
+        uint64_t *landed = &sh->landed[ring.stage];
+        const int k = w.k_begin + kb * kBK;
+        ring.advance(kStages);
+        seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
+        if (kCut && is_cut(live_of(w, kb))) {
+          if (chosen) {
             // this CTA's bytes on its own barrier: warp 1 cuts them
-            uint64_t *bar = &sh->landed[stage];
-            mbar_arrive_expect_tx(bar, tx);
+            mbar_arrive_expect_tx(landed, tx);
             for (int c = 0; c < kRows / 64; ++c)
-              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, landed, pa + c * 64, k, za);
             for (int c = 0; c < half_q / 64; ++c)
-              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
-          } else {
-            uint64_t *bar = &sh->full[stage];
-            if (leader)
-              mbar_arrive_expect_tx(bar, 2 * tx);
-            if constexpr (kAMn) {
-              for (int c = 0; c < kRows / 64; ++c)
-                tma_load_3d_pair(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
-            } else {
-              tma_load_3d_pair(a_dst, &tm_a, bar, k, pa, za);
-            }
-            if constexpr (kBMn) {
-              for (int c = 0; c < half_q / 64; ++c)
-                tma_load_3d_pair(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
-            } else {
-              tma_load_3d_pair(b_dst, &tm_b, bar, k, qb, zb);
-            }
+              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, landed, qb + c * 64, k, zb);
           }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
+        } else if (chosen) {
+          if (leader)
+            mbar_arrive_expect_tx(bar, 2 * tx);
+          if constexpr (kAMn) {
+#pragma unroll
+            for (int c = 0; c < kRows / 64; ++c)
+              tma_load_3d_pair(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+          } else {
+            tma_load_3d_pair(a_dst, &tm_a, bar, k, pa, za);
+          }
+          if constexpr (kBMn) {
+#pragma unroll
+            for (int c = 0; c < kTN / 128; ++c)
+              if (c * 64 < half_q)
+                tma_load_3d_pair(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
+          } else {
+            tma_load_3d_pair(b_dst, &tm_b, bar, k, qb, zb);
           }
         }
+        __syncwarp();
       }
-      if (!ok)
-        bounded_delay(1 << 21);
     }
+    if (!ok)
+      bounded_delay(1 << 21);
   } else if (warp == 1) {
     // ---------------------- UMMA issue (leader), cutting of last stages (both)
-    // The loop over whole stages is kept as bare as in linear_sm100.cu.
-    if (kCut || (leader && lane == 0)) {
+    if (kCut || leader) {
       const uint32_t idesc = umma_idesc_f16(kPairP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
       constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
       constexpr uint64_t kStep = kStageBytes >> 4;
       const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
       const uint64_t da0 = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
       const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
+      const uint32_t tmem_d = static_cast<uint32_t>(warp_uniform(static_cast<int>(tmem_base)));
+      const bool chosen = elect_one();
       TileWalk<false> walk(p, table, kPairP);
       Tile w;
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0, cut_phases = 0; // of landed and cut: a bit to a stage
+      Ring ring;
+      int acc = 0;
+      uint32_t acc_phase = 0, cut_phases = 0; // of landed and cut: a bit to a stage
       bool ok = true;
-      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+      for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
         const int kbs = (w.k_len + kBK - 1) / kBK;
         if (kbs <= 0)
           continue;
         const int live = live_of(w, kbs - 1);
         const bool cut = is_cut(live);
         const int whole = kbs - (cut ? 1 : 0);
-        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTN);
+        const uint32_t d = tmem_d + static_cast<uint32_t>(acc * kTN);
         uint32_t more = 0; // the accumulator holds something
-        if (leader && lane == 0) {
-          ok = mbar_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag);
-          if (!ok)
+        if (leader) {
+          ok = warp_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag, false);
+          if (!ok) {
             pair_report(kStatusWaitTimeout, 1, 100 + acc);
-          tc_fence_after_sync();
-          int st = stage;
-          uint32_t ph = phase;
-          for (int i = 0; ok && i < whole; ++i) {
-            if (!mbar_wait(&sh->full[st], ph, abort_flag)) {
-              pair_report(kStatusWaitTimeout, 1, st);
-              ok = false;
+            break;
+          }
+          bool seen = false;
+          for (int i = 0; i < whole; ++i) {
+            ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, seen);
+            if (!ok) {
+              pair_report(kStatusWaitTimeout, 1, ring.stage);
               break;
             }
             tc_fence_after_sync();
-            const uint64_t da = da0 + static_cast<uint64_t>(st) * kStep, db = db0 + static_cast<uint64_t>(st) * kStep;
-            umma_ss_pair(d, da, db, idesc, more);
+            const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
+            uint64_t *done = &sh->empty[ring.stage];
+            ring.advance(kStages);
+            seen = warp_peek(&sh->full[ring.stage], ring.phase);
+            if (chosen) {
+              umma_ss_pair(d, da, db, idesc, more);
 #pragma unroll
-            for (int k = 1; k < kBK / 16; ++k)
-              umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
-            more = 1;
-            umma_commit_pair(&sh->empty[st], 3); // frees the stage in both CTAs
-            if (++st == kStages) {
-              st = 0;
-              ph ^= 1;
+              for (int k = 1; k < kBK / 16; ++k)
+                umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+              umma_commit_pair(done, 3); // frees the stage in both CTAs
             }
+            __syncwarp();
+            more = 1;
           }
-        }
-        {
-          const int at = stage + whole; // every lane, in both CTAs, keeps count
-          phase ^= static_cast<uint32_t>(at / kStages) & 1u;
-          stage = at % kStages;
+          if (!ok)
+            break;
+        } else { // only the last stage is this CTA's business
+          const int at = ring.stage + whole;
+          ring.phase ^= static_cast<uint32_t>(at / kStages) & 1u;
+          ring.stage = at % kStages;
         }
         if constexpr (kCut) {
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-          if (ok && cut) {
-            const uint32_t parity = (cut_phases >> stage) & 1u;
-            cut_phases ^= 1u << stage;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh->landed[stage], parity, abort_flag)) != 0;
+          if (cut) {
+            const uint32_t parity = (cut_phases >> ring.stage) & 1u;
+            cut_phases ^= 1u << ring.stage;
+            ok = warp_wait(&sh->landed[ring.stage], parity, abort_flag, false);
             if (!ok) {
-              pair_report(kStatusWaitTimeout, 1, 50 + stage);
+              pair_report(kStatusWaitTimeout, 1, 50 + ring.stage);
               break;
             }
-            uint8_t *a_tile = tiles + stage * kStageBytes;
+            uint8_t *a_tile = tiles + ring.stage * kStageBytes;
             const int steps = (live + 15) / 16;
             const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
             const int chunks = kRows / 64 + p.tile_q / 128;
@@ -266,33 +273,34 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             fence_proxy_async_smem();
             __syncwarp();
             if (leader) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&sh->cut[stage], parity, abort_flag)) != 0;
+              ok = warp_wait(&sh->cut[ring.stage], parity, abort_flag, false);
               if (!ok) {
-                pair_report(kStatusWaitTimeout, 1, 70 + stage);
+                pair_report(kStatusWaitTimeout, 1, 70 + ring.stage);
                 break;
               }
               fence_acquire_cluster();
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0) {
-                mbar_arrive(&sh->full[stage]); // the stage's turn of this barrier
+              if (chosen) {
+                mbar_arrive(&sh->full[ring.stage]); // the stage's turn of this barrier
                 tc_fence_after_sync();
-                const uint64_t da = da0 + static_cast<uint64_t>(stage) * kStep, db = db0 + static_cast<uint64_t>(stage) * kStep;
+                const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
                 for (int k = 0; k < steps; ++k, more = 1)
                   umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, more);
-                umma_commit_pair(&sh->empty[stage], 3);
+                umma_commit_pair(&sh->empty[ring.stage], 3);
               }
-            } else if (lane == 0) {
-              mbar_arrive_cluster(map_to_cta(&sh->cut[stage], 0));
+              __syncwarp();
+            } else {
+              if (lane == 0)
+                mbar_arrive_cluster(map_to_cta(&sh->cut[ring.stage], 0));
+              __syncwarp();
             }
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
-            }
+            ring.advance(kStages);
           }
         }
-        if (ok && leader && lane == 0)
+        if (leader && chosen)
           umma_commit_pair(&sh->tfull[acc], 3);
+        __syncwarp();
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;

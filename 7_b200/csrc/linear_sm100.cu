@@ -123,7 +123,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   table.blocks = table.begin + p.groups + 1;
   volatile int *abort_flag = &sh->abort_flag;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
   const int splits = p.splits;
   const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -171,122 +171,117 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
-    if (lane == 0) {
-      TileWalk<kSwap> walk(p, table, kTileP);
-      Tile w;
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t tx = kABytes + static_cast<uint32_t>(p.tile_q) * kBK * 2;
-      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
-        int kb0, kb1;
-        k_blocks(w, kb0, kb1);
-        const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag)) {
-            report(kStatusWaitTimeout, 0, stage);
-            ok = false;
-            break;
-          }
-          uint8_t *a_dst = tiles + stage * C::kStageBytes;
-          uint8_t *b_dst = a_dst + kABytes;
-          uint64_t *bar = &sh->full[stage];
-          const int k = w.k_begin + kb * kBK;
+    // Like the issuing warp below, the whole warp walks and waits and one elected
+    // lane acts: with the loop in one lane's branch the compiler cannot keep the
+    // operands of the copies and products in uniform registers, and a stage takes
+    // 0.28 us to issue whatever the size of its tile (now 0.11).
+    TileWalk<kSwap> walk(p, table, kTileP);
+    Tile w;
+    Ring ring;
+    bool ok = true;
+    const bool chosen = elect_one();
+    const uint32_t tx = kABytes + static_cast<uint32_t>(p.tile_q) * kBK * 2;
+    for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
+      int kb0, kb1;
+      k_blocks(w, kb0, kb1);
+      const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
+      bool seen = false;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = warp_wait(&sh->empty[ring.stage], ring.phase ^ 1, abort_flag, seen);
+        if (!ok) {
+          report(kStatusWaitTimeout, 0, ring.stage);
+          break;
+        }
+        uint8_t *a_dst = tiles + ring.stage * C::kStageBytes;
+        uint8_t *b_dst = a_dst + kABytes;
+        uint64_t *bar = &sh->full[ring.stage];
+        const int k = w.k_begin + kb * kBK;
+        ring.advance(num_stages);
+        seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
+        if (chosen) {
           mbar_arrive_expect_tx(bar, tx);
           if constexpr (kAMn) {
+#pragma unroll
             for (int c = 0; c < kTileP / 64; ++c)
               tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, w.p0 + c * 64, k, za);
           } else {
             tma_load_3d(a_dst, &tm_a, bar, k, w.p0, za);
           }
           if constexpr (kBMn) {
-            for (int c = 0; c < p.tile_q / 64; ++c)
-              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, w.q0 + c * 64, k, zb);
+#pragma unroll
+            for (int c = 0; c < TN / 64; ++c)
+              if (c * 64 < p.tile_q)
+                tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, w.q0 + c * 64, k, zb);
           } else {
             tma_load_3d(b_dst, &tm_b, bar, k, w.q0, zb);
           }
-          if (++stage == num_stages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
+        __syncwarp();
       }
-      if (!ok)
-        bounded_delay(1 << 21); // let copies in flight land before teardown
     }
+    if (!ok)
+      bounded_delay(1 << 21); // let copies in flight land before teardown
   } else if (warp == 1) {
     // -------------------------------------------------------- UMMA issue
-    // One thread issues; the loop over whole stages holds nothing but a wait, four
-    // products and a commit (descriptors are one addition away from those of stage
-    // 0: built anew for each stage, with the number of steps looked at, 8192^3 took
-    // 14 % longer).  The weight gradient's warp stays together for the last stage
-    // of an expert, which all its lanes cut.
-    if (kCut || lane == 0) {
-      const uint32_t idesc = umma_idesc_f16(kTileP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
-      constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
-      constexpr uint64_t kStep = C::kStageBytes >> 4;
-      const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
-      const uint64_t da0 = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
-      const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
-      TileWalk<kSwap> walk(p, table, kTileP);
-      Tile w;
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
-        int kb0, kb1;
-        k_blocks(w, kb0, kb1);
-        // the stage with an expert's last rows, if it is one of this CTA's
-        const int live = w.k_len & (kBK - 1);
-        const bool cut = kCut && p.ragged == kRaggedK && live != 0 && kb1 > kb0 && kb1 * kBK > w.k_len;
-        for (int kb = kb0; ok && kb < kb1;) {
-          const int end = kF32 ? min(kb + kSegment, kb1) : kb1;
-          const bool cut_here = cut && end == kb1;
-          const int whole = end - kb - (cut_here ? 1 : 0);
-          const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TN);
-          uint32_t more = 0; // the accumulator holds something
-          if (lane == 0) {
-            ok = mbar_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag);
-            if (!ok)
-              report(kStatusWaitTimeout, 1, 100 + acc);
-            tc_fence_after_sync();
-            int st = stage;
-            uint32_t ph = phase;
-            for (int i = 0; ok && i < whole; ++i) {
-              if (!mbar_wait(&sh->full[st], ph, abort_flag)) {
-                report(kStatusWaitTimeout, 1, st);
-                ok = false;
-                break;
-              }
-              tc_fence_after_sync();
-              const uint64_t da = da0 + static_cast<uint64_t>(st) * kStep, db = db0 + static_cast<uint64_t>(st) * kStep;
-              umma_ss(d, da, db, idesc, more);
+    // The loop over whole stages holds nothing but a wait, four products and a
+    // commit (descriptors are one addition away from those of stage 0).
+    const uint32_t idesc = umma_idesc_f16(kTileP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
+    constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
+    constexpr uint64_t kStep = C::kStageBytes >> 4;
+    const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
+    const uint64_t da0 = kAMn ? umma_desc_mnmajor_sw128(a_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(a_addr);
+    const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
+    const uint32_t tmem_d = static_cast<uint32_t>(warp_uniform(static_cast<int>(tmem_base)));
+    const bool chosen = elect_one();
+    TileWalk<kSwap> walk(p, table, kTileP);
+    Tile w;
+    Ring ring;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
+      int kb0, kb1;
+      k_blocks(w, kb0, kb1);
+      // the stage with an expert's last rows, if it is one of this CTA's
+      const int live = w.k_len & (kBK - 1);
+      const bool cut = kCut && p.ragged == kRaggedK && live != 0 && kb1 > kb0 && kb1 * kBK > w.k_len;
+      for (int kb = kb0; ok && kb < kb1;) {
+        const int end = kF32 ? min(kb + kSegment, kb1) : kb1;
+        const bool cut_here = cut && end == kb1;
+        const int whole = end - kb - (cut_here ? 1 : 0);
+        const uint32_t d = tmem_d + static_cast<uint32_t>(acc * TN);
+        ok = warp_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag, false);
+        if (!ok) {
+          report(kStatusWaitTimeout, 1, 100 + acc);
+          break;
+        }
+        uint32_t more = 0; // the accumulator holds something
+        bool seen = false;
+        for (int i = 0; i < whole; ++i) {
+          ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, seen);
+          if (!ok)
+            break;
+          tc_fence_after_sync();
+          const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
+          uint64_t *done = &sh->empty[ring.stage];
+          ring.advance(num_stages);
+          seen = warp_peek(&sh->full[ring.stage], ring.phase);
+          if (chosen) {
+            umma_ss(d, da, db, idesc, more);
 #pragma unroll
-              for (int k = 1; k < kBK / 16; ++k)
-                umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
-              more = 1;
-              umma_commit(&sh->empty[st]);
-              if (++st == num_stages) {
-                st = 0;
-                ph ^= 1;
-              }
-            }
+            for (int k = 1; k < kBK / 16; ++k)
+              umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+            umma_commit(done);
           }
-          {
-            const int at = stage + whole; // every lane keeps count
-            phase ^= static_cast<uint32_t>(at / num_stages) & 1u;
-            stage = at % num_stages;
-          }
-          if constexpr (kCut) {
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-            if (ok && cut_here) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag)) != 0;
-              if (!ok) {
-                report(kStatusWaitTimeout, 1, stage);
-                break;
-              }
+          __syncwarp();
+          more = 1;
+        }
+        if constexpr (kCut) {
+          if (ok && cut_here) {
+            ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, false);
+            if (ok) {
               // rows [live, steps * 16) belong to the next expert or to nobody
-              uint8_t *a_tile = tiles + stage * C::kStageBytes;
+              uint8_t *a_tile = tiles + ring.stage * C::kStageBytes;
               const int steps = (live + 15) / 16;
               const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
               const int chunks = kTileP / 64 + p.tile_q / 64;
@@ -296,27 +291,30 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               }
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0) {
+              if (chosen) {
                 tc_fence_after_sync();
-                const uint64_t da = da0 + static_cast<uint64_t>(stage) * kStep, db = db0 + static_cast<uint64_t>(stage) * kStep;
+                const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
                 for (int k = 0; k < steps; ++k, more = 1)
                   umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, more);
-                umma_commit(&sh->empty[stage]);
+                umma_commit(&sh->empty[ring.stage]);
               }
-              if (++stage == num_stages) {
-                stage = 0;
-                phase ^= 1;
-              }
+              __syncwarp();
+              ring.advance(num_stages);
             }
           }
-          if (ok && lane == 0)
-            umma_commit(&sh->tfull[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
-          kb = end;
         }
+        if (!ok) {
+          report(kStatusWaitTimeout, 1, ring.stage);
+          break;
+        }
+        if (chosen)
+          umma_commit(&sh->tfull[acc]);
+        __syncwarp();
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+        kb = end;
       }
     }
   } else {
