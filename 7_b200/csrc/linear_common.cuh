@@ -519,38 +519,87 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
   __syncwarp();
 }
 
-// Tokens as columns: v[j] is feature `lane0 + lane` of token q0 + j * step; a
-// warp's store of one token covers 32 neighbouring features.
+// Tokens as columns: v[j] is feature `lane0 + lane` of token q0 + j.  A few tokens
+// are stored as they are, 32 neighbouring features to a store; more change places
+// in the warp's slot (a token to a row) and leave as 16-byte pieces.
 template <bool kF32, int W>
-__device__ __forceinline__ void epilogue_columns(const LinearParams &p, const EpiTile &t, int q0, int step,
-                                                 float (&v)[W], float bias, int lane) {
+__device__ __forceinline__ void epilogue_columns(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
+                                                 float bias, uint8_t *slot, int lane) {
   const int n = t.lane0 + lane;
-  if (n >= t.lane_end)
-    return;
+  const int tokens = min(W, t.q_end - q0), features = min(32, t.lane_end - t.lane0);
+  if (tokens <= 0 || features <= 0)
+    return; // the same for the whole warp
+  const bool staged = W > 8 && tokens > 8;
 #pragma unroll
   for (int j = 0; j < W; ++j)
     v[j] += bias;
-  if (p.Z) {
+  if (staged) {
+    // the lane's place in row j of the slot
+    auto place = [&](int elem, int j) {
+      return elem == 4 ? Slot<4, 32>::at(j, lane >> 2) + (lane & 3) * 4 : Slot<2, 32>::at(j, lane >> 3) + (lane & 7) * 2;
+    };
+    if (p.Z) {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (q0 + j * step < t.q_end)
-        static_cast<uint16_t *>(p.Z)[static_cast<long long>(q0 + j * step) * p.ldz + n] = to_16bit(v[j], p.is_bf16);
+      for (int j = 0; j < W; ++j)
+        *reinterpret_cast<uint16_t *>(slot + place(2, j)) = to_16bit(v[j], p.is_bf16);
+      __syncwarp();
+      slot_to_global<2, 32>(slot, static_cast<uint16_t *>(p.Z) + static_cast<long long>(q0) * p.ldz + t.lane0, p.ldz, tokens,
+                            features, p.vec_z != 0, lane);
+      __syncwarp();
+    }
+    apply_act<W>(v, p.act);
+    if (p.R) {
+      using S = Slot<2, 32>;
+      uint4 res[4];
+      global_to_regs<32>(res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(q0) * p.ldr + t.lane0, p.ldr,
+                         tokens, features, p.vec_r != 0, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4 *>(slot + S::at(lane / 4 + i * 8, lane % 4)) = res[i];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        v[j] += from_16bit(*reinterpret_cast<const uint16_t *>(slot + place(2, j)), p.is_bf16);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if constexpr (kF32)
+        *reinterpret_cast<float *>(slot + place(4, j)) = v[j];
+      else
+        *reinterpret_cast<uint16_t *>(slot + place(2, j)) = to_16bit(v[j], p.is_bf16);
+    }
+    __syncwarp();
+    uint8_t *base = static_cast<uint8_t *>(p.D) + (static_cast<long long>(q0) * p.ldd + t.lane0) * (kF32 ? 4 : 2);
+    slot_to_global<kF32 ? 4 : 2, 32>(slot, base, p.ldd, tokens, features, p.vec_d != 0, lane);
+    __syncwarp();
+    return;
+  }
+  if (lane >= features)
+    return;
+  if (p.Z) {
+    uint16_t *z = static_cast<uint16_t *>(p.Z) + static_cast<long long>(q0) * p.ldz + n;
+#pragma unroll
+    for (int j = 0; j < W && j < 8; ++j, z += p.ldz)
+      if (j < tokens)
+        *z = to_16bit(v[j], p.is_bf16);
   }
   apply_act<W>(v, p.act);
   if (p.R) {
+    const uint16_t *r = static_cast<const uint16_t *>(p.R) + static_cast<long long>(q0) * p.ldr + n;
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (q0 + j * step < t.q_end)
-        v[j] += from_16bit(static_cast<const uint16_t *>(p.R)[static_cast<long long>(q0 + j * step) * p.ldr + n], p.is_bf16);
+    for (int j = 0; j < W && j < 8; ++j, r += p.ldr)
+      if (j < tokens)
+        v[j] += from_16bit(*r, p.is_bf16);
   }
+  uint8_t *d = static_cast<uint8_t *>(p.D) + (static_cast<long long>(q0) * p.ldd + n) * (kF32 ? 4 : 2);
 #pragma unroll
-  for (int j = 0; j < W; ++j)
-    if (q0 + j * step < t.q_end) {
-      const long long at = static_cast<long long>(q0 + j * step) * p.ldd + n;
+  for (int j = 0; j < W && j < 8; ++j, d += p.ldd * (kF32 ? 4 : 2))
+    if (j < tokens) {
       if constexpr (kF32)
-        static_cast<float *>(p.D)[at] = v[j];
+        *reinterpret_cast<float *>(d) = v[j];
       else
-        static_cast<uint16_t *>(p.D)[at] = to_16bit(v[j], p.is_bf16);
+        *reinterpret_cast<uint16_t *>(d) = to_16bit(v[j], p.is_bf16);
     }
 }
 __device__ __forceinline__ float column_bias(const LinearParams &p, const EpiTile &t, int lane) {

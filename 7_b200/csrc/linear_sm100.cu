@@ -367,7 +367,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int j = 0; j < W; j += 4)
             part[(c + j) / 4 * kTileP] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else if constexpr (kSwap) {
-          epilogue_columns<kF32, W>(p, t, w.q0 + c, 1, v, col_bias, lane);
+          epilogue_columns<kF32, W>(p, t, w.q0 + c, v, col_bias, slot, lane);
         } else {
           epilogue_rows<kF32, W>(p, t, w.q0 + c, v, f, slot, lane);
         }
@@ -495,7 +495,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int i = rank + half * splits; i * 4 < live; i += kColGroups * splits) {
             const float4 f = four(i * 4);
             float v[4] = {f.x, f.y, f.z, f.w};
-            epilogue_columns<kF32, 4>(p, t, w.q0 + i * 4, 1, v, col_bias, lane);
+            epilogue_columns<kF32, 4>(p, t, w.q0 + i * 4, v, col_bias, slot, lane);
           }
         } else {
           constexpr int V = 16; // columns at a time

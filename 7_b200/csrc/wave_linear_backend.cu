@@ -180,18 +180,96 @@ int operand_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_cols, i
   return wave::make_tensor_map_16bit(map, is_bf16, o.ptr, 3, dims, strides, box);
 }
 
-// Tile choice of one product.  `tokens` rows over `matrices` experts (grouped)
-// or all with one matrix; P x Q and the contraction as in LinearParams.
+// ------------------------------------------------------------ tile choice
+// What a launch takes is predicted for every tile and split it could have, and
+// the cheapest is taken.  Times in us, fitted to 140 problems (1 to 8192 tokens,
+// 256 to 16384 features, the three products, inputs in turn out of L2 and DRAM),
+// each timed in every variant: the choice is 0.5 % slower than the best variant
+// on average and 9 % at worst.
+//   base    launch, first loads, the last tile's epilogue
+//   stage   64 of the contraction of one tile with nothing else in the way
+//   epi     a tile's epilogue, which hides behind the next tile's stages
+struct TileCost {
+  int tile; // columns; 512: CTA pair, 256 x 256
+  double base, stage, epi;
+};
+constexpr TileCost kTileCosts[] = {{16, 3.28, 0.23, 0.35},  {32, 4.02, 0.21, 1.1},   {64, 5.36, 0.19, 0.97},
+                                   {128, 5.79, 0.30, 1.33}, {256, 7.23, 0.52, 1.84}, {512, 8.58, 0.29, 3.4}};
+constexpr int kPairTile = 512;
+constexpr double kL2BytesPerUs = 12.6e6; // all SMs together
+constexpr double kSplitCost = 1.9;       // the cluster's barriers and the sum over its CTAs, + 0.06 for each
+// CTAs that run side by side in clusters of a size (an SM each): clusters do not
+// straddle the GPCs, whose SMs are no multiple of every size (measured with
+// cudaOccupancyMaxActiveClusters; 148 SMs).
+constexpr int kClusterFit[wave::kLinearMaxSplits + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+
 struct Plan {
   LinearLaunch launch;
   int tile_q, p_blocks, q_blocks, raster, splits, stages;
 };
 
-int tile_for(int want) {
-  for (int t : {16, 32, 64, 128})
-    if (want <= t)
-      return t;
-  return 128;
+// A product's extents as the tiles see them.
+struct Extents {
+  Product kind;
+  bool grouped;
+  long long M;     // tokens
+  int matrices, N, K;
+  long long p, q, k; // k: of one tile, an expert's share of the rows for its weight gradient
+};
+
+struct Candidate {
+  int tile, tile_q, splits;
+  bool swap;
+  long long pb, qb, tiles; // tiles: as many as the launch has to provide for
+  double us;
+};
+
+// Blocks of `rows` tokens: at most / about.
+long long row_blocks_most(const Extents &e, int rows) {
+  return e.grouped ? e.M / rows + (e.matrices < e.M ? e.matrices : e.M) : (e.M + rows - 1) / rows;
+}
+double row_blocks_about(const Extents &e, int rows) {
+  if (!e.grouped)
+    return static_cast<double>((e.M + rows - 1) / rows);
+  const double experts = static_cast<double>(e.matrices < e.M ? e.matrices : e.M);
+  const double each = static_cast<double>(e.M) / experts / rows;
+  return experts * (each + 0.5 > 1.0 ? each + 0.5 : 1.0);
+}
+
+void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
+  const bool pair = t.tile == kPairTile;
+  const int tile_p = pair ? 256 : 128, tile_n = pair ? 256 : t.tile;
+  c->pb = (e.p + tile_p - 1) / tile_p;
+  c->qb = (e.q + c->tile_q - 1) / c->tile_q;
+  double about;
+  if (e.kind == Product::kWeightGrad) {
+    c->tiles = c->pb * c->qb * e.matrices;
+    about = static_cast<double>(c->tiles);
+  } else if (c->swap) {
+    c->tiles = c->pb * row_blocks_most(e, c->tile_q);
+    about = static_cast<double>(c->pb) * row_blocks_about(e, c->tile_q);
+  } else {
+    c->tiles = c->qb * row_blocks_most(e, tile_p);
+    about = static_cast<double>(c->qb) * row_blocks_about(e, tile_p);
+  }
+  const double fit = (pair ? sms / 2 : sms * (kClusterFit[c->splits] / 148.0));
+  const double ctas = about * c->splits, side = ctas < fit ? ctas : fit;
+  // (experts' tiles are dealt over the CTAs unevenly enough that half a round is not a whole one)
+  const double rounds = e.grouped && ctas > fit ? ctas / fit + 0.5 : static_cast<double>(static_cast<long long>((ctas + fit - 1e-6) / fit));
+  const long long k_iters = (e.k + 63) / 64;
+  const double mine = static_cast<double>((k_iters + c->splits - 1) / c->splits);
+  const double bytes = (tile_p + c->tile_q) * 128.0;
+  double stage = t.stage * c->tile_q / tile_n;
+  if (stage < 0.18) // the issue of a stage
+    stage = 0.18;
+  if (stage < bytes * side / kL2BytesPerUs)
+    stage = bytes * side / kL2BytesPerUs;
+  const double epi = t.epi * c->tile_q / tile_n;
+  const double each = mine * stage;
+  if (c->splits == 1)
+    c->us = t.base + rounds * (each > epi ? each : epi);
+  else
+    c->us = t.base + kSplitCost + 0.06 * c->splits + rounds * each + (rounds - 1.0) * (t.base - 1.0);
 }
 
 Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
@@ -203,110 +281,94 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   l.b_mn = kind != Product::kForward;
   l.out_f32 = out_f32;
   l.pdl = env.linear_pdl;
-  const long long M = d.tokens;
-  const int N = d.out_features, K = d.in_features;
-  const long long per_expert = (M + s.matrices - 1) / s.matrices;
-  // Few tokens: the weights on the 128 rows of the tile, the tokens on its columns.
-  l.swap = kind == Product::kForward && per_expert <= (s.grouped ? 64 : 128);
-  if (env.linear_swap >= 0 && kind == Product::kForward)
-    l.swap = env.linear_swap;
-  long long p_ext, q_ext, k_ext;
-  if (kind == Product::kForward) {
-    p_ext = l.swap ? N : M;
-    q_ext = l.swap ? M : N;
-    k_ext = K;
-  } else if (kind == Product::kInputGrad) {
-    p_ext = M;
-    q_ext = K;
-    k_ext = N;
-  } else {
-    p_ext = N;
-    q_ext = K;
-    k_ext = s.grouped ? per_expert : M;
-  }
-  const long long k_iters = (k_ext + 63) / 64;
-  auto blocks = [&](int tile_q, long long *pb, long long *qb) -> long long {
-    *pb = (p_ext + 127) / 128;
-    *qb = (q_ext + tile_q - 1) / tile_q;
-    long long tiles;
-    if (kind == Product::kWeightGrad)
-      tiles = *pb * *qb * s.matrices;
-    else if (!s.grouped)
-      tiles = *pb * *qb;
-    else if (l.swap) // an upper bound: every expert may add a ragged block
-      tiles = *pb * (M / tile_q + (s.matrices < M ? s.matrices : M));
-    else
-      tiles = *qb * (M / 128 + (s.matrices < M ? s.matrices : M));
-    return tiles;
+  Extents e{kind, s.grouped, d.tokens, s.matrices, d.out_features, d.in_features, 0, 0, 0};
+  const long long per_expert = (e.M + s.matrices - 1) / s.matrices;
+  Candidate best{};
+  best.us = -1.0;
+  auto consider = [&](const TileCost &t, bool swap, int splits, int tile_q) {
+    Candidate c{};
+    c.tile = t.tile;
+    c.swap = swap;
+    c.splits = splits;
+    c.tile_q = tile_q;
+    predict(e, t, sms, &c);
+    // a split launch has a cluster for every tile there could be
+    if (splits > 1 && !env.linear_splits && c.tiles * splits > 2ll * kClusterFit[splits])
+      return;
+    if (best.us < 0.0 || c.us < best.us)
+      best = c;
   };
-  long long pb = 0, qb = 0, tiles = 0;
-  if (l.swap) {
-    const long long want = s.grouped ? 2 * per_expert : M;
-    l.tile_n = tile_for(static_cast<int>(want < 128 ? (want < M ? want : M) : 128));
-    if (env.linear_tile && env.linear_tile <= 128)
-      l.tile_n = env.linear_tile;
-    pl.tile_q = l.tile_n;
-    if (!s.grouped) // no columns of padding beyond the multiple of 16
-      pl.tile_q = static_cast<int>(round_up((M + (M + l.tile_n - 1) / l.tile_n - 1) / ((M + l.tile_n - 1) / l.tile_n), 16));
-    tiles = blocks(pl.tile_q, &pb, &qb);
-  } else {
-    l.tile_n = 64;
-    for (int t : {256, 128}) {
-      if (t == 256 && out_f32)
+  // Tokens as columns pay while they leave rows of the tensor core's tile empty
+  // otherwise; beyond two tiles of them the two ways are the same.
+  const bool may_swap = kind == Product::kForward && env.linear_swap != 0 && (env.linear_swap == 1 || per_expert <= 256);
+  const bool may_rows = kind != Product::kForward || (env.linear_swap != 1 && (env.linear_swap == 0 || per_expert > 16));
+  for (int swap = may_rows ? 0 : 1; swap <= (may_swap ? 1 : 0); ++swap) {
+    e.p = kind == Product::kForward ? (swap ? e.N : e.M) : kind == Product::kInputGrad ? e.M : e.N;
+    e.q = kind == Product::kForward ? (swap ? e.M : e.N) : e.K;
+    e.k = kind == Product::kForward ? e.K : kind == Product::kInputGrad ? e.N : (s.grouped ? per_expert : e.M);
+    for (const TileCost &t : kTileCosts) {
+      const bool pair = t.tile == kPairTile;
+      const int tile_n = pair ? 256 : t.tile;
+      if (swap ? t.tile > 128 : t.tile < 64)
         continue;
-      if (blocks(t, &pb, &qb) >= sms * (t == 256 ? 1 : 1) && q_ext > t / 2) {
-        l.tile_n = t;
-        break;
+      if (out_f32 && t.tile > 128)
+        continue;
+      // the knobs take what they can of their choice
+      if (pair ? env.linear_pair == 0 || env.linear_splits > 1 || swap : env.linear_pair == 1 && !out_f32 && !swap)
+        continue;
+      const int knob = env.linear_tile;
+      if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
+        continue;
+      // columns of no use are left out where the layout allows: tiles of equal width
+      const int unit = l.b_mn ? (pair ? 128 : 64) : (pair ? 32 : 16);
+      int tile_q = tile_n;
+      if (!(swap && s.grouped)) {
+        const long long n = (e.q + tile_n - 1) / tile_n;
+        tile_q = static_cast<int>(round_up((e.q + (n > 0 ? n : 1) - 1) / (n > 0 ? n : 1), unit));
+        tile_q = tile_q > tile_n ? tile_n : tile_q < unit ? unit : tile_q;
       }
+      if (swap && !knob && t.tile > 16 && tile_q <= t.tile / 2)
+        continue; // the next smaller tile does it
+      if (env.linear_splits > 0) {
+        consider(t, swap, pair ? 1 : env.linear_splits, tile_q);
+        continue;
+      }
+      for (int c : {1, 2, 3, 4, 6, 8})
+        if (c == 1 || (!pair && t.tile < 256 && (e.k + 63) / 64 >= 2 * c && (swap || tile_q / 16 >= c)))
+          consider(t, swap, c, tile_q);
     }
-    if (l.tile_n == 64 && q_ext > 64)
-      l.tile_n = 128;
-    if (env.linear_tile && env.linear_tile >= 64 && !(out_f32 && env.linear_tile == 256))
-      l.tile_n = env.linear_tile;
-    pl.tile_q = l.tile_n;
-    tiles = blocks(pl.tile_q, &pb, &qb);
   }
-  if (!l.swap && !out_f32 && env.linear_pair != 0 && !env.linear_splits) {
+  if (best.us < 0.0) { // knobs that exclude one another
+    e.p = kind == Product::kWeightGrad ? e.N : e.M;
+    e.q = kind == Product::kForward ? e.N : e.K;
+    consider(kTileCosts[3], false, 1, 128);
+  }
+  l.swap = best.swap;
+  l.pair = best.tile == kPairTile;
+  l.tile_n = l.pair ? 256 : best.tile;
+  pl.tile_q = best.tile_q;
+  pl.splits = best.splits;
+  pl.p_blocks = static_cast<int>(best.pb);
+  pl.q_blocks = static_cast<int>(best.qb);
+  // 2048 rows of tiles share their columns' panel
+  pl.raster = l.pair ? 8 : 16;
+  if (l.pair) {
     const long long pairs = sms / 2;
-    const long long p_pair = (p_ext + 255) / 256, q_pair = (q_ext + 255) / 256;
-    const long long pair_tiles = kind == Product::kWeightGrad ? p_pair * q_pair * s.matrices
-                                 : s.grouped ? q_pair * (M / 256 + (s.matrices < M ? s.matrices : M)) : p_pair * q_pair;
-    if ((pair_tiles >= pairs && per_expert >= 256) || env.linear_pair == 1) {
-      l.pair = 1;
-      l.tile_n = pl.tile_q = 256;
-      pb = p_pair;
-      qb = q_pair;
-      tiles = pair_tiles;
-      pl.raster = 8;
-      pl.splits = 1;
-      pl.p_blocks = static_cast<int>(pb);
-      pl.q_blocks = static_cast<int>(qb);
-      l.grid = static_cast<int>(2 * (tiles < pairs ? (tiles > 0 ? tiles : 1) : pairs));
-      return pl;
-    }
+    l.grid = static_cast<int>(2 * (best.tiles < pairs ? (best.tiles > 0 ? best.tiles : 1) : pairs));
+    pl.stages = 6; // (the kernel's own constant)
+    return pl;
   }
-  // Few tiles: a cluster of CTAs shares a tile's contraction.
-  pl.splits = 1;
-  if (tiles > 0)
-    for (int c : {8, 4, 2})
-      if (tiles * c <= sms && k_iters / c >= 2 && (l.swap || pl.tile_q / 16 >= c)) {
-        pl.splits = c;
-        break;
-      }
-  if (env.linear_splits > 0 && tiles * env.linear_splits <= 65535)
-    pl.splits = env.linear_splits;
-  pl.p_blocks = static_cast<int>(pb);
-  pl.q_blocks = static_cast<int>(qb);
-  pl.raster = 16;
-  l.grid = static_cast<int>(pl.splits > 1 ? tiles * pl.splits : (tiles < sms ? tiles : sms));
+  l.grid = static_cast<int>(pl.splits > 1 ? best.tiles * pl.splits : (best.tiles < sms ? best.tiles : sms));
   if (l.grid < 1)
-    l.grid = 1;
+    l.grid = pl.splits;
   // A CTA with one tile takes no more stages than that has: what it leaves of the
-  // SM lets the next kernel of the stream set itself up meanwhile.
+  // SM lets the next kernel of the stream set itself up meanwhile (one token,
+  // 2048 x 2048: 12.3 -> 6.5 us).
   pl.stages = wave::linear_max_stages(l.tile_n, l.out_f32);
   if (kind != Product::kWeightGrad || !s.grouped) {
-    const long long need = (k_iters + pl.splits - 1) / pl.splits;
-    if ((pl.splits > 1 || tiles <= sms) && need < pl.stages)
+    const long long k_ext = kind == Product::kForward ? e.K : kind == Product::kInputGrad ? e.N : e.M;
+    const long long need = ((k_ext + 63) / 64 + pl.splits - 1) / pl.splits;
+    if ((pl.splits > 1 || best.tiles <= sms) && need < pl.stages)
       pl.stages = need < 4 ? 4 : static_cast<int>(need);
   }
   return pl;
@@ -452,6 +514,21 @@ int wave_cuda_linear_workspace_bytes(const wave_linear_desc *d, int backward, si
     return rc;
   const BackwardLayout b = backward_layout(s, sms);
   *bytes = b.dz_bytes + b.partial_bytes + b.x_bytes + b.w_bytes;
+  return WAVE_OK;
+}
+
+int wave_cuda_linear_plan_for_sms(const wave_linear_desc *d, int product, int sm_count, wave_linear_plan *plan) {
+  const int rc = validate(d);
+  if (rc != WAVE_OK)
+    return rc;
+  if (product < 0 || product > 2 || sm_count < 2 || !plan)
+    return fail(WAVE_E_INVALID, "product must be 0 (forward), 1 (input gradient) or 2 (weight gradient), sm_count at least 2 "
+                                "and the result pointer non-null; got product=%d, sm_count=%d", product, sm_count);
+  const Shape s = resolve(*d);
+  const Product kind = product == 0 ? Product::kForward : product == 1 ? Product::kInputGrad : Product::kWeightGrad;
+  const bool f32 = product == 0 ? d->y_type == WAVE_F32 : product == 2 && d->dweight_type == WAVE_F32;
+  const Plan pl = plan_product(kind, s, f32, sm_count);
+  *plan = wave_linear_plan{pl.launch.pair ? 256 : 128, pl.tile_q, pl.launch.swap, pl.splits, pl.launch.grid, pl.stages};
   return WAVE_OK;
 }
 

@@ -49,6 +49,10 @@ class LinearDesc(C.Structure):
             "ldx", "ldw", "ldy", "ldr", "ldz", "lddx", "lddw", "expert_stride_w", "expert_stride_dw")]
 
 
+class LinearPlan(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("tile_rows", "tile_columns", "tokens_on_columns", "splits", "grid", "stages")]
+
+
 EXPORTS = [
     "wave_cuda_last_error", "wave_cuda_version", "wave_cuda_reload_env",
     "_mlir_ciface_wave_memref_to_ptr_global_i32", "_mlir_ciface_wave_memref_to_ptr_global_i8",
@@ -60,7 +64,7 @@ EXPORTS = [
     "wave_cuda_gemm_plan", "wave_cuda_gemm_plan_for_sms", "wave_cuda_gemm_streamk_static", "wave_cuda_fa_validate", "wave_cuda_flash_attention_fwd",
     "wave_cuda_flash_attention_fwd_multi_output", "wave_cuda_flash_attention_fwd_multicast_output",
     "wave_cuda_flash_attention_fwd_host", "wave_cuda_linear_desc_init", "wave_cuda_linear_validate",
-    "wave_cuda_linear_workspace_bytes", "wave_cuda_linear_fwd", "wave_cuda_linear_bwd", "wave_cuda_module_get_function", "wave_cuda_launch",
+    "wave_cuda_linear_workspace_bytes", "wave_cuda_linear_plan_for_sms", "wave_cuda_linear_fwd", "wave_cuda_linear_bwd", "wave_cuda_module_get_function", "wave_cuda_launch",
     "wave_cuda_function_release", "wave_cuda_check_device_status",
     # include/wave_mgpu.h: the wrappers a host module lowered by gpu-to-llvm calls
     "wave_cuda_module_blob_bytes", "wave_cuda_module_blob_write", "wave_cuda_mgpu_status", "wave_cuda_memref_region",
@@ -114,6 +118,7 @@ def lib() -> C.CDLL:
     L.wave_cuda_linear_desc_init.restype = None
     L.wave_cuda_linear_validate.argtypes = [C.POINTER(LinearDesc)]
     L.wave_cuda_linear_workspace_bytes.argtypes = [C.POINTER(LinearDesc), C.c_int, C.POINTER(C.c_size_t)]
+    L.wave_cuda_linear_plan_for_sms.argtypes = [C.POINTER(LinearDesc), C.c_int, C.c_int, C.POINTER(LinearPlan)]
     L.wave_cuda_linear_fwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 9
     L.wave_cuda_linear_bwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 10
     L.wave_cuda_module_get_function.argtypes = [C.c_char_p, vp, C.POINTER(vp)]
@@ -283,6 +288,13 @@ def linear_workspace_bytes(desc: LinearDesc, backward: bool) -> int:
     n = C.c_size_t(0)
     check(lib().wave_cuda_linear_workspace_bytes(C.byref(desc), int(backward), C.byref(n)))
     return n.value
+
+
+def linear_plan_for_sms(desc: LinearDesc, product: int, sm_count: int) -> dict:
+    """The tiles of one product (0 forward, 1 input gradient, 2 weight gradient) on a GPU of `sm_count` SMs."""
+    plan = LinearPlan()
+    check(lib().wave_cuda_linear_plan_for_sms(C.byref(desc), product, sm_count, C.byref(plan)))
+    return {n: getattr(plan, n) for n, _ in LinearPlan._fields_}
 
 
 def check_device_status() -> None:

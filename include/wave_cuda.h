@@ -350,6 +350,15 @@ int wave_cuda_linear_validate(const wave_linear_desc *desc); /* needs no GPU */
 /* Device workspace of a call (16-byte aligned; may be NULL when 0).  The forward
  * pass needs one only for operands that have to be laid out. */
 int wave_cuda_linear_workspace_bytes(const wave_linear_desc *desc, int backward, size_t *bytes);
+/* The tiles of one product (0 forward, 1 input gradient, 2 weight gradient) on a
+ * GPU of `sm_count` SMs that need not be present.  For planning tools and tests. */
+typedef struct wave_linear_plan {
+  int tile_rows, tile_columns; /* of the tensor core's tile; 256 rows: a pair of CTAs */
+  int tokens_on_columns;       /* forward with few tokens: features on the tile's rows */
+  int splits;                  /* CTAs of a cluster that share a tile's contraction */
+  int grid, stages;
+} wave_linear_plan;
+int wave_cuda_linear_plan_for_sms(const wave_linear_desc *desc, int product, int sm_count, wave_linear_plan *plan);
 /* bias, residual and Z (the pre-activation, io_type) may be NULL; offsets is
  * read only with experts; experts take no residual. */
 int wave_cuda_linear_fwd(const wave_linear_desc *desc, const void *X, const void *W, const void *bias,

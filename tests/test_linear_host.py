@@ -122,3 +122,52 @@ def test_python_refuses_cpu_tensors(wl):
             call()
     with pytest.raises(ValueError, match="offsets must be given"):
         wl.grouped_linear(x, w[None], None)
+
+
+@pytest.mark.parametrize("knobs", [{}, dict(TILE=16), dict(TILE=256, SWAP=1), dict(SPLITS=5), dict(PAIR=1), dict(PAIR=0, SWAP=0),
+                                   dict(PAIR=1, SWAP=1, TILE=64), dict(PAIR=1, SPLITS=8)])
+def test_every_plan_can_run(wc, knobs):
+    """Whatever the sizes: a tile the kernels have, whole clusters, a ring of at least four stages, a block for every tile."""
+    import math
+    import random
+
+    from _util import env_knobs
+
+    rng = random.Random(7)
+    size = lambda hi: int(math.exp(rng.uniform(0, math.log(hi))))  # noqa: E731
+    with env_knobs(wc, **{f"WAVE_CUDA_LINEAR_{k}": v for k, v in knobs.items()}):
+        for _ in range(400):
+            m, n, k = size(200000), size(40000), size(40000)
+            d = desc(wc, m if rng.random() > 0.02 else 0, n, k, experts=rng.choice([0, size(1024)]))
+            if rng.random() < 0.3:
+                d.y_type = d.dweight_type = wc.F32
+            for product in range(3):
+                sms = rng.choice([2, 16, 100, 132, 148])
+                p = wc.linear_plan_for_sms(d, product, sms)
+                pair = p["tile_rows"] == 256
+                f32 = product != 1 and d.y_type == wc.F32
+                unit = (128 if pair else 64) if product else (32 if pair else 16)
+                assert p["tile_columns"] % unit == 0 and unit <= p["tile_columns"] <= (128 if f32 else 256), (m, n, k, p)
+                assert 1 <= p["splits"] <= 8 and p["grid"] >= 1 and p["grid"] % p["splits"] == 0
+                assert 4 <= p["stages"] <= 12
+                assert not pair or (p["splits"] == 1 and p["grid"] % 2 == 0 and not p["tokens_on_columns"] and not f32)
+                assert not p["tokens_on_columns"] or (product == 0 and p["tile_columns"] <= 128)
+                if p["splits"] > 1:  # one cluster to a tile
+                    rows, cols = p["tile_rows"], p["tile_columns"]
+                    up = lambda a, b: -(-a // b)  # noqa: E731
+                    P, Q = [((n, d.tokens) if p["tokens_on_columns"] else (d.tokens, n)), (d.tokens, k), (n, k)][product]
+                    if not d.experts:
+                        tiles = up(P, rows) * up(Q, cols)
+                    elif product == 2:
+                        tiles = up(P, rows) * up(Q, cols) * d.experts
+                    else:
+                        tokens, other = (cols, up(P, rows)) if p["tokens_on_columns"] else (rows, up(Q, cols))
+                        # experts that each have one token more than whole tiles
+                        tiles = other * max((d.tokens - e) // tokens + e for e in range(min(d.experts, d.tokens) + 1))
+                    assert p["grid"] >= tiles * p["splits"], (m, n, k, p)
+
+
+def test_plan_refusals(wc):
+    for product, sms in ((-1, 148), (3, 148), (0, 1)):
+        with pytest.raises(wc.WaveCudaError, match="product must be"):
+            wc.linear_plan_for_sms(desc(wc), product, sms)
