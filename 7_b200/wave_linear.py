@@ -29,19 +29,43 @@ def _types():
     return torch, {torch.bfloat16: wc.BF16, torch.float16: wc.F16, torch.float32: wc.F32}
 
 
-@functools.lru_cache(maxsize=4096)
-def _plan(device: int, backward: bool, *fields):
-    """A descriptor (a pure function of sizes, strides and types) and the bytes
-    of workspace a call with it takes on that device."""
-    desc = wc.LinearDesc(*fields)
-    try:
-        wc.linear_validate(desc)
-        need = wc.linear_workspace_bytes(desc, backward)
-    except wc.WaveCudaError as err:
-        if err.code in (wc.E_INVALID, wc.E_UNSUPPORTED):
-            raise ValueError(err.message) from None
-        raise
-    return desc, C.byref(desc), need
+class _Plan:
+    """What a call makes of its tensors' shapes, strides and types: the
+    descriptor, the bytes of workspace and the results' shapes and types.
+    Everything here is a function of those alone and is checked once for each
+    combination of them; addresses and contents are looked at in every call."""
+    __slots__ = ("desc", "ref", "need", "device", "index", "outs")
+
+    def __init__(self, device, backward: bool, fields, outs):
+        self.desc = wc.LinearDesc(*fields)
+        self.ref = C.byref(self.desc)
+        self.device, self.index, self.outs = device, device.index, outs
+        with _types()[0].cuda.device(device):  # the workspace goes by the device's SMs
+            try:
+                wc.linear_validate(self.desc)
+                self.need = wc.linear_workspace_bytes(self.desc, backward)
+            except wc.WaveCudaError as err:
+                if err.code in (wc.E_INVALID, wc.E_UNSUPPORTED):
+                    raise ValueError(err.message) from None
+                raise
+
+
+_plans: dict = {}
+
+
+def _remember(key, plan):
+    if len(_plans) >= 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _matrix(t, name: str, rows: int, cols: int, dtypes, device):
@@ -116,33 +140,20 @@ def _aligned(t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-class _On:
-    """The tensors' device made current (its streams and the library's launches
-    go by the current device), and its current stream."""
-
-    def __init__(self, torch, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-        self.torch, self.device = torch, device
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(plan, call):
+    """Runs `call(workspace, stream)` with the tensors' device current (the
+    library launches on the current device) on its current stream."""
+    torch, _ = _types()
+    if torch.cuda.current_device() != plan.index:
+        with torch.cuda.device(plan.device):
+            return _launch(plan, call)
+    ws = torch.empty(plan.need, dtype=torch.uint8, device=plan.device) if plan.need else None
+    wc.check(call(_ptr(ws), torch._C._cuda_getCurrentRawStream(plan.index)))
 
 
-def _forward(x, weight, offsets, bias, residual, activation, out, out_dtype, save):
+def _plan_forward(x, weight, offsets, bias, residual, activation, out, out_dtype):
     torch, types, device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
     io = x.dtype
-    x, weight = (t if t.data_ptr() % 16 == 0 else _aligned(t) for t in (x, weight))
-    ldx = ldx if tokens <= 1 else x.stride(0)
-    if weight.stride(-1) == 1 and n > 1:
-        ldw = weight.stride(-2)
-    if experts > 1:
-        stride_w = weight.stride(0)
     bias_type = io
     if bias is not None:
         shape = (experts, n) if offsets is not None else (n,)
@@ -158,60 +169,76 @@ def _forward(x, weight, offsets, bias, residual, activation, out, out_dtype, sav
         y_type = io if out_dtype is None else out_dtype
         if y_type not in (io, torch.float32):
             raise ValueError(f"out_dtype must be {io} or f32; got {y_type}")
-        y, zero_rest, ldy = torch.empty((tokens, n), dtype=y_type, device=device), int(offsets is not None), 0
+        zero_rest, ldy = int(offsets is not None), 0
     else:
         y_type, zero_rest = out.dtype, 0
         if out_dtype is not None and out_dtype != y_type:
             raise ValueError(f"out has dtype {y_type}, out_dtype says {out_dtype}")
-        y, ldy = out, _matrix(out, "out", tokens, n, (io, torch.float32), device)
+        ldy = _matrix(out, "out", tokens, n, (io, torch.float32), device)
+    fields = (tokens, n, k, experts, types[io], types[y_type], types[bias_type], types[io], wc.F32, _act(activation), zero_rest, 0,
+              ldx, ldw, ldy, ldr, 0, 0, 0, stride_w, 0)
+    return _Plan(device, False, fields, ((tokens, n), y_type))
+
+
+def _forward(x, weight, offsets, bias, residual, activation, out, out_dtype, save):
+    key = (x.shape, x.stride(), x.dtype, x.device, weight.shape, weight.stride(), weight.dtype, weight.device, _meta(offsets),
+           _meta(bias), _meta(residual), activation, _meta(out), out_dtype)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _plan_forward(x, weight, offsets, bias, residual, activation, out, out_dtype))
+    px, pw = x.data_ptr(), weight.data_ptr()
+    if (px | pw) & 15:
+        return _forward(_aligned(x), _aligned(weight), offsets, bias, residual, activation, out, out_dtype, save)
+    torch, _ = _types()
+    shape, y_type = plan.outs
+    y = out
+    if y is None:
+        y = x.new_empty(shape) if y_type == x.dtype else torch.empty(shape, dtype=y_type, device=plan.device)
     z = None
-    if save:
-        z = (torch.zeros if offsets is not None and not zero_rest else torch.empty)((tokens, n), dtype=io, device=device)
-    with _On(torch, device) as stream:
-        _, ref, need = _plan(device.index, False, tokens, n, k, experts, types[io], types[y_type], types[bias_type], types[io],
-                             wc.F32, _act(activation), zero_rest, 0, ldx, ldw, ldy, ldr, 0, 0, 0, stride_w, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        wc.check(wc.lib().wave_cuda_linear_fwd(
-            ref, x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
-            residual.data_ptr() if residual is not None else None, offsets.data_ptr() if offsets is not None else None,
-            y.data_ptr(), z.data_ptr() if save else None, ws.data_ptr() if need else None, stream))
+    if save:  # rows that belong to no expert are left alone with `out`
+        z = x.new_zeros(shape) if offsets is not None and out is not None else x.new_empty(shape)
+    _launch(plan, lambda ws, stream: wc.lib().wave_cuda_linear_fwd(
+        plan.ref, px, pw, _ptr(bias), _ptr(residual), _ptr(offsets), y.data_ptr(), _ptr(z), ws, stream))
     return (y, z) if save else y
 
 
-def _backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype, need_dx, need_dweight,
-              need_dbias):
+def _plan_backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype):
     torch, types, device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
     io = x.dtype
     act = _act(activation)
-    _matrix(dy, "dy", tokens, n, (io, torch.float32), device)
+    ldy = _matrix(dy, "dy", tokens, n, (io, torch.float32), device)
     ldz = 0
     if act:
         if pre_activation is None:
             raise ValueError(f"the gradient of {activation} needs the pre-activation")
         ldz = _matrix(pre_activation, "pre_activation", tokens, n, (io,), device)
-    dweight_dtype = io if dweight_dtype is None else dweight_dtype
-    for name, t in (("dweight_dtype", dweight_dtype), ("dbias_dtype", dbias_dtype or torch.float32)):
+    dweight_dtype = dweight_dtype or io
+    dbias_dtype = dbias_dtype or torch.float32
+    for name, t in (("dweight_dtype", dweight_dtype), ("dbias_dtype", dbias_dtype)):
         if t not in (io, torch.float32):
             raise ValueError(f"{name} must be {io} or f32; got {t}")
-    dbias_dtype = dbias_dtype or torch.float32
-    x, weight, dy = (t if t.data_ptr() % 16 == 0 else _aligned(t) for t in (x, weight, dy))
-    ldx, ldy = (t.stride(0) if tokens > 1 else 0 for t in (x, dy))
-    if n > 1:
-        ldw = weight.stride(-2)
-    if experts > 1:
-        stride_w = weight.stride(0)
     lead = (experts,) if offsets is not None else ()
-    dx = torch.empty((tokens, k), dtype=io, device=device) if need_dx else None
-    dw = torch.empty((*lead, n, k), dtype=dweight_dtype, device=device) if need_dweight else None
-    db = torch.empty((*lead, n), dtype=dbias_dtype, device=device) if need_dbias else None
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    with _On(torch, device) as stream:
-        _, ref, need = _plan(device.index, True, tokens, n, k, experts, types[io], types[dy.dtype], types[io],
-                             types[dweight_dtype], types[dbias_dtype], act, int(offsets is not None), 0, ldx, ldw, ldy, 0, ldz,
-                             0, 0, stride_w, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        wc.check(wc.lib().wave_cuda_linear_bwd(ref, ptr(dy), ptr(x), ptr(weight), ptr(pre_activation) if act else None,
-                                               ptr(offsets), ptr(dx), ptr(dw), ptr(db), ptr(ws), stream))
+    fields = (tokens, n, k, experts, types[io], types[dy.dtype], types[io], types[dweight_dtype], types[dbias_dtype], act,
+              int(offsets is not None), 0, ldx, ldw, ldy, 0, ldz, 0, 0, stride_w, 0)
+    return _Plan(device, True, fields, (((tokens, k), io), ((*lead, n, k), dweight_dtype), ((*lead, n), dbias_dtype)))
+
+
+def _backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype, need_dx, need_dweight,
+              need_dbias):
+    key = (_meta(dy), _meta(x), _meta(weight), _meta(offsets), activation, _meta(pre_activation), dweight_dtype, dbias_dtype)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _plan_backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype))
+    pdy, px, pw = dy.data_ptr(), x.data_ptr(), weight.data_ptr()
+    if (pdy | px | pw) & 15:
+        return _backward(_aligned(dy), _aligned(x), _aligned(weight), offsets, activation, pre_activation, dweight_dtype,
+                         dbias_dtype, need_dx, need_dweight, need_dbias)
+    torch, _ = _types()
+    dx, dw, db = (torch.empty(shape, dtype=t, device=plan.device) if need else None
+                  for need, (shape, t) in zip((need_dx, need_dweight, need_dbias), plan.outs))
+    z = _ptr(pre_activation) if plan.desc.activation else None
+    _launch(plan, lambda ws, stream: wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw),
+                                                                   _ptr(db), ws, stream))
     return dx, dw, db
 
 
