@@ -74,17 +74,33 @@ struct Tile {
   int k_begin = 0, k_len = 0; // contraction: first index (rows of the group when ragged) and length
 };
 
-// Local tile id -> (row block, column block): `raster` row blocks are walked
-// down before the next column block, so that the tiles in flight at one time
-// share panels of both operands in L2.
-__device__ __forceinline__ void raster_coords(int id, int num_r, int num_c, int raster, int &r, int &c) {
-  const int per = raster * num_c;
-  const int band = id / per;
-  const int first = band * raster;
-  const int rows = min(num_r - first, raster);
-  const int in = id - band * per;
-  r = first + in % rows;
-  c = in / rows;
+// n / d for 0 <= n < 2^31 without a division (the tiles' ids have to be taken
+// apart once in each role and tile: with the machine's divisions that took 1000
+// cycles, more than the products of a small expert).  m = ceil(2^(31+s) / d),
+// s = ceil(log2 d): m d - 2^(31+s) < d <= 2^s, so the error stays below one step.
+__device__ __forceinline__ int fast_div(int n, const FastDiv &f) {
+  return f.s == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), f.m) >> (f.s - 1));
+}
+// n / d: below 2^22 a quotient in f32 is off by one at most.
+__device__ __forceinline__ int small_div(int n, int d) {
+  if (n >= 1 << 22)
+    return n / d;
+  int q = __float2int_rz(__fdividef(static_cast<float>(n), static_cast<float>(d)));
+  const int r = n - q * d;
+  q += r >= d ? 1 : r < 0 ? -1 : 0;
+  return q;
+}
+
+// Local tile id -> (row block, column block): 2^raster_log2 row blocks are
+// walked down before the next column block, so that the tiles in flight at one
+// time share panels of both operands in L2.
+__device__ __forceinline__ void raster_coords(int id, int num_r, const LinearParams &p, int &r, int &c) {
+  const int band = fast_div(id, p.band_tiles);
+  const int first = band << p.raster_log2;
+  const int in = id - band * static_cast<int>(p.band_tiles.d);
+  const int rows = min(num_r - first, 1 << p.raster_log2);
+  c = rows == 1 << p.raster_log2 ? in >> p.raster_log2 : small_div(in, rows);
+  r = first + in - c * rows;
 }
 
 template <bool kSwap> struct TileWalk {
@@ -114,7 +130,7 @@ template <bool kSwap> struct TileWalk {
         return false;
       int rb, fb;
       const int blocks = t.blocks[g + 1] - t.blocks[g];
-      raster_coords(id - t.blocks[g] * other, blocks, other, p.raster, rb, fb);
+      raster_coords(id - t.blocks[g] * other, blocks, p, rb, fb);
       w.group = g;
       if (kSwap) {
         w.p0 = fb * tile_p;
@@ -137,7 +153,7 @@ template <bool kSwap> struct TileWalk {
     w.k_begin = 0;
     w.k_len = p.K;
     if (p.ragged == kRaggedK) {
-      w.group = id / per;
+      w.group = fast_div(id, p.group_tiles);
       if (w.group >= p.groups)
         return false;
       id -= w.group * per;
@@ -146,7 +162,7 @@ template <bool kSwap> struct TileWalk {
     } else if (id >= per) {
       return false;
     }
-    raster_coords(id, p.p_blocks, p.q_blocks, p.raster, pb, qb);
+    raster_coords(id, p.p_blocks, p, pb, qb);
     w.p0 = pb * tile_p;
     w.p_end = p.P;
     w.q0 = qb * p.tile_q;
@@ -451,20 +467,61 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
   }
 }
 
+// What an epilogue warp has of its own: its slot, 32 floats for the bias, and
+// the tensor maps of D and z (their boxes are a slot: 32 rows of 32 columns).
+//
+// Blocks leave the slot by one TMA store where they can: through the load-store
+// unit a block is read from shared memory and written to L1 a second time, which
+// bounds tiles of short sums (the f32 weight gradients of 24 experts with 29 rows
+// each: 3100 of a tile's 5500 cycles).  The store cuts what lies behind the
+// tensor's last row or column; only a block that ends at an expert's last row has
+// to be written row by row.
+struct EpiWarp {
+  uint8_t *slot;
+  float *bias;
+  const CUtensorMap *map_d, *map_z;
+  int lane;
+};
+// The slot may be written: the stores that read it have done so.
+__device__ __forceinline__ void slot_wait(const EpiWarp &e) {
+  if (e.lane == 0)
+    tma_store_wait_read<0>();
+  __syncwarp();
+}
+template <int kElem, int W>
+__device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *map, bool tma, void *base, long long ld, int rows,
+                                         int cols, bool vec, int q0, int p0, int group) {
+  if (W == 32 && tma) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (e.lane == 0) {
+      tma_store_3d(map, e.slot, q0, p0, group);
+      tma_store_commit();
+    }
+  } else {
+    __syncwarp();
+    slot_to_global<kElem, W>(e.slot, base, ld, rows, cols, vec, e.lane);
+    __syncwarp();
+  }
+}
+
 // Tokens as rows: v holds columns q0 .. q0 + W of the lane's row.
 template <bool kF32, int W>
 __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
-                                              const Ahead<W> &f, uint8_t *slot, int lane) {
+                                              const Ahead<W> &f, const EpiWarp &e) {
+  uint8_t *slot = e.slot;
+  const int lane = e.lane;
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
   if (rows <= 0 || cols <= 0)
     return; // the same for the whole warp
-  if (p.bias) { // handed round through the slot
+  const bool whole = rows == 32 || p.ragged != kRaggedRows; // no row behind these is another expert's
+  if (p.bias) { // handed round
     if (lane < W)
-      reinterpret_cast<float *>(slot)[lane] = f.bias;
+      e.bias[lane] = f.bias;
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
-      const float4 b = reinterpret_cast<const float4 *>(slot)[k];
+      const float4 b = reinterpret_cast<const float4 *>(e.bias)[k];
       const float2 lo = __fadd2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(b.x, b.y));
       const float2 hi = __fadd2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(b.z, b.w));
       v[4 * k] = lo.x;
@@ -475,13 +532,13 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
     __syncwarp();
   }
   if (p.Z) {
+    slot_wait(e);
     row_to_slot_16bit<W>(slot, v, p.is_bf16, lane);
-    __syncwarp();
-    slot_to_global<2, W>(slot, static_cast<uint16_t *>(p.Z) + static_cast<long long>(t.lane0) * p.ldz + q0, p.ldz, rows,
-                         cols, p.vec_z != 0, lane);
-    __syncwarp();
+    slot_out<2, W>(e, e.map_z, p.tma_z && whole, static_cast<uint16_t *>(p.Z) + static_cast<long long>(t.lane0) * p.ldz + q0,
+                   p.ldz, rows, cols, p.vec_z != 0, q0, t.lane0, 0);
   }
   apply_act<W>(v, p.act);
+  slot_wait(e);
   if (p.R) {
     using S = Slot<2, W>;
     constexpr int kRowStep = 32 / S::kPieces;
@@ -509,14 +566,13 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
     for (int k = 0; k < W / 4; ++k)
       *reinterpret_cast<float4 *>(slot + Slot<4, W>::at(lane, k)) =
           make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-    __syncwarp();
-    slot_to_global<4, W>(slot, static_cast<float *>(p.D) + at, p.ldd, rows, cols, p.vec_d != 0, lane);
+    slot_out<4, W>(e, e.map_d, p.tma_d && whole, static_cast<float *>(p.D) + at, p.ldd, rows, cols, p.vec_d != 0, q0, t.lane0,
+                   p.ragged == kRaggedK ? t.group : 0);
   } else {
     row_to_slot_16bit<W>(slot, v, p.is_bf16, lane);
-    __syncwarp();
-    slot_to_global<2, W>(slot, static_cast<uint16_t *>(p.D) + at, p.ldd, rows, cols, p.vec_d != 0, lane);
+    slot_out<2, W>(e, e.map_d, p.tma_d && whole, static_cast<uint16_t *>(p.D) + at, p.ldd, rows, cols, p.vec_d != 0, q0, t.lane0,
+                   p.ragged == kRaggedK ? t.group : 0);
   }
-  __syncwarp();
 }
 
 // Tokens as columns: v[j] is feature `lane0 + lane` of token q0 + j.  A few tokens

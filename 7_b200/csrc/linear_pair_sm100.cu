@@ -42,7 +42,7 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMyCols = kTN / 2; // columns of an epilogue warp
 constexpr int kW = 32;
-constexpr int kSlots = kEpiWarps * slot_bytes<false>();
+constexpr int kSlots = kEpiWarps * (slot_bytes<false>() + 32 * 4); // and the bias
 constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
 constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots;
 static_assert(kSmemFixed + kTableBytes <= 227 * 1024, "does not fit the shared memory of an SM");
@@ -80,6 +80,7 @@ __device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.ac
 template <bool kAMn, bool kBMn>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                   const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
                    const __grid_constant__ LinearParams p) {
   constexpr bool kCut = kAMn && kBMn;
   extern __shared__ uint8_t smem_raw[];
@@ -312,12 +313,23 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const int quarter = warp & 3;
     const int col0 = ((warp - 2) >> 2) * kMyCols;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint8_t *slot = slots + (warp - 2) * slot_bytes<false>();
+    const EpiWarp ew{slots + (warp - 2) * slot_bytes<false>(),
+                     reinterpret_cast<float *>(slots + kEpiWarps * slot_bytes<false>()) + (warp - 2) * 32, &tm_d, &tm_z, lane};
     const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
     TileWalk<false> walk(p, table, kPairP);
     Tile w;
     int acc = 0;
     uint32_t acc_phase = 0;
+    auto release = [&]() {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive_cluster(tempty_leader[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    };
     for (int id = first_tile; walk.get(id, w); id += tile_step) {
       const bool empty = w.k_len <= 0; // nothing to multiply: the epilogue of zero
       EpiTile t;
@@ -352,22 +364,18 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           for (int j = 0; j < kW; ++j)
             v[j] = __uint_as_float(r[j]);
         }
+        if (!empty && c + kW >= my_cols)
+          release(); // read out: the tile after the next may use it
         const Ahead<kW> now = next;
         if (c + kW < my_cols)
           fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + kW, lane);
-        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, now, slot, lane);
+        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, now, ew);
       }
-      if (!empty) {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive_cluster(tempty_leader[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
-      }
+      if (!empty && my_cols <= 0)
+        release();
     }
+    if (lane == 0)
+      tma_store_wait<0>(); // the slots outlive the stores that read them
     if (p.zero_rest && p.ragged == kRaggedRows) {
       const int wid = static_cast<int>(blockIdx.x) * kEpiWarps + warp - 2, warps = static_cast<int>(gridDim.x) * kEpiWarps;
       zero_rows(p.D, 2, p.ldd, 0, table.begin[0], p.Q, wid, warps, lane);
@@ -393,8 +401,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 }
 
 template <bool kAMn, bool kBMn>
-cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
-                       cudaStream_t stream) {
+cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
   auto kernel = linear_pair_kernel<kAMn, kBMn>;
   cudaError_t err = prepare_kernel(kernel, kSmemFixed + kTableBytes, nullptr);
   if (err != cudaSuccess)
@@ -409,16 +416,15 @@ cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const Linea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = l.pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  return cudaLaunchKernelEx(&cfg, kernel, m.a, m.b, m.d, m.z, p);
 }
 
 } // namespace
 
-cudaError_t launch_linear_pair(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
-                               cudaStream_t stream) {
+cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
   if (!l.a_mn)
-    return l.b_mn ? launch_one<false, true>(ta, tb, p, l, stream) : launch_one<false, false>(ta, tb, p, l, stream);
-  return l.b_mn ? launch_one<true, true>(ta, tb, p, l, stream) : cudaErrorInvalidValue;
+    return l.b_mn ? launch_one<false, true>(m, p, l, stream) : launch_one<false, false>(m, p, l, stream);
+  return l.b_mn ? launch_one<true, true>(m, p, l, stream) : cudaErrorInvalidValue;
 }
 
 cudaError_t linear_pair_read_status(int out[4], bool clear) {

@@ -63,7 +63,8 @@ template <int TN, bool kF32> struct Cfg {
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kBBytes = TN * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kSlots = kEpiWarps * slot_bytes<kF32>();
+  static constexpr int kBias = kEpiWarps * 32 * 4;
+  static constexpr int kSlots = kEpiWarps * slot_bytes<kF32>() + kBias;
   static constexpr int kFit = (kSmemLimit - 1024 - 1024 - kTableBytes - kSlots) / kStageBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr int kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
@@ -105,6 +106,7 @@ template <int W> __device__ __forceinline__ void tmem_load(uint32_t addr, float 
 template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
 __global__ void __launch_bounds__(Cfg<TN, kF32>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+              const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
               const __grid_constant__ LinearParams p) {
   using C = Cfg<TN, kF32>;
   const int num_stages = p.stages;
@@ -160,6 +162,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : (kSwap ? p.Q : p.P),
                       kSwap ? p.tile_q : kTileP);
 
+  EpiWarp epi_warp;
+  epi_warp.slot = slots + (warp - 2) * slot_bytes<kF32>();
+  epi_warp.bias = reinterpret_cast<float *>(slots + C::kEpiWarps * slot_bytes<kF32>()) + (warp - 2) * 32;
+  epi_warp.map_d = &tm_d;
+  epi_warp.map_z = &tm_z;
+  epi_warp.lane = lane;
   float col_bias = 0.0f; // tokens as columns: the bias of the lane's feature, fetched while the tile accumulates
 
   // This CTA's share of a tile's stages.
@@ -322,7 +330,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     const int quarter = warp & 3; // tensor-memory lanes this warp may read
     const int col0 = ((warp - 2) >> 2) * kMyCols;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint8_t *slot = slots + (warp - 2) * slot_bytes<kF32>();
+    const EpiWarp ew = epi_warp;
     TileWalk<kSwap> walk(p, table, kTileP);
     Tile w;
     int acc = 0;
@@ -367,9 +375,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int j = 0; j < W; j += 4)
             part[(c + j) / 4 * kTileP] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else if constexpr (kSwap) {
-          epilogue_columns<kF32, W>(p, t, w.q0 + c, v, col_bias, slot, lane);
+          epilogue_columns<kF32, W>(p, t, w.q0 + c, v, col_bias, ew.slot, lane);
         } else {
-          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, f, slot, lane);
+          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, f, ew);
         }
       };
       if constexpr (kF32) {
@@ -427,15 +435,19 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           } else {
             tmem_load<W>(lane_addr + static_cast<uint32_t>(acc * TN + col0 + c), v);
           }
+          if (!empty && c + W >= my_cols)
+            release_acc(); // read out: the tile after the next may use it
           const Ahead<W> now = next;
           if (!kSwap && splits == 1 && c + W < my_cols)
             fetch_ahead<W>(next, p, t, w.q0 + col0 + c + W, lane);
           chunk(col0 + c, v, now);
         }
-        if (!empty)
+        if (!empty && my_cols <= 0)
           release_acc();
       }
     }
+    if (lane == 0)
+      tma_store_wait<0>(); // the slots outlive the stores that read them
     if (p.zero_rest && p.ragged == kRaggedRows) {
       // the rows in front of the first and behind the last group
       const int rows = kSwap ? p.Q : p.P, cols = kSwap ? p.P : p.Q;
@@ -458,7 +470,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     cluster_wait();
     if (warp >= 2 && *abort_flag == 0) {
       const int quarter = warp & 3, half = (warp - 2) >> 2;
-      uint8_t *slot = slots + (warp - 2) * slot_bytes<kF32>();
+      const EpiWarp ew = epi_warp;
       TileWalk<kSwap> walk(p, table, kTileP);
       Tile w;
       if (walk.get(first_tile, w)) {
@@ -495,7 +507,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int i = rank + half * splits; i * 4 < live; i += kColGroups * splits) {
             const float4 f = four(i * 4);
             float v[4] = {f.x, f.y, f.z, f.w};
-            epilogue_columns<kF32, 4>(p, t, w.q0 + i * 4, v, col_bias, slot, lane);
+            epilogue_columns<kF32, 4>(p, t, w.q0 + i * 4, v, col_bias, ew.slot, lane);
           }
         } else {
           constexpr int V = 16; // columns at a time
@@ -512,11 +524,13 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               v[j + 2] = q.z;
               v[j + 3] = q.w;
             }
-            epilogue_rows<kF32, V>(p, t, q0, v, f, slot, lane);
+            epilogue_rows<kF32, V>(p, t, q0, v, f, ew);
           }
         }
       }
     }
+    if (warp >= 2 && lane == 0)
+      tma_store_wait<0>();
     __syncwarp();
     cluster_arrive(); // nobody leaves while its part may still be read
     cluster_wait();
@@ -532,7 +546,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
 }
 
 template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
-cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l,
                        cudaStream_t stream) {
   using C = Cfg<TN, kF32>;
   auto kernel = linear_kernel<TN, kAMn, kBMn, kSwap, kF32>;
@@ -557,47 +571,47 @@ cudaError_t launch_one(const CUtensorMap &ta, const CUtensorMap &tb, const Linea
     ++cfg.numAttrs;
   }
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  return cudaLaunchKernelEx(&cfg, kernel, m.a, m.b, m.d, m.z, p);
 }
 
 template <bool kAMn, bool kBMn, bool kSwap, bool kF32>
-cudaError_t launch_tile(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+cudaError_t launch_tile(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l,
                         cudaStream_t stream) {
   if constexpr (kSwap) {
     switch (l.tile_n) {
     case 16:
-      return launch_one<16, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+      return launch_one<16, kAMn, kBMn, kSwap, kF32>(m, p, l, stream);
     case 32:
-      return launch_one<32, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+      return launch_one<32, kAMn, kBMn, kSwap, kF32>(m, p, l, stream);
     }
   }
   switch (l.tile_n) {
   case 64:
-    return launch_one<64, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+    return launch_one<64, kAMn, kBMn, kSwap, kF32>(m, p, l, stream);
   case 128:
-    return launch_one<128, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+    return launch_one<128, kAMn, kBMn, kSwap, kF32>(m, p, l, stream);
   }
   if constexpr (!kSwap && !kF32) {
     if (l.tile_n == 256)
-      return launch_one<256, kAMn, kBMn, kSwap, kF32>(ta, tb, p, l, stream);
+      return launch_one<256, kAMn, kBMn, kSwap, kF32>(m, p, l, stream);
   }
   return cudaErrorInvalidValue;
 }
 
 template <bool kF32>
-cudaError_t launch_layout(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
+cudaError_t launch_layout(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l,
                           cudaStream_t stream) {
   if (!l.a_mn && !l.b_mn)
-    return l.swap ? launch_tile<false, false, true, kF32>(ta, tb, p, l, stream)
-                  : launch_tile<false, false, false, kF32>(ta, tb, p, l, stream);
+    return l.swap ? launch_tile<false, false, true, kF32>(m, p, l, stream)
+                  : launch_tile<false, false, false, kF32>(m, p, l, stream);
   if (l.swap)
     return cudaErrorInvalidValue;
   if (!l.a_mn && l.b_mn) {
     if constexpr (!kF32) // the input gradient has the operands' type
-      return launch_tile<false, true, false, kF32>(ta, tb, p, l, stream);
+      return launch_tile<false, true, false, kF32>(m, p, l, stream);
   }
   if (l.a_mn && l.b_mn)
-    return launch_tile<true, true, false, kF32>(ta, tb, p, l, stream);
+    return launch_tile<true, true, false, kF32>(m, p, l, stream);
   return cudaErrorInvalidValue;
 }
 
@@ -613,11 +627,10 @@ int linear_max_stages(int tile_n, int out_f32) {
   return Cfg<256, false>::kStages;
 }
 
-cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
-                          cudaStream_t stream) {
+cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
   if (l.pair)
-    return launch_linear_pair(ta, tb, p, l, stream);
-  return l.out_f32 ? launch_layout<true>(ta, tb, p, l, stream) : launch_layout<false>(ta, tb, p, l, stream);
+    return launch_linear_pair(m, p, l, stream);
+  return l.out_f32 ? launch_layout<true>(m, p, l, stream) : launch_layout<false>(m, p, l, stream);
 }
 
 cudaError_t linear_read_status(int out[4], bool clear) {

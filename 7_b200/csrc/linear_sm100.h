@@ -26,6 +26,18 @@ constexpr int kLinearMaxSplits = 8;    // CTAs of a cluster that share one tile'
 // tokens), otherwise tokens are rows; the weight gradient has out-features on P
 // and in-features on Q.  D's element (token m, feature n) is at m * ldd + n
 // either way.
+struct FastDiv { // see fast_div
+  uint32_t d, m, s;
+};
+inline FastDiv make_fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  while ((1ull << f.s) < d)
+    ++f.s;
+  if (f.s > 0)
+    f.m = static_cast<uint32_t>(((1ull << (31 + f.s)) + d - 1) / d);
+  return f;
+}
+
 struct LinearParams {
   int P, Q, K;       // extents; the ragged one is its upper bound (all tokens)
   int ragged, groups;
@@ -33,7 +45,9 @@ struct LinearParams {
   int group_a, group_b; // the operand has one matrix for each group (third coordinate of its tensor map)
   int tile_q;        // columns of a tile: a multiple of 16 (of 64 where B is stored [K][Q]) <= the kernel's tile
   int p_blocks, q_blocks; // tiles along each side (ragged side: unused)
-  int raster;        // row blocks that are walked down before the next column block
+  int raster_log2;   // row blocks (its power of two) that are walked down before the next column block
+  FastDiv band_tiles;  // tiles of so many row blocks
+  FastDiv group_tiles; // weight gradient: tiles of a group
   int stages;        // ring depth of this launch (at most the kernel's)
   int splits;        // CTAs of a cluster that share a tile's contraction; then one tile for each cluster
   int is_bf16;       // operands, z, residual and 16-bit outputs: bf16 or f16
@@ -49,6 +63,7 @@ struct LinearParams {
   int bias_f32;
   long long group_bias;
   int vec_d, vec_z, vec_r; // 16-byte accesses are aligned in D / Z / R
+  int tma_d, tma_z;  // whole blocks of D / Z leave by TMA stores (tokens as rows, the maps are there)
   int zero_rest;     // rows of D and Z that belong to no group are set to zero
 };
 
@@ -64,12 +79,13 @@ struct LinearLaunch {
 
 // Ring depth the kernel has room for; a launch may take fewer stages, at least 4.
 int linear_max_stages(int tile_n, int out_f32);
-cudaError_t launch_linear(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
-                          cudaStream_t stream);
+struct LinearMaps {
+  CUtensorMap a, b, d, z; // d and z: read where tma_d / tma_z are set, boxes of 32 columns x 32 rows
+};
+cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_read_status(int out[4], bool clear);
 // tile_q a multiple of 32 (of 128 where B is stored [K][Q]) up to 256; grid even.
-cudaError_t launch_linear_pair(const CUtensorMap &ta, const CUtensorMap &tb, const LinearParams &p, const LinearLaunch &l,
-                               cudaStream_t stream);
+cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_pair_read_status(int out[4], bool clear);
 
 // ---- helpers around the products (linear_aux_sm100.cu)

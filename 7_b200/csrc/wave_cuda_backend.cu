@@ -164,6 +164,26 @@ int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int r
   return WAVE_OK;
 }
 
+// Rank-3 map for stores of 32-column blocks out of shared memory rows of 64
+// (16-bit) or 128 (f32) bytes, swizzled by as much.
+int make_tensor_map_store(CUtensorMap *map, int type, void *base, const uint64_t *dims, const uint64_t *strides_bytes,
+                          uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn)
+    return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]}, gstr[2] = {strides_bytes[0], strides_bytes[1]};
+  const cuuint32_t box[3] = {32, box_rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, type == WAVE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == WAVE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        3, base, gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        type == WAVE_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (store, dims %llu x %llu x %llu)", static_cast<int>(r),
+                static_cast<unsigned long long>(dims[0]), static_cast<unsigned long long>(dims[1]),
+                static_cast<unsigned long long>(dims[2]));
+  return WAVE_OK;
+}
+
 } // namespace wave
 
 namespace {

@@ -11,8 +11,10 @@
 #include <cstring>
 #include <exception>
 
-namespace wave {
-void set_last_error(const char *message); // wave_cuda_backend.cu
+namespace wave { // wave_cuda_backend.cu
+void set_last_error(const char *message);
+int make_tensor_map_store(CUtensorMap *map, int type, void *base, const uint64_t *dims, const uint64_t *strides_bytes,
+                          uint32_t box_rows);
 }
 
 namespace {
@@ -205,7 +207,7 @@ constexpr int kClusterFit[wave::kLinearMaxSplits + 1] = {0, 148, 148, 135, 132, 
 
 struct Plan {
   LinearLaunch launch;
-  int tile_q, p_blocks, q_blocks, raster, splits, stages;
+  int tile_q, p_blocks, q_blocks, raster_log2, splits, stages;
 };
 
 // A product's extents as the tiles see them.
@@ -320,7 +322,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
       if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
         continue;
       // columns of no use are left out where the layout allows: tiles of equal width
-      const int unit = l.b_mn ? (pair ? 128 : 64) : (pair ? 32 : 16);
+      const int unit = l.b_mn ? (pair ? 128 : 64) : (swap ? 16 : 32);
       int tile_q = tile_n;
       if (!(swap && s.grouped)) {
         const long long n = (e.q + tile_n - 1) / tile_n;
@@ -351,7 +353,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   pl.p_blocks = static_cast<int>(best.pb);
   pl.q_blocks = static_cast<int>(best.qb);
   // 2048 rows of tiles share their columns' panel
-  pl.raster = l.pair ? 8 : 16;
+  pl.raster_log2 = l.pair ? 3 : 4;
   if (l.pair) {
     const long long pairs = sms / 2;
     l.grid = static_cast<int>(2 * (best.tiles < pairs ? (best.tiles > 0 ? best.tiles : 1) : pairs));
@@ -414,7 +416,11 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   p.tile_q = pl.tile_q;
   p.p_blocks = pl.p_blocks;
   p.q_blocks = pl.q_blocks;
-  p.raster = pl.raster;
+  p.raster_log2 = pl.raster_log2;
+  // (tokens on the columns: their blocks are the rows of the walk with experts)
+  const uint32_t across = static_cast<uint32_t>(l.swap && s.grouped ? pl.p_blocks : pl.q_blocks);
+  p.band_tiles = wave::make_fast_div((across > 0 ? across : 1u) << pl.raster_log2);
+  p.group_tiles = wave::make_fast_div(static_cast<uint32_t>(pl.p_blocks) * static_cast<uint32_t>(pl.q_blocks > 0 ? pl.q_blocks : 1));
   p.splits = pl.splits;
   p.stages = pl.stages;
   p.is_bf16 = is_bf16;
@@ -433,14 +439,38 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   p.vec_z = aligned16(o.Z) && d.ldz % 8 == 0;
   p.vec_r = aligned16(o.R) && d.ldr % 8 == 0;
   p.zero_rest = zero_rest;
-  CUtensorMap ta, tb;
-  int rc = operand_map(&ta, a, is_bf16, 64, l.a_mn ? 64 : 128);
+  wave::LinearMaps m;
+  int rc = operand_map(&m.a, a, is_bf16, 64, l.a_mn ? 64 : 128);
   if (rc != WAVE_OK)
     return rc;
-  rc = operand_map(&tb, b, is_bf16, 64, l.b_mn ? 64 : l.pair ? pl.tile_q / 2 : pl.tile_q);
+  rc = operand_map(&m.b, b, is_bf16, 64, l.b_mn ? 64 : l.pair ? pl.tile_q / 2 : pl.tile_q);
   if (rc != WAVE_OK)
     return rc;
-  cudaError_t err = wave::launch_linear(ta, tb, p, l, stream);
+  // Results leave by TMA where their rows allow it: a store cuts a row at a
+  // multiple of 16 bytes, so its length has to be one.  (A split tile's are written
+  // in blocks of 16 columns, tokens on columns by other means.)
+  m.d = m.z = m.a;
+  if (!l.swap && pl.splits == 1) {
+    const bool per_group = p.ragged == wave::kRaggedK;
+    const uint64_t rows = static_cast<uint64_t>(p.P), cols = static_cast<uint64_t>(p.Q);
+    if (p.vec_d && p.Q * o.elem % 16 == 0) {
+      const uint64_t dims[3] = {cols, rows, per_group ? static_cast<uint64_t>(s.matrices) : 1};
+      const uint64_t row = static_cast<uint64_t>(o.ldd) * o.elem;
+      const uint64_t strides[2] = {row, per_group ? static_cast<uint64_t>(o.group_d) * o.elem : row * rows};
+      rc = wave::make_tensor_map_store(&m.d, out_f32 ? WAVE_F32 : d.io_type, o.D, dims, strides, 32);
+      if (rc != WAVE_OK)
+        return rc;
+      p.tma_d = 1;
+    }
+    if (p.Z && p.vec_z && p.Q % 8 == 0) {
+      const uint64_t dims[3] = {cols, rows, 1}, row = static_cast<uint64_t>(d.ldz) * 2;
+      const uint64_t strides[2] = {row, row * rows};
+      if ((rc = wave::make_tensor_map_store(&m.z, d.io_type, o.Z, dims, strides, 32)) != WAVE_OK)
+        return rc;
+      p.tma_z = 1;
+    }
+  }
+  cudaError_t err = wave::launch_linear(m, p, l, stream);
   return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear launch");
 }
 

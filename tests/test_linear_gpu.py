@@ -104,7 +104,7 @@ def test_forward_exact(cuda, wc, wl, m, n, k, io, out):
     wc.check_device_status()
 
 
-@pytest.mark.parametrize("gap", [1, 3, 8, 40])
+@pytest.mark.parametrize("gap", [1, 3, 7, 8, 40])
 @pytest.mark.parametrize("m,n,k", [(5, 40, 64), (140, 96, 200), (300, 33, 65)])
 def test_forward_strided_rows(cuda, wc, wl, m, n, k, gap):
     """Every operand with gaps between its rows (filled with NaN), outputs written between guard values."""
@@ -140,6 +140,15 @@ def test_pairs(cuda, wc, wl):
         check_all(cuda, wc, wl, make_gen(cuda, 3), ((45, 300, 712), (261, 136, 330), (1000, 520, 1032), (513, 1001, 777)))
         # more tiles than pairs, several cut stages of one expert after the other in the ring
         check_all(cuda, wc, wl, make_gen(cuda, 4), ((300, 2504, 2568),), [3, 17, 0, 5, 33, 1, 2, 64, 80, 15, 16, 40])
+
+
+@pytest.mark.parametrize("pair", [0, 1])
+def test_bands_of_tiles(cuda, wc, wl, pair):
+    """More row blocks than a band of the walk over the tiles has, with a last band that is cut short."""
+    with env_knobs(wc, WAVE_CUDA_LINEAR_SWAP=0, WAVE_CUDA_LINEAR_PAIR=pair):
+        check_all(cuda, wc, wl, make_gen(cuda, 5), ((4700, 328, 72), (2700, 1160, 136)), [2500, 0, 60, 17])
+    with env_knobs(wc, WAVE_CUDA_LINEAR_SWAP=1, WAVE_CUDA_LINEAR_TILE=16):
+        check_all(cuda, wc, wl, make_gen(cuda, 6), ((700, 2440, 72),), [500, 0, 60, 17])
 
 
 def check_all(torch, wc, wl, gen, shapes, rows=None):
@@ -218,7 +227,7 @@ def test_backward_exact(cuda, wc, wl, m, n, k, io):
     wc.check_device_status()
 
 
-@pytest.mark.parametrize("gap", [1, 8])
+@pytest.mark.parametrize("gap", [1, 6, 8])
 def test_backward_strided_rows(cuda, wc, wl, gap):
     torch, gen = cuda, make_gen(cuda, 5)
     m, n, k = 70, 130, 90
