@@ -58,7 +58,7 @@ int launch_flash_attention_decoupled(const FaParams &p, const FaExtra &extra, co
                                      const void *V, int poly, int stagger_cycles, int sm_count, cudaStream_t stream);
 cudaError_t fa_decoupled_read_status(int out[4], bool clear);
 
-// Provided by the backend: rank-2/3 tensor map over 16-bit elements with the
+// Provided by the backend: rank-2 to rank-4 tensor map over 16-bit elements with the
 // 128-byte swizzle and zero fill outside the tensor.
 int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int rank, const uint64_t *dims,
                           const uint64_t *strides_bytes, const uint32_t *box);

@@ -191,8 +191,37 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
 }
+// An arrival in another CTA (or this one) that hands over no memory, such as that
+// an accumulator has been read out of tensor memory.  With release semantics it
+// waits for whatever the thread has written: 1500 to 2500 cycles of every tile.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// warp_wait that also orders what follows behind what the other CTA's threads
+// wrote before they arrived.
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+  if (!warp_wait(bar, parity, abort_flag, false))
+    return false;
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+               "selp.b32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory"); // (complete already)
+  return __all_sync(0xffffffffu, ok != 0) != 0;
+}
 __device__ __forceinline__ bool warp_peek(uint64_t *bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)) != 0;
+}
+
+// All 64-column chunks of an operand that is stored with the contraction as its
+// slow direction, by one copy: the tensor is seen as [matrices][chunks][rows][64].
+__device__ __forceinline__ void tma_load_chunks(void *dst, const CUtensorMap *map, uint64_t *bar, int row, int chunk, int z) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+               " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(chunk), "r"(z)
+               : "memory");
 }
 
 // ------------------------------------------------------------- activations
@@ -347,7 +376,7 @@ template <int kElem, int W> struct Slot {
   static constexpr int kVals = 16 / kElem;
   static constexpr int kRowsPerLine = 8 / kPieces; // rows in 128 bytes
   static constexpr int kBytes = 32 * kPieces * 16;
-  static_assert(kPieces == 2 || kPieces == 4 || kPieces == 8, "16 or 32 columns of 2 or 4 bytes");
+  static_assert(kPieces == 2 || kPieces == 4 || kPieces == 8, "rows of 32, 64 or 128 bytes");
   static __device__ __forceinline__ int at(int r, int c) {
     return (r * kPieces + (c ^ ((r / kRowsPerLine) & (kPieces - 1)))) * 16;
   }
@@ -427,12 +456,33 @@ __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *
   }
 }
 
-template <int W> __device__ __forceinline__ void row_to_slot_16bit(uint8_t *slot, const float (&v)[W], int bf16, int lane) {
+template <int W, bool kBf16> __device__ __forceinline__ void row_to_slot_type(uint8_t *slot, const float (&v)[W], int lane) {
 #pragma unroll
   for (int k = 0; k < W / 8; ++k)
     *reinterpret_cast<uint4 *>(slot + Slot<2, W>::at(lane, k)) =
-        make_uint4(pack_pair(v[8 * k], v[8 * k + 1], bf16), pack_pair(v[8 * k + 2], v[8 * k + 3], bf16),
-                   pack_pair(v[8 * k + 4], v[8 * k + 5], bf16), pack_pair(v[8 * k + 6], v[8 * k + 7], bf16));
+        make_uint4(pack_pair(v[8 * k], v[8 * k + 1], kBf16), pack_pair(v[8 * k + 2], v[8 * k + 3], kBf16),
+                   pack_pair(v[8 * k + 4], v[8 * k + 5], kBf16), pack_pair(v[8 * k + 6], v[8 * k + 7], kBf16));
+}
+template <int W> __device__ __forceinline__ void row_to_slot_16bit(uint8_t *slot, const float (&v)[W], int bf16, int lane) {
+  if (bf16) // outside the loop
+    row_to_slot_type<W, true>(slot, v, lane);
+  else
+    row_to_slot_type<W, false>(slot, v, lane);
+}
+// The residual of the lane's row, as it lies in the slot, added to v.
+template <int W, bool kBf16> __device__ __forceinline__ void add_row_from_slot(float (&v)[W], const uint8_t *slot, int lane) {
+#pragma unroll
+  for (int k = 0; k < W / 8; ++k) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(slot + Slot<2, W>::at(lane, k));
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = 8 * k + 2 * e;
+      const float2 sum = __fadd2_rn(make_float2(v[j], v[j + 1]), unpack_pair(words[e], kBf16));
+      v[j] = sum.x;
+      v[j + 1] = sum.y;
+    }
+  }
 }
 
 // What a warp's epilogue needs to know of its tile.
@@ -443,15 +493,15 @@ struct EpiTile {
   int q_end;     // end of the live Q columns
 };
 
-// Bytes of a warp's slot.
-template <bool kF32> __host__ __device__ constexpr int slot_bytes() { return kF32 ? Slot<4, 32>::kBytes : Slot<2, 32>::kBytes; }
+// Bytes of a warp's slot: 32 rows of 128.
+constexpr int kSlotBytes = 4096;
 
 // What a chunk's epilogue reads from memory, fetched while the chunk before it
 // is worked on (tokens as rows): the residual in the order of slot_to_global,
 // and the bias, one value to a lane.
 template <int W> struct Ahead {
   uint4 res[W / 8];
-  float bias;
+  float bias[(W + 31) / 32];
 };
 template <int W>
 __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, const EpiTile &t, int q0, int lane) {
@@ -459,16 +509,19 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
   if (p.R)
     global_to_regs<W>(f.res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(t.lane0) * p.ldr + q0, p.ldr, rows,
                       cols, p.vec_r != 0, lane);
-  f.bias = 0.0f;
-  if (p.bias && lane < cols) {
-    const long long at = t.group * p.group_bias + q0 + lane;
-    f.bias = p.bias_f32 ? static_cast<const float *>(p.bias)[at]
-                        : from_16bit(static_cast<const uint16_t *>(p.bias)[at], p.is_bf16);
+#pragma unroll
+  for (int i = 0; i < (W + 31) / 32; ++i) {
+    f.bias[i] = 0.0f;
+    if (p.bias && lane + 32 * i < cols) {
+      const long long at = t.group * p.group_bias + q0 + lane + 32 * i;
+      f.bias[i] = p.bias_f32 ? static_cast<const float *>(p.bias)[at]
+                             : from_16bit(static_cast<const uint16_t *>(p.bias)[at], p.is_bf16);
+    }
   }
 }
 
-// What an epilogue warp has of its own: its slot, 32 floats for the bias, and
-// the tensor maps of D and z (their boxes are a slot: 32 rows of 32 columns).
+// What an epilogue warp has of its own: its slot, 64 floats for the bias, and
+// the tensor maps of D and z (their boxes are a slot: 32 rows of 128 bytes).
 //
 // Blocks leave the slot by one TMA store where they can: through the load-store
 // unit a block is read from shared memory and written to L1 a second time, which
@@ -491,7 +544,7 @@ __device__ __forceinline__ void slot_wait(const EpiWarp &e) {
 template <int kElem, int W>
 __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *map, bool tma, void *base, long long ld, int rows,
                                          int cols, bool vec, int q0, int p0, int group) {
-  if (W == 32 && tma) {
+  if (W * kElem == 128 && tma) {
     fence_proxy_async_smem();
     __syncwarp();
     if (e.lane == 0) {
@@ -509,15 +562,16 @@ __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *ma
 template <bool kF32, int W>
 __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
                                               const Ahead<W> &f, const EpiWarp &e) {
-  uint8_t *slot = e.slot;
   const int lane = e.lane;
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
   if (rows <= 0 || cols <= 0)
     return; // the same for the whole warp
   const bool whole = rows == 32 || p.ragged != kRaggedRows; // no row behind these is another expert's
   if (p.bias) { // handed round
-    if (lane < W)
-      e.bias[lane] = f.bias;
+#pragma unroll
+    for (int i = 0; i < (W + 31) / 32; ++i)
+      if (lane + 32 * i < W)
+        e.bias[lane + 32 * i] = f.bias[i];
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
@@ -533,12 +587,13 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
   }
   if (p.Z) {
     slot_wait(e);
-    row_to_slot_16bit<W>(slot, v, p.is_bf16, lane);
+    row_to_slot_16bit<W>(e.slot, v, p.is_bf16, lane);
     slot_out<2, W>(e, e.map_z, p.tma_z && whole, static_cast<uint16_t *>(p.Z) + static_cast<long long>(t.lane0) * p.ldz + q0,
                    p.ldz, rows, cols, p.vec_z != 0, q0, t.lane0, 0);
   }
   apply_act<W>(v, p.act);
   slot_wait(e);
+  uint8_t *slot = e.slot;
   if (p.R) {
     using S = Slot<2, W>;
     constexpr int kRowStep = 32 / S::kPieces;
@@ -546,18 +601,10 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
     for (int i = 0; i < S::kPieces; ++i)
       *reinterpret_cast<uint4 *>(slot + S::at(lane / S::kPieces + i * kRowStep, lane % S::kPieces)) = f.res[i];
     __syncwarp();
-#pragma unroll
-    for (int k = 0; k < W / 8; ++k) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(slot + S::at(lane, k));
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 8 * k + 2 * e;
-        const float2 sum = __fadd2_rn(make_float2(v[j], v[j + 1]), unpack_pair(words[e], p.is_bf16));
-        v[j] = sum.x;
-        v[j + 1] = sum.y;
-      }
-    }
+    if (p.is_bf16)
+      add_row_from_slot<W, true>(v, slot, lane);
+    else
+      add_row_from_slot<W, false>(v, slot, lane);
     __syncwarp(); // f32 rows are longer: the slot may be rewritten once every lane has its residual
   }
   const long long at = t.group * p.group_d + static_cast<long long>(t.lane0) * p.ldd + q0;

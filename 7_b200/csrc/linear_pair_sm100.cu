@@ -12,10 +12,10 @@
 //              tried: a remote arrival with release costs that thread so long that
 //              8192^3 took 1500 us)
 //   landed[s]  one per CTA: the last stage of an expert's weight gradient lands
-//              here, and the CTA's own warp 1 zeroes the rows behind the expert's
+//              here, and the CTA's cutting warp zeroes the rows behind the expert's
 //              last (several such stages may be in the ring, so each has a barrier)
-//   cut[s]     in the leader: the other CTA has done so; the leader then completes
-//              full[s] itself
+//   cut[s]     in the leader: both CTAs have done so; the leader's issuing warp
+//              then completes full[s] itself
 //   empty[s], tfull[a]  one per CTA; the leader's tcgen05.commit arrives on both
 //   tempty[a]  in the leader; the epilogue warps of both CTAs arrive
 #include "launch_cache.h"
@@ -37,12 +37,12 @@ constexpr int kChunkBytes = 64 * 128;
 constexpr int kABytes = kRows * kBK * 2;
 constexpr int kBBytes = kTN / 2 * kBK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStages = 6;
+constexpr int kStages = 5; // (six, with slots of half the size: 0.5 % on a bare 8192^3, lost again in the epilogue)
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kMyCols = kTN / 2; // columns of an epilogue warp
-constexpr int kW = 32;
-constexpr int kSlots = kEpiWarps * (slot_bytes<false>() + 32 * 4); // and the bias
+constexpr int kThreadsCut = kThreads + 32; // the weight gradient has a warp that cuts
+constexpr int kW = 64; // columns of an epilogue chunk; the two groups of four warps take them in turn
+constexpr int kSlots = kEpiWarps * (kSlotBytes + 64 * 4); // and the bias
 constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
 constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots;
 static_assert(kSmemFixed + kTableBytes <= 227 * 1024, "does not fit the shared memory of an SM");
@@ -73,12 +73,15 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *m
                : "memory");
 }
 
-// Orders what this thread does next behind what the other CTA's threads wrote
-// before they arrived on a barrier that this thread has seen complete.
-__device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_chunks_pair(void *dst, const CUtensorMap *map, uint64_t *bar, int row, int chunk, int z) {
+  asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+               " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar) & kPeerBitMask), "r"(0), "r"(row), "r"(chunk), "r"(z)
+               : "memory");
+}
 
 template <bool kAMn, bool kBMn>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAMn && kBMn ? kThreadsCut : kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
                    const __grid_constant__ LinearParams p) {
@@ -105,7 +108,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
       mbar_init(&sh->landed[s], 1);
-      mbar_init(&sh->cut[s], 1);
+      mbar_init(&sh->cut[s], 2);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&sh->tfull[a], 1);
@@ -162,28 +165,44 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
         if (kCut && is_cut(live_of(w, kb))) {
           if (chosen) {
-            // this CTA's bytes on its own barrier: warp 1 cuts them
+            // this CTA's bytes on its own barrier: the cutting warp takes them over
             mbar_arrive_expect_tx(landed, tx);
-            for (int c = 0; c < kRows / 64; ++c)
-              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, landed, pa + c * 64, k, za);
-            for (int c = 0; c < half_q / 64; ++c)
-              tma_load_3d(b_dst + c * kChunkBytes, &tm_b, landed, qb + c * 64, k, zb);
+            if (p.chunks_a) {
+              tma_load_chunks(a_dst, &tm_a, landed, k, pa / 64, za);
+            } else {
+              for (int c = 0; c < kRows / 64; ++c)
+                tma_load_3d(a_dst + c * kChunkBytes, &tm_a, landed, pa + c * 64, k, za);
+            }
+            if (p.chunks_b) {
+              tma_load_chunks(b_dst, &tm_b, landed, k, qb / 64, zb);
+            } else {
+              for (int c = 0; c < half_q / 64; ++c)
+                tma_load_3d(b_dst + c * kChunkBytes, &tm_b, landed, qb + c * 64, k, zb);
+            }
           }
         } else if (chosen) {
           if (leader)
             mbar_arrive_expect_tx(bar, 2 * tx);
           if constexpr (kAMn) {
+            if (p.chunks_a) {
+              tma_load_chunks_pair(a_dst, &tm_a, bar, k, pa / 64, za);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kRows / 64; ++c)
-              tma_load_3d_pair(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+              for (int c = 0; c < kRows / 64; ++c)
+                tma_load_3d_pair(a_dst + c * kChunkBytes, &tm_a, bar, pa + c * 64, k, za);
+            }
           } else {
             tma_load_3d_pair(a_dst, &tm_a, bar, k, pa, za);
           }
           if constexpr (kBMn) {
+            if (p.chunks_b) {
+              tma_load_chunks_pair(b_dst, &tm_b, bar, k, qb / 64, zb);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kTN / 128; ++c)
-              if (c * 64 < half_q)
-                tma_load_3d_pair(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
+              for (int c = 0; c < kTN / 128; ++c)
+                if (c * 64 < half_q)
+                  tma_load_3d_pair(b_dst + c * kChunkBytes, &tm_b, bar, qb + c * 64, k, zb);
+            }
           } else {
             tma_load_3d_pair(b_dst, &tm_b, bar, k, qb, zb);
           }
@@ -194,8 +213,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     if (!ok)
       bounded_delay(1 << 21);
   } else if (warp == 1) {
-    // ---------------------- UMMA issue (leader), cutting of last stages (both)
-    if (kCut || leader) {
+    // ------------------------------------------------ UMMA issue (leader)
+    if (leader) {
       const uint32_t idesc = umma_idesc_f16(kPairP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
       constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
       constexpr uint64_t kStep = kStageBytes >> 4;
@@ -205,21 +224,23 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       const uint32_t tmem_d = static_cast<uint32_t>(warp_uniform(static_cast<int>(tmem_base)));
       const bool chosen = elect_one();
       TileWalk<false> walk(p, table, kPairP);
-      Tile w;
+      Tile w, next_w;
       Ring ring;
       int acc = 0;
-      uint32_t acc_phase = 0, cut_phases = 0; // of landed and cut: a bit to a stage
+      uint32_t acc_phase = 0, cut_phases = 0; // of cut: a bit to a stage
       bool ok = true;
-      for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
+      bool more_tiles = walk.get_uniform(first_tile, next_w);
+      for (int id = first_tile; ok && more_tiles;) {
+        w = next_w;
+        id += tile_step;
+        bool looked = false; // where the next tile lies: worked out while products are under way
         const int kbs = (w.k_len + kBK - 1) / kBK;
-        if (kbs <= 0)
-          continue;
-        const int live = live_of(w, kbs - 1);
-        const bool cut = is_cut(live);
-        const int whole = kbs - (cut ? 1 : 0);
-        const uint32_t d = tmem_d + static_cast<uint32_t>(acc * kTN);
-        uint32_t more = 0; // the accumulator holds something
-        if (leader) {
+        if (kbs > 0) {
+          const int live = live_of(w, kbs - 1);
+          const bool cut = is_cut(live);
+          const int whole = kbs - (cut ? 1 : 0);
+          const uint32_t d = tmem_d + static_cast<uint32_t>(acc * kTN);
+          uint32_t more = 0; // the accumulator holds something
           ok = warp_wait(&sh->tempty[acc], acc_phase ^ 1, abort_flag, false);
           if (!ok) {
             pair_report(kStatusWaitTimeout, 1, 100 + acc);
@@ -246,75 +267,92 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             }
             __syncwarp();
             more = 1;
+            if (!looked) {
+              more_tiles = walk.get_uniform(id, next_w);
+              looked = true;
+            }
           }
           if (!ok)
             break;
-        } else { // only the last stage is this CTA's business
-          const int at = ring.stage + whole;
-          ring.phase ^= static_cast<uint32_t>(at / kStages) & 1u;
-          ring.stage = at % kStages;
-        }
-        if constexpr (kCut) {
-          if (cut) {
-            const uint32_t parity = (cut_phases >> ring.stage) & 1u;
-            cut_phases ^= 1u << ring.stage;
-            ok = warp_wait(&sh->landed[ring.stage], parity, abort_flag, false);
-            if (!ok) {
-              pair_report(kStatusWaitTimeout, 1, 50 + ring.stage);
-              break;
-            }
-            uint8_t *a_tile = tiles + ring.stage * kStageBytes;
-            const int steps = (live + 15) / 16;
-            const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
-            const int chunks = kRows / 64 + p.tile_q / 128;
-            for (int i = lane; i < chunks * vecs; i += 32) {
-              uint8_t *dst = a_tile + (i / vecs) * kChunkBytes + live * 128 + (i % vecs) * 16;
-              *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (leader) {
-              ok = warp_wait(&sh->cut[ring.stage], parity, abort_flag, false);
+          if constexpr (kCut) {
+            if (cut) {
+              const uint32_t parity = (cut_phases >> ring.stage) & 1u;
+              cut_phases ^= 1u << ring.stage;
+              ok = warp_wait_cluster(&sh->cut[ring.stage], parity, abort_flag);
               if (!ok) {
                 pair_report(kStatusWaitTimeout, 1, 70 + ring.stage);
                 break;
               }
-              fence_acquire_cluster();
               fence_proxy_async_smem();
-              __syncwarp();
+              tc_fence_after_sync();
+              const int steps = (live + 15) / 16;
               if (chosen) {
                 mbar_arrive(&sh->full[ring.stage]); // the stage's turn of this barrier
-                tc_fence_after_sync();
                 const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
                 for (int k = 0; k < steps; ++k, more = 1)
                   umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, more);
                 umma_commit_pair(&sh->empty[ring.stage], 3);
               }
               __syncwarp();
-            } else {
-              if (lane == 0)
-                mbar_arrive_cluster(map_to_cta(&sh->cut[ring.stage], 0));
-              __syncwarp();
+              ring.advance(kStages);
             }
-            ring.advance(kStages);
+          }
+          if (chosen)
+            umma_commit_pair(&sh->tfull[acc], 3);
+          __syncwarp();
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
           }
         }
-        if (leader && chosen)
-          umma_commit_pair(&sh->tfull[acc], 3);
-        __syncwarp();
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
+        if (!looked)
+          more_tiles = walk.get_uniform(id, next_w);
+      }
+    }
+  } else if (kCut && warp == 2 + kEpiWarps) {
+    // ------------------------------------- cutting of last stages (both CTAs)
+    if constexpr (kCut) {
+      TileWalk<false> walk(p, table, kPairP);
+      Tile w;
+      Ring ring;
+      uint32_t phases = 0; // of landed: a bit to a stage
+      for (int id = first_tile; p.ragged == kRaggedK && walk.get_uniform(id, w); id += tile_step) {
+        const int kbs = (w.k_len + kBK - 1) / kBK;
+        if (kbs <= 0)
+          continue;
+        const int live = live_of(w, kbs - 1);
+        const bool cut = is_cut(live);
+        ring.stage = (ring.stage + kbs - (cut ? 1 : 0)) % kStages;
+        if (!cut)
+          continue;
+        const uint32_t parity = (phases >> ring.stage) & 1u;
+        phases ^= 1u << ring.stage;
+        if (!warp_wait(&sh->landed[ring.stage], parity, abort_flag, false)) {
+          pair_report(kStatusWaitTimeout, 3, ring.stage);
+          break;
         }
+        uint8_t *a_tile = tiles + ring.stage * kStageBytes;
+        const int steps = (live + 15) / 16;
+        const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
+        const int chunks = kRows / 64 + p.tile_q / 128;
+        for (int c = 0; c < chunks; ++c)
+          for (int i = lane; i < vecs; i += 32)
+            *reinterpret_cast<uint4 *>(a_tile + c * kChunkBytes + live * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive_cluster(map_to_cta(&sh->cut[ring.stage], 0));
+        __syncwarp();
+        ring.stage = (ring.stage + 1) % kStages;
       }
     }
   } else {
     // ---------------------------------------------------------- epilogue
     const int quarter = warp & 3;
-    const int col0 = ((warp - 2) >> 2) * kMyCols;
+    const int col0 = ((warp - 2) >> 2) * kW;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const EpiWarp ew{slots + (warp - 2) * slot_bytes<false>(),
-                     reinterpret_cast<float *>(slots + kEpiWarps * slot_bytes<false>()) + (warp - 2) * 32, &tm_d, &tm_z, lane};
+    const EpiWarp ew{slots + (warp - 2) * kSlotBytes, reinterpret_cast<float *>(slots + kEpiWarps * kSlotBytes) + (warp - 2) * 64,
+                     &tm_d, &tm_z, lane};
     const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
     TileWalk<false> walk(p, table, kPairP);
     Tile w;
@@ -324,20 +362,26 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0)
-        mbar_arrive_cluster(tempty_leader[acc]);
+        mbar_arrive_cluster_relaxed(tempty_leader[acc]);
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
       }
     };
-    for (int id = first_tile; walk.get(id, w); id += tile_step) {
+    // (where the next tile lies is worked out while this one's accumulator is waited for)
+    Tile next_w;
+    bool more_tiles = walk.get(first_tile, next_w);
+    for (int id = first_tile; more_tiles;) {
+      w = next_w;
+      id += tile_step;
+      more_tiles = walk.get(id, next_w);
       const bool empty = w.k_len <= 0; // nothing to multiply: the epilogue of zero
       EpiTile t;
       t.group = w.group;
       t.lane0 = w.p0 + rank * kRows + quarter * 32;
       t.lane_end = w.p_end;
       t.q_end = min(w.q_end, w.q0 + p.tile_q);
-      const int my_cols = min(kMyCols, p.tile_q - col0);
+      const int my_cols = p.tile_q - col0;
       Ahead<kW> next;
       if (my_cols > 0)
         fetch_ahead<kW>(next, p, t, w.q0 + col0, lane);
@@ -350,7 +394,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         tc_fence_after_sync();
       }
 #pragma unroll 1
-      for (int c = 0; c < my_cols; c += kW) {
+      for (int c = 0; c < my_cols; c += 2 * kW) {
         float v[kW];
         if (empty) {
 #pragma unroll
@@ -358,18 +402,19 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             v[j] = 0.0f;
         } else {
           uint32_t r[kW];
-          tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTN + col0 + c), r);
+          const uint32_t at = lane_addr + static_cast<uint32_t>(acc * kTN + col0 + c);
+          tmem_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+          tmem_ld_32x32b_x32(at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < kW; ++j)
             v[j] = __uint_as_float(r[j]);
+          if (c + 2 * kW >= my_cols)
+            release(); // read out: the tile after the next may use it
         }
-        if (!empty && c + kW >= my_cols)
-          release(); // read out: the tile after the next may use it
-        const Ahead<kW> now = next;
-        if (c + kW < my_cols)
-          fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + kW, lane);
-        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, now, ew);
+        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, next, ew);
+        if (c + 2 * kW < my_cols)
+          fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + 2 * kW, lane);
       }
       if (!empty && my_cols <= 0)
         release();
@@ -408,7 +453,7 @@ cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearL
     return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kAMn && kBMn ? kThreadsCut : kThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(kSmemFixed) + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

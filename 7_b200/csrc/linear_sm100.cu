@@ -21,7 +21,8 @@
 // Experts: the row ranges are read on the device (no host sync).  A row block
 // ends at its expert's last row by not storing the rows behind it; a weight
 // gradient's last 64 rows are cut to the expert's by zeroing what TMA brought in
-// of the next one's in shared memory (in both operands: 0 * NaN would stay).
+// of the next one's in shared memory (in both operands: 0 * NaN would stay), by a
+// warp of its own: done by the issuing warp it took 1000 cycles of each tile.
 //
 // f32 results: the tensor core adds to its f32 accumulator by truncation, an
 // error that grows with the length of the sum (measured relative to the norm:
@@ -44,6 +45,7 @@ constexpr int kBK = 64;
 constexpr int kChunkBytes = 64 * 128; // 64 rows of 128 bytes: a 64-element MN chunk of a stage
 constexpr int kABytes = kTileP * kBK * 2;
 constexpr int kMaxStages = 12;
+constexpr int kMinStages = 3;
 constexpr int kSegment = 8; // stages of an accumulator that is summed in registers
 constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
 constexpr int kSmemLimit = 227 * 1024;
@@ -53,6 +55,10 @@ struct Shared {
   uint64_t empty[kMaxStages];
   uint64_t tfull[2];
   uint64_t tempty[2];
+  // The stage with an expert's last rows: it lands on a barrier of its own (the
+  // cutting warp sees only these stages, and a wait for a parity must not skip a
+  // turn), and has been cut.
+  uint64_t landed[kMaxStages], cut[kMaxStages];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -61,16 +67,17 @@ static_assert(sizeof(Shared) <= 1024, "Shared outgrew its slot");
 template <int TN, bool kF32> struct Cfg {
   static constexpr int kEpiWarps = TN >= 128 ? 8 : 4;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kThreadsCut = kThreads + 32; // the weight gradient has a warp that cuts
   static constexpr int kBBytes = TN * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kBias = kEpiWarps * 32 * 4;
-  static constexpr int kSlots = kEpiWarps * slot_bytes<kF32>() + kBias;
+  static constexpr int kBias = kEpiWarps * 64 * 4;
+  static constexpr int kSlots = kEpiWarps * kSlotBytes + kBias;
   static constexpr int kFit = (kSmemLimit - 1024 - 1024 - kTableBytes - kSlots) / kStageBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr int kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
   static constexpr int kSmemFixed = 1024 + 1024 + kSlots; // + the stages, the group table
-  static_assert(kStages >= 4, "ring too short");
-  static_assert(TN * kTileP * 4 <= 4 * kStageBytes, "a partial tile must fit the shortest ring");
+  static_assert(kStages >= kMinStages, "ring too short");
+  static_assert(TN * kTileP * 4 <= kMinStages * kStageBytes, "a partial tile must fit the shortest ring");
 };
 
 __device__ __noinline__ void report(int code, int role, int detail) {
@@ -91,9 +98,12 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 }
 
 template <int W> __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[W]) {
-  static_assert(W == 16 || W == 32, "16 or 32 columns");
+  static_assert(W == 16 || W == 32 || W == 64, "16, 32 or 64 columns");
   uint32_t r[W];
-  if constexpr (W == 32)
+  if constexpr (W == 64) {
+    tmem_ld_32x32b_x32(addr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+    tmem_ld_32x32b_x32(addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+  } else if constexpr (W == 32)
     tmem_ld_32x32b_x32(addr, r);
   else
     tmem_ld_32x32b_x16(addr, r);
@@ -104,7 +114,7 @@ template <int W> __device__ __forceinline__ void tmem_load(uint32_t addr, float 
 }
 
 template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
-__global__ void __launch_bounds__(Cfg<TN, kF32>::kThreads, 1)
+__global__ void __launch_bounds__(kAMn && kBMn ? Cfg<TN, kF32>::kThreadsCut : Cfg<TN, kF32>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
               const __grid_constant__ LinearParams p) {
@@ -113,7 +123,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   constexpr bool kCut = kAMn && kBMn; // the weight gradient: stages may have to be cut at the last row
   constexpr int kColGroups = C::kEpiWarps / 4;
   constexpr int kMyCols = TN / kColGroups; // columns of an epilogue warp
-  constexpr int W = kMyCols < 32 ? kMyCols : 32;
+  // Columns of a chunk: tokens as rows and 16-bit results take 64, rows of 128
+  // bytes.  (With 32 the fixed cost of a chunk -- fence, store, waits -- and its
+  // latencies came twice as often: 1400 cycles each, which bounded short sums.)
+  constexpr int W = kSwap || kF32 ? (kMyCols < 32 ? kMyCols : 32) : 64;
+  // The groups of four warps take chunks in turn.
+  constexpr int kStride = kF32 || kSwap ? W : W * kColGroups;
   static_assert(!kF32 || kMyCols <= 64, "running sums stay in registers");
 
   extern __shared__ uint8_t smem_raw[];
@@ -138,6 +153,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     for (int s = 0; s < num_stages; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
+      mbar_init(&sh->landed[s], 1);
+      mbar_init(&sh->cut[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&sh->tfull[a], 1);
@@ -163,8 +180,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
                       kSwap ? p.tile_q : kTileP);
 
   EpiWarp epi_warp;
-  epi_warp.slot = slots + (warp - 2) * slot_bytes<kF32>();
-  epi_warp.bias = reinterpret_cast<float *>(slots + C::kEpiWarps * slot_bytes<kF32>()) + (warp - 2) * 32;
+  epi_warp.slot = slots + (warp - 2) * kSlotBytes;
+  epi_warp.bias = reinterpret_cast<float *>(slots + C::kEpiWarps * kSlotBytes) + (warp - 2) * 64;
   epi_warp.map_d = &tm_d;
   epi_warp.map_z = &tm_z;
   epi_warp.lane = lane;
@@ -175,6 +192,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     const int total = (w.k_len + kBK - 1) / kBK;
     kb0 = splits > 1 ? static_cast<int>(static_cast<long long>(total) * rank / splits) : 0;
     kb1 = splits > 1 ? static_cast<int>(static_cast<long long>(total) * (rank + 1) / splits) : total;
+  };
+
+  // Whether the last of them holds an expert's last rows and more.
+  auto has_cut = [&](const Tile &w, int kb0, int kb1) {
+    return kCut && p.ragged == kRaggedK && (w.k_len & (kBK - 1)) != 0 && kb1 > kb0 && kb1 * kBK > w.k_len;
   };
 
   if (warp == 0) {
@@ -202,24 +224,32 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         }
         uint8_t *a_dst = tiles + ring.stage * C::kStageBytes;
         uint8_t *b_dst = a_dst + kABytes;
-        uint64_t *bar = &sh->full[ring.stage];
+        uint64_t *bar = kCut && kb + 1 == kb1 && has_cut(w, kb0, kb1) ? &sh->landed[ring.stage] : &sh->full[ring.stage];
         const int k = w.k_begin + kb * kBK;
         ring.advance(num_stages);
         seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
         if (chosen) {
           mbar_arrive_expect_tx(bar, tx);
           if constexpr (kAMn) {
+            if (p.chunks_a) {
+              tma_load_chunks(a_dst, &tm_a, bar, k, w.p0 / 64, za);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kTileP / 64; ++c)
-              tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, w.p0 + c * 64, k, za);
+              for (int c = 0; c < kTileP / 64; ++c)
+                tma_load_3d(a_dst + c * kChunkBytes, &tm_a, bar, w.p0 + c * 64, k, za);
+            }
           } else {
             tma_load_3d(a_dst, &tm_a, bar, k, w.p0, za);
           }
           if constexpr (kBMn) {
+            if (p.chunks_b) {
+              tma_load_chunks(b_dst, &tm_b, bar, k, w.q0 / 64, zb);
+            } else {
 #pragma unroll
-            for (int c = 0; c < TN / 64; ++c)
-              if (c * 64 < p.tile_q)
-                tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, w.q0 + c * 64, k, zb);
+              for (int c = 0; c < TN / 64; ++c)
+                if (c * 64 < p.tile_q)
+                  tma_load_3d(b_dst + c * kChunkBytes, &tm_b, bar, w.q0 + c * 64, k, zb);
+            }
           } else {
             tma_load_3d(b_dst, &tm_b, bar, k, w.q0, zb);
           }
@@ -242,17 +272,20 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     const uint32_t tmem_d = static_cast<uint32_t>(warp_uniform(static_cast<int>(tmem_base)));
     const bool chosen = elect_one();
     TileWalk<kSwap> walk(p, table, kTileP);
-    Tile w;
+    Tile w, next_w;
     Ring ring;
     int acc = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_phase = 0, cut_phases = 0; // of cut: a bit to a stage
     bool ok = true;
-    for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
+    bool more_tiles = walk.get_uniform(first_tile, next_w);
+    for (int id = first_tile; ok && more_tiles;) {
+      w = next_w;
+      id += tile_step;
+      bool looked = false; // where the next tile lies: worked out while products are under way
       int kb0, kb1;
       k_blocks(w, kb0, kb1);
-      // the stage with an expert's last rows, if it is one of this CTA's
       const int live = w.k_len & (kBK - 1);
-      const bool cut = kCut && p.ragged == kRaggedK && live != 0 && kb1 > kb0 && kb1 * kBK > w.k_len;
+      const bool cut = has_cut(w, kb0, kb1);
       for (int kb = kb0; ok && kb < kb1;) {
         const int end = kF32 ? min(kb + kSegment, kb1) : kb1;
         const bool cut_here = cut && end == kb1;
@@ -283,24 +316,21 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           }
           __syncwarp();
           more = 1;
+          if (!looked) {
+            more_tiles = walk.get_uniform(id, next_w);
+            looked = true;
+          }
         }
         if constexpr (kCut) {
           if (ok && cut_here) {
-            ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, false);
+            const uint32_t parity = (cut_phases >> ring.stage) & 1u;
+            cut_phases ^= 1u << ring.stage;
+            ok = warp_wait(&sh->cut[ring.stage], parity, abort_flag, false);
             if (ok) {
-              // rows [live, steps * 16) belong to the next expert or to nobody
-              uint8_t *a_tile = tiles + ring.stage * C::kStageBytes;
               const int steps = (live + 15) / 16;
-              const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
-              const int chunks = kTileP / 64 + p.tile_q / 64;
-              for (int i = lane; i < chunks * vecs; i += 32) {
-                uint8_t *dst = a_tile + (i / vecs) * kChunkBytes + live * 128 + (i % vecs) * 16;
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
+              tc_fence_after_sync();
               if (chosen) {
-                tc_fence_after_sync();
+                mbar_arrive(&sh->full[ring.stage]); // the stage's turn of this barrier
                 const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
                 for (int k = 0; k < steps; ++k, more = 1)
                   umma_ss(d, da + k * kStepA, db + k * kStepB, idesc, more);
@@ -324,11 +354,50 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         }
         kb = end;
       }
+      if (ok && !looked)
+        more_tiles = walk.get_uniform(id, next_w);
+    }
+  } else if (kCut && warp == 2 + C::kEpiWarps) {
+    // ------------------------------------------------- cutting of last stages
+    // Rows [live, the next multiple of 16) of an expert's last stage belong to the
+    // next expert or to nobody: zero in both operands before they are multiplied.
+    if constexpr (kCut) {
+      TileWalk<kSwap> walk(p, table, kTileP);
+      Tile w;
+      Ring ring;
+      uint32_t phases = 0; // of landed: a bit to a stage
+      for (int id = first_tile; p.ragged == kRaggedK && walk.get_uniform(id, w); id += tile_step) {
+        int kb0, kb1;
+        k_blocks(w, kb0, kb1);
+        const bool cut = has_cut(w, kb0, kb1);
+        ring.stage = (ring.stage + kb1 - kb0 - (cut ? 1 : 0)) % num_stages;
+        if (!cut)
+          continue;
+        const uint32_t parity = (phases >> ring.stage) & 1u;
+        phases ^= 1u << ring.stage;
+        if (!warp_wait(&sh->landed[ring.stage], parity, abort_flag, false)) {
+          report(kStatusWaitTimeout, 3, ring.stage);
+          break;
+        }
+        uint8_t *a_tile = tiles + ring.stage * C::kStageBytes;
+        const int live = w.k_len & (kBK - 1), steps = (live + 15) / 16;
+        const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
+        const int chunks = kTileP / 64 + p.tile_q / 64;
+        for (int c = 0; c < chunks; ++c)
+          for (int i = lane; i < vecs; i += 32)
+            *reinterpret_cast<uint4 *>(a_tile + c * kChunkBytes + live * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&sh->cut[ring.stage]);
+        __syncwarp();
+        ring.stage = (ring.stage + 1) % num_stages;
+      }
     }
   } else {
     // ---------------------------------------------------------- epilogue
     const int quarter = warp & 3; // tensor-memory lanes this warp may read
-    const int col0 = ((warp - 2) >> 2) * kMyCols;
+    const int col0 = ((warp - 2) >> 2) * (kF32 || kSwap ? kMyCols : W);
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const EpiWarp ew = epi_warp;
     TileWalk<kSwap> walk(p, table, kTileP);
@@ -355,7 +424,13 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         acc_phase ^= 1;
       }
     };
-    for (int id = first_tile; ok && walk.get(id, w); id += tile_step) {
+    // (where the next tile lies is worked out while this one's accumulator is waited for)
+    Tile next_w;
+    bool more_tiles = walk.get(first_tile, next_w);
+    for (int id = first_tile; ok && more_tiles;) {
+      w = next_w;
+      id += tile_step;
+      more_tiles = walk.get(id, next_w);
       int kb0, kb1;
       k_blocks(w, kb0, kb1);
       EpiTile t;
@@ -366,7 +441,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       if constexpr (kSwap)
         col_bias = column_bias(p, t, lane);
       // columns of this warp that exist, in chunks of W
-      const int my_cols = min(kMyCols, p.tile_q - col0);
+      const int my_cols = kF32 || kSwap ? min(kMyCols, p.tile_q - col0) : p.tile_q - col0;
       // split: four columns c .. c + 3 of a row side by side, 128 rows of them one after the other
       float4 *part = reinterpret_cast<float4 *>(tiles) + quarter * 32 + lane;
       auto chunk = [&](int c, float (&v)[W], const Ahead<W> &f) {
@@ -426,7 +501,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           break;
         }
 #pragma unroll 1
-        for (int c = 0; c < my_cols; c += W) {
+        for (int c = 0; c < my_cols; c += kStride) {
           float v[W];
           if (empty) {
 #pragma unroll
@@ -435,12 +510,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           } else {
             tmem_load<W>(lane_addr + static_cast<uint32_t>(acc * TN + col0 + c), v);
           }
-          if (!empty && c + W >= my_cols)
+          if (!empty && c + kStride >= my_cols)
             release_acc(); // read out: the tile after the next may use it
-          const Ahead<W> now = next;
-          if (!kSwap && splits == 1 && c + W < my_cols)
-            fetch_ahead<W>(next, p, t, w.q0 + col0 + c + W, lane);
-          chunk(col0 + c, v, now);
+          chunk(col0 + c, v, next);
+          if (!kSwap && splits == 1 && c + kStride < my_cols)
+            fetch_ahead<W>(next, p, t, w.q0 + col0 + c + kStride, lane);
         }
         if (!empty && my_cols <= 0)
           release_acc();
@@ -468,7 +542,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     __syncthreads();
     cluster_arrive();
     cluster_wait();
-    if (warp >= 2 && *abort_flag == 0) {
+    if (warp >= 2 && warp < 2 + C::kEpiWarps && *abort_flag == 0) {
       const int quarter = warp & 3, half = (warp - 2) >> 2;
       const EpiWarp ew = epi_warp;
       TileWalk<kSwap> walk(p, table, kTileP);
@@ -555,7 +629,7 @@ cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearL
     return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
-  cfg.blockDim = dim3(C::kThreads);
+  cfg.blockDim = dim3(kAMn && kBMn ? C::kThreadsCut : C::kThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + static_cast<size_t>(p.stages) * C::kStageBytes + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

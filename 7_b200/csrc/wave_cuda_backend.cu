@@ -136,7 +136,7 @@ void reload_env_knobs() {
 // Lets the library's other translation units record a failure message.
 void set_last_error(const char *message) { g_last_error = message ? message : ""; }
 
-// rank-2 or rank-3 map over 16-bit elements, 128-byte swizzle, zero fill
+// rank-2 to rank-4 map over 16-bit elements, 128-byte swizzle, zero fill
 // outside the tensor.  dims/strides innermost first; strides in bytes for
 // dims 1.. (dim 0 is contiguous).
 int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int rank, const uint64_t *dims,
@@ -144,8 +144,8 @@ int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int r
   EncodeTiledFn fn = encode_fn();
   if (!fn)
     return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  cuuint64_t gdim[3], gstr[2];
-  cuuint32_t bdim[3], estr[3];
+  cuuint64_t gdim[4], gstr[3];
+  cuuint32_t bdim[4], estr[4];
   for (int i = 0; i < rank; ++i) {
     gdim[i] = dims[i];
     bdim[i] = box[i];
@@ -164,18 +164,18 @@ int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int r
   return WAVE_OK;
 }
 
-// Rank-3 map for stores of 32-column blocks out of shared memory rows of 64
-// (16-bit) or 128 (f32) bytes, swizzled by as much.
+// Rank-3 map for stores out of shared memory rows of 128 bytes (64 columns of a
+// 16-bit type, 32 of f32) with the 128-byte swizzle.
 int make_tensor_map_store(CUtensorMap *map, int type, void *base, const uint64_t *dims, const uint64_t *strides_bytes,
                           uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn)
     return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]}, gstr[2] = {strides_bytes[0], strides_bytes[1]};
-  const cuuint32_t box[3] = {32, box_rows, 1}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {type == WAVE_F32 ? 32u : 64u, box_rows, 1}, estr[3] = {1, 1, 1};
   const CUresult r = fn(map, type == WAVE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == WAVE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         3, base, gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        type == WAVE_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (store, dims %llu x %llu x %llu)", static_cast<int>(r),

@@ -182,6 +182,20 @@ int operand_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_cols, i
   return wave::make_tensor_map_16bit(map, is_bf16, o.ptr, 3, dims, strides, box);
 }
 
+// The same seen as [matrices][chunks of 64 columns][rows][64], so that a stage of
+// an MN-major operand is one copy instead of one for each chunk (a copy keeps the
+// loading thread 100 cycles, which with four of them bounded the weight gradient).
+// Only where the columns are whole chunks: a chunk is not cut at the row's end.
+bool chunked(const Operand &o) { return o.cols % 64 == 0; }
+int chunk_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_chunks, int box_rows) {
+  const uint64_t dims[4] = {64, static_cast<uint64_t>(o.rows), static_cast<uint64_t>(o.cols / 64),
+                            static_cast<uint64_t>(o.matrices)};
+  const long long group = o.matrices > 1 ? o.group : o.ld * o.rows;
+  const uint64_t strides[3] = {static_cast<uint64_t>(o.ld) * 2, 128, static_cast<uint64_t>(group) * 2};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(box_chunks), 1};
+  return wave::make_tensor_map_16bit(map, is_bf16, o.ptr, 4, dims, strides, box);
+}
+
 // ------------------------------------------------------------ tile choice
 // What a launch takes is predicted for every tile and split it could have, and
 // the cheapest is taken.  Times in us, fitted to 140 problems (1 to 8192 tokens,
@@ -322,7 +336,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
       if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
         continue;
       // columns of no use are left out where the layout allows: tiles of equal width
-      const int unit = l.b_mn ? (pair ? 128 : 64) : (swap ? 16 : 32);
+      const int unit = swap ? 16 : l.b_mn && pair ? 128 : 64;
       int tile_q = tile_n;
       if (!(swap && s.grouped)) {
         const long long n = (e.q + tile_n - 1) / tile_n;
@@ -357,7 +371,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   if (l.pair) {
     const long long pairs = sms / 2;
     l.grid = static_cast<int>(2 * (best.tiles < pairs ? (best.tiles > 0 ? best.tiles : 1) : pairs));
-    pl.stages = 6; // (the kernel's own constant)
+    pl.stages = 5; // (the kernel's own constant)
     return pl;
   }
   l.grid = static_cast<int>(pl.splits > 1 ? best.tiles * pl.splits : (best.tiles < sms ? best.tiles : sms));
@@ -371,7 +385,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
     const long long k_ext = kind == Product::kForward ? e.K : kind == Product::kInputGrad ? e.N : e.M;
     const long long need = ((k_ext + 63) / 64 + pl.splits - 1) / pl.splits;
     if ((pl.splits > 1 || best.tiles <= sms) && need < pl.stages)
-      pl.stages = need < 4 ? 4 : static_cast<int>(need);
+      pl.stages = need < 3 ? 3 : static_cast<int>(need);
   }
   return pl;
 }
@@ -440,10 +454,13 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   p.vec_r = aligned16(o.R) && d.ldr % 8 == 0;
   p.zero_rest = zero_rest;
   wave::LinearMaps m;
-  int rc = operand_map(&m.a, a, is_bf16, 64, l.a_mn ? 64 : 128);
+  const int b_cols = l.pair ? pl.tile_q / 2 : pl.tile_q; // of one CTA
+  p.chunks_a = l.a_mn && chunked(a);
+  p.chunks_b = l.b_mn && chunked(b);
+  int rc = p.chunks_a ? chunk_map(&m.a, a, is_bf16, 2, 64) : operand_map(&m.a, a, is_bf16, 64, l.a_mn ? 64 : 128);
   if (rc != WAVE_OK)
     return rc;
-  rc = operand_map(&m.b, b, is_bf16, 64, l.b_mn ? 64 : l.pair ? pl.tile_q / 2 : pl.tile_q);
+  rc = p.chunks_b ? chunk_map(&m.b, b, is_bf16, b_cols / 64, 64) : operand_map(&m.b, b, is_bf16, 64, l.b_mn ? 64 : b_cols);
   if (rc != WAVE_OK)
     return rc;
   // Results leave by TMA where their rows allow it: a store cuts a row at a
