@@ -520,8 +520,8 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
   }
 }
 
-// What an epilogue warp has of its own: its slot, 64 floats for the bias, and
-// the tensor maps of D and z (their boxes are a slot: 32 rows of 128 bytes).
+// What an epilogue warp has of its own: its slot and the
+// tensor maps of D and z (their boxes are a slot: 32 rows of 128 bytes).
 //
 // Blocks leave the slot by one TMA store where they can: through the load-store
 // unit a block is read from shared memory and written to L1 a second time, which
@@ -531,7 +531,6 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
 // to be written row by row.
 struct EpiWarp {
   uint8_t *slot;
-  float *bias;
   const CUtensorMap *map_d, *map_z;
   int lane;
 };
@@ -558,43 +557,37 @@ __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *ma
   }
 }
 
-// Tokens as rows: v holds columns q0 .. q0 + W of the lane's row.
-template <bool kF32, int W>
+// Tokens as rows: v holds columns q0 .. q0 + W of the lane's row.  kFull: the
+// forward pass; the products of the backward pass only store.
+template <bool kF32, int W, bool kFull>
 __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
                                               const Ahead<W> &f, const EpiWarp &e) {
   const int lane = e.lane;
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
   if (rows <= 0 || cols <= 0)
     return; // the same for the whole warp
-  const bool whole = rows == 32 || p.ragged != kRaggedRows; // no row behind these is another expert's
-  if (p.bias) { // handed round
+  // No row behind these is another expert's, no column another tile's.
+  const bool whole = (rows == 32 || p.ragged != kRaggedRows) && (q0 + W <= t.q_end || t.q_end == p.Q);
+  if (kFull && p.bias) { // a lane's value handed round (through shared memory it would take a place in the ring of stages)
 #pragma unroll
-    for (int i = 0; i < (W + 31) / 32; ++i)
-      if (lane + 32 * i < W)
-        e.bias[lane + 32 * i] = f.bias[i];
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < W / 4; ++k) {
-      const float4 b = reinterpret_cast<const float4 *>(e.bias)[k];
-      const float2 lo = __fadd2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(b.x, b.y));
-      const float2 hi = __fadd2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(b.z, b.w));
-      v[4 * k] = lo.x;
-      v[4 * k + 1] = lo.y;
-      v[4 * k + 2] = hi.x;
-      v[4 * k + 3] = hi.y;
+    for (int j = 0; j < W; j += 2) {
+      const float2 sum = __fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(__shfl_sync(0xffffffffu, f.bias[j / 32], j % 32),
+                                                                             __shfl_sync(0xffffffffu, f.bias[j / 32], j % 32 + 1)));
+      v[j] = sum.x;
+      v[j + 1] = sum.y;
     }
-    __syncwarp();
   }
-  if (p.Z) {
+  if (kFull && p.Z) {
     slot_wait(e);
     row_to_slot_16bit<W>(e.slot, v, p.is_bf16, lane);
     slot_out<2, W>(e, e.map_z, p.tma_z && whole, static_cast<uint16_t *>(p.Z) + static_cast<long long>(t.lane0) * p.ldz + q0,
                    p.ldz, rows, cols, p.vec_z != 0, q0, t.lane0, 0);
   }
-  apply_act<W>(v, p.act);
+  if constexpr (kFull)
+    apply_act<W>(v, p.act);
   slot_wait(e);
   uint8_t *slot = e.slot;
-  if (p.R) {
+  if (kFull && p.R) {
     using S = Slot<2, W>;
     constexpr int kRowStep = 32 / S::kPieces;
 #pragma unroll

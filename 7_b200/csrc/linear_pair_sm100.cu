@@ -37,23 +37,24 @@ constexpr int kChunkBytes = 64 * 128;
 constexpr int kABytes = kRows * kBK * 2;
 constexpr int kBBytes = kTN / 2 * kBK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStages = 5; // (six, with slots of half the size: 0.5 % on a bare 8192^3, lost again in the epilogue)
+constexpr int kMaxStages = 6; // five where the experts' table is long
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kThreadsCut = kThreads + 32; // the weight gradient has a warp that cuts
 constexpr int kW = 64; // columns of an epilogue chunk; the two groups of four warps take them in turn
-constexpr int kSlots = kEpiWarps * (kSlotBytes + 64 * 4); // and the bias
-constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
-constexpr int kSmemFixed = 1024 + kStages * kStageBytes + 1024 + kSlots;
-static_assert(kSmemFixed + kTableBytes <= 227 * 1024, "does not fit the shared memory of an SM");
+constexpr int kSlots = kEpiWarps * kSlotBytes;
+constexpr int kSmemLimit = 227 * 1024;
+constexpr int kSmemFixed = 1024 + 1024 + kSlots; // + the stages, the group table
+static_assert(kSmemFixed + 5 * kStageBytes + linear_table_bytes(kRaggedRows, kLinearMaxGroups) <= kSmemLimit,
+              "does not fit the shared memory of an SM");
 
 struct PairShared {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
   uint64_t tfull[2];
   uint64_t tempty[2];
-  uint64_t landed[kStages];
-  uint64_t cut[kStages];
+  uint64_t landed[kMaxStages];
+  uint64_t cut[kMaxStages];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -85,11 +86,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAMn && kBMn ? kThre
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
                    const __grid_constant__ LinearParams p) {
+  constexpr bool kFull = !kAMn && !kBMn; // the forward pass
   constexpr bool kCut = kAMn && kBMn;
+  const int num_stages = p.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  PairShared *sh = reinterpret_cast<PairShared *>(tiles + kStages * kStageBytes);
-  uint8_t *slots = tiles + kStages * kStageBytes + 1024;
+  PairShared *sh = reinterpret_cast<PairShared *>(tiles + num_stages * kStageBytes);
+  uint8_t *slots = tiles + num_stages * kStageBytes + 1024;
   GroupTable table;
   table.begin = reinterpret_cast<int *>(slots + kSlots);
   table.blocks = table.begin + p.groups + 1;
@@ -104,7 +107,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_a);
     tma_prefetch_desc(&tm_b);
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < num_stages; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
       mbar_init(&sh->landed[s], 1);
@@ -161,7 +164,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         uint64_t *bar = &sh->full[ring.stage];
         uint64_t *landed = &sh->landed[ring.stage];
         const int k = w.k_begin + kb * kBK;
-        ring.advance(kStages);
+        ring.advance(num_stages);
         seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
         if (kCut && is_cut(live_of(w, kb))) {
           if (chosen) {
@@ -256,7 +259,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             tc_fence_after_sync();
             const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
             uint64_t *done = &sh->empty[ring.stage];
-            ring.advance(kStages);
+            ring.advance(num_stages);
             seen = warp_peek(&sh->full[ring.stage], ring.phase);
             if (chosen) {
               umma_ss_pair(d, da, db, idesc, more);
@@ -294,7 +297,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
                 umma_commit_pair(&sh->empty[ring.stage], 3);
               }
               __syncwarp();
-              ring.advance(kStages);
+              ring.advance(num_stages);
             }
           }
           if (chosen)
@@ -322,7 +325,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           continue;
         const int live = live_of(w, kbs - 1);
         const bool cut = is_cut(live);
-        ring.stage = (ring.stage + kbs - (cut ? 1 : 0)) % kStages;
+        ring.stage = (ring.stage + kbs - (cut ? 1 : 0)) % num_stages;
         if (!cut)
           continue;
         const uint32_t parity = (phases >> ring.stage) & 1u;
@@ -343,7 +346,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         if (lane == 0)
           mbar_arrive_cluster(map_to_cta(&sh->cut[ring.stage], 0));
         __syncwarp();
-        ring.stage = (ring.stage + 1) % kStages;
+        ring.stage = (ring.stage + 1) % num_stages;
       }
     }
   } else {
@@ -351,8 +354,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const int quarter = warp & 3;
     const int col0 = ((warp - 2) >> 2) * kW;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const EpiWarp ew{slots + (warp - 2) * kSlotBytes, reinterpret_cast<float *>(slots + kEpiWarps * kSlotBytes) + (warp - 2) * 64,
-                     &tm_d, &tm_z, lane};
+    const EpiWarp ew{slots + (warp - 2) * kSlotBytes, &tm_d, &tm_z, lane};
     const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
     TileWalk<false> walk(p, table, kPairP);
     Tile w;
@@ -383,7 +385,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       t.q_end = min(w.q_end, w.q0 + p.tile_q);
       const int my_cols = p.tile_q - col0;
       Ahead<kW> next;
-      if (my_cols > 0)
+      if (kFull && my_cols > 0)
         fetch_ahead<kW>(next, p, t, w.q0 + col0, lane);
       if (!empty) {
         if (!mbar_wait(&sh->tfull[acc], acc_phase, abort_flag)) {
@@ -412,8 +414,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           if (c + 2 * kW >= my_cols)
             release(); // read out: the tile after the next may use it
         }
-        epilogue_rows<false, kW>(p, t, w.q0 + col0 + c, v, next, ew);
-        if (c + 2 * kW < my_cols)
+        epilogue_rows<false, kW, kFull>(p, t, w.q0 + col0 + c, v, next, ew);
+        if (kFull && c + 2 * kW < my_cols)
           fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + 2 * kW, lane);
       }
       if (!empty && my_cols <= 0)
@@ -447,14 +449,17 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 
 template <bool kAMn, bool kBMn>
 cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
+  if (p.stages != linear_pair_stages(p.ragged, p.groups))
+    return cudaErrorInvalidValue;
   auto kernel = linear_pair_kernel<kAMn, kBMn>;
-  cudaError_t err = prepare_kernel(kernel, kSmemFixed + kTableBytes, nullptr);
+  cudaError_t err = prepare_kernel(kernel, kSmemLimit, nullptr);
   if (err != cudaSuccess)
     return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
   cfg.blockDim = dim3(kAMn && kBMn ? kThreadsCut : kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(kSmemFixed) + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
+  cfg.dynamicSmemBytes = static_cast<size_t>(kSmemFixed) + static_cast<size_t>(p.stages) * kStageBytes +
+                         linear_table_bytes(p.ragged, p.groups);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -465,6 +470,11 @@ cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearL
 }
 
 } // namespace
+
+int linear_pair_stages(int ragged, int groups) {
+  const int fit = (kSmemLimit - kSmemFixed - linear_table_bytes(ragged, groups)) / kStageBytes;
+  return fit < kMaxStages ? fit : kMaxStages;
+}
 
 cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
   if (!l.a_mn)

@@ -47,7 +47,7 @@ constexpr int kABytes = kTileP * kBK * 2;
 constexpr int kMaxStages = 12;
 constexpr int kMinStages = 3;
 constexpr int kSegment = 8; // stages of an accumulator that is summed in registers
-constexpr int kTableBytes = 2 * 4 * (kLinearMaxGroups + 1) + 8;
+constexpr int kTableBytes = linear_table_bytes(kRaggedRows, kLinearMaxGroups);
 constexpr int kSmemLimit = 227 * 1024;
 
 struct Shared {
@@ -70,13 +70,15 @@ template <int TN, bool kF32> struct Cfg {
   static constexpr int kThreadsCut = kThreads + 32; // the weight gradient has a warp that cuts
   static constexpr int kBBytes = TN * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kBias = kEpiWarps * 64 * 4;
-  static constexpr int kSlots = kEpiWarps * kSlotBytes + kBias;
-  static constexpr int kFit = (kSmemLimit - 1024 - 1024 - kTableBytes - kSlots) / kStageBytes;
-  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  static constexpr int kSlots = kEpiWarps * kSlotBytes;
+  // Stages that fit beside a table of so many bytes.
+  static constexpr int stages(int table) {
+    const int fit = (kSmemLimit - kSmemFixed - table) / kStageBytes;
+    return fit < kMaxStages ? fit : kMaxStages;
+  }
   static constexpr int kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
   static constexpr int kSmemFixed = 1024 + 1024 + kSlots; // + the stages, the group table
-  static_assert(kStages >= kMinStages, "ring too short");
+  static_assert((kSmemLimit - kSmemFixed - kTableBytes) / kStageBytes >= kMinStages, "ring too short");
   static_assert(TN * kTileP * 4 <= kMinStages * kStageBytes, "a partial tile must fit the shortest ring");
 };
 
@@ -120,6 +122,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               const __grid_constant__ LinearParams p) {
   using C = Cfg<TN, kF32>;
   const int num_stages = p.stages;
+  constexpr bool kFull = !kAMn && !kBMn; // the forward pass
   constexpr bool kCut = kAMn && kBMn; // the weight gradient: stages may have to be cut at the last row
   constexpr int kColGroups = C::kEpiWarps / 4;
   constexpr int kMyCols = TN / kColGroups; // columns of an epilogue warp
@@ -181,7 +184,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
 
   EpiWarp epi_warp;
   epi_warp.slot = slots + (warp - 2) * kSlotBytes;
-  epi_warp.bias = reinterpret_cast<float *>(slots + C::kEpiWarps * kSlotBytes) + (warp - 2) * 64;
   epi_warp.map_d = &tm_d;
   epi_warp.map_z = &tm_z;
   epi_warp.lane = lane;
@@ -452,7 +454,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         } else if constexpr (kSwap) {
           epilogue_columns<kF32, W>(p, t, w.q0 + c, v, col_bias, ew.slot, lane);
         } else {
-          epilogue_rows<kF32, W>(p, t, w.q0 + c, v, f, ew);
+          epilogue_rows<kF32, W, kFull>(p, t, w.q0 + c, v, f, ew);
         }
       };
       if constexpr (kF32) {
@@ -483,7 +485,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (c >= my_cols)
             break;
           Ahead<W> f;
-          if (!kSwap && splits == 1)
+          if (!kSwap && kFull && splits == 1)
             fetch_ahead<W>(f, p, t, w.q0 + col0 + c, lane);
           float v[W];
 #pragma unroll
@@ -494,7 +496,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       } else {
         const bool empty = kb0 == kb1; // nothing to multiply: the epilogue of zero
         Ahead<W> next;
-        if (!kSwap && splits == 1 && my_cols > 0)
+        if (!kSwap && kFull && splits == 1 && my_cols > 0)
           fetch_ahead<W>(next, p, t, w.q0 + col0, lane);
         if (!empty && !wait_acc()) {
           ok = false;
@@ -513,7 +515,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (!empty && c + kStride >= my_cols)
             release_acc(); // read out: the tile after the next may use it
           chunk(col0 + c, v, next);
-          if (!kSwap && splits == 1 && c + kStride < my_cols)
+          if (!kSwap && kFull && splits == 1 && c + kStride < my_cols)
             fetch_ahead<W>(next, p, t, w.q0 + col0 + c + kStride, lane);
         }
         if (!empty && my_cols <= 0)
@@ -588,7 +590,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           for (int i = rank + half * splits; i * V < p.tile_q; i += kColGroups * splits) {
             const int q0 = w.q0 + i * V;
             Ahead<V> f;
-            fetch_ahead<V>(f, p, t, q0, lane);
+            if constexpr (kFull)
+              fetch_ahead<V>(f, p, t, q0, lane);
             float v[V];
 #pragma unroll
             for (int j = 0; j < V; j += 4) {
@@ -598,7 +601,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               v[j + 2] = q.z;
               v[j + 3] = q.w;
             }
-            epilogue_rows<kF32, V>(p, t, q0, v, f, ew);
+            epilogue_rows<kF32, V, kFull>(p, t, q0, v, f, ew);
           }
         }
       }
@@ -623,14 +626,16 @@ template <int TN, bool kAMn, bool kBMn, bool kSwap, bool kF32>
 cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l,
                        cudaStream_t stream) {
   using C = Cfg<TN, kF32>;
+  if (p.stages < kMinStages || p.stages > C::stages(linear_table_bytes(p.ragged, p.groups)))
+    return cudaErrorInvalidValue;
   auto kernel = linear_kernel<TN, kAMn, kBMn, kSwap, kF32>;
-  cudaError_t err = prepare_kernel(kernel, C::kSmemFixed + C::kStages * C::kStageBytes + kTableBytes, nullptr);
+  cudaError_t err = prepare_kernel(kernel, kSmemLimit, nullptr);
   if (err != cudaSuccess)
     return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.grid));
   cfg.blockDim = dim3(kAMn && kBMn ? C::kThreadsCut : C::kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + static_cast<size_t>(p.stages) * C::kStageBytes + (p.ragged != kRaggedNone ? 2 * 4 * (p.groups + 1) + 8 : 0);
+  cfg.dynamicSmemBytes = static_cast<size_t>(C::kSmemFixed) + static_cast<size_t>(p.stages) * C::kStageBytes + linear_table_bytes(p.ragged, p.groups);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.numAttrs = 0;
@@ -691,14 +696,15 @@ cudaError_t launch_layout(const LinearMaps &m, const LinearParams &p, const Line
 
 } // namespace
 
-int linear_max_stages(int tile_n, int out_f32) {
+int linear_max_stages(int tile_n, int out_f32, int ragged, int groups) {
+  const int table = linear_table_bytes(ragged, groups);
   switch (tile_n) {
-  case 16: return out_f32 ? Cfg<16, true>::kStages : Cfg<16, false>::kStages;
-  case 32: return out_f32 ? Cfg<32, true>::kStages : Cfg<32, false>::kStages;
-  case 64: return out_f32 ? Cfg<64, true>::kStages : Cfg<64, false>::kStages;
-  case 128: return out_f32 ? Cfg<128, true>::kStages : Cfg<128, false>::kStages;
+  case 16: return out_f32 ? Cfg<16, true>::stages(table) : Cfg<16, false>::stages(table);
+  case 32: return out_f32 ? Cfg<32, true>::stages(table) : Cfg<32, false>::stages(table);
+  case 64: return out_f32 ? Cfg<64, true>::stages(table) : Cfg<64, false>::stages(table);
+  case 128: return out_f32 ? Cfg<128, true>::stages(table) : Cfg<128, false>::stages(table);
   }
-  return Cfg<256, false>::kStages;
+  return Cfg<256, false>::stages(table);
 }
 
 cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {

@@ -44,7 +44,7 @@ struct LinearParams {
   const int *offsets; // [groups + 1], on the device; null when not ragged
   int group_a, group_b; // the operand has one matrix for each group (third coordinate of its tensor map)
   int chunks_a, chunks_b; // an MN-major operand's map is one over 64-column chunks: a stage of it is one copy
-  int tile_q;        // columns of a tile <= the kernel's: a multiple of 16 with `swap`, else of 64
+  int tile_q;        // columns of a tile <= the kernel's: a multiple of 16, of 64 where B is stored [K][Q]
   int p_blocks, q_blocks; // tiles along each side (ragged side: unused)
   int raster_log2;   // row blocks (its power of two) that are walked down before the next column block
   FastDiv band_tiles;  // tiles of so many row blocks
@@ -78,14 +78,17 @@ struct LinearLaunch {
   int pdl;        // launch with programmatic stream serialization
 };
 
-// Ring depth the kernel has room for; a launch may take fewer stages, at least 3.
-int linear_max_stages(int tile_n, int out_f32);
+// Bytes of the experts' table in shared memory.
+constexpr int linear_table_bytes(int ragged, int groups) { return ragged == kRaggedNone ? 0 : 2 * 4 * (groups + 1); }
+// Ring depth the kernel has room for beside it; a launch may take fewer stages, at least 3.
+int linear_max_stages(int tile_n, int out_f32, int ragged, int groups);
+int linear_pair_stages(int ragged, int groups); // (taken whole)
 struct LinearMaps {
   CUtensorMap a, b, d, z; // d and z: read where tma_d / tma_z are set, boxes of 128 bytes x 32 rows
 };
 cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_read_status(int out[4], bool clear);
-// tile_q a multiple of 64 (of 128 where B is stored [K][Q]) up to 256; grid even.
+// tile_q a multiple of 32 (of 128 where B is stored [K][Q]) up to 256; grid even.
 cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_pair_read_status(int out[4], bool clear);
 

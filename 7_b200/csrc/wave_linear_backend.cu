@@ -143,6 +143,10 @@ int validate(const wave_linear_desc *d) {
 // ------------------------------------------------------------------ products
 enum class Product { kForward, kInputGrad, kWeightGrad };
 
+int ragged_of(Product kind, const Shape &s) {
+  return !s.grouped ? wave::kRaggedNone : kind == Product::kWeightGrad ? wave::kRaggedK : wave::kRaggedRows;
+}
+
 // One 16-bit operand as the tensor maps see it: `rows` x `cols` of each matrix,
 // cols contiguous.
 struct Operand {
@@ -336,7 +340,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
       if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
         continue;
       // columns of no use are left out where the layout allows: tiles of equal width
-      const int unit = swap ? 16 : l.b_mn && pair ? 128 : 64;
+      const int unit = l.b_mn ? (pair ? 128 : 64) : (pair ? 32 : 16);
       int tile_q = tile_n;
       if (!(swap && s.grouped)) {
         const long long n = (e.q + tile_n - 1) / tile_n;
@@ -371,7 +375,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   if (l.pair) {
     const long long pairs = sms / 2;
     l.grid = static_cast<int>(2 * (best.tiles < pairs ? (best.tiles > 0 ? best.tiles : 1) : pairs));
-    pl.stages = 5; // (the kernel's own constant)
+    pl.stages = wave::linear_pair_stages(ragged_of(kind, s), s.matrices);
     return pl;
   }
   l.grid = static_cast<int>(pl.splits > 1 ? best.tiles * pl.splits : (best.tiles < sms ? best.tiles : sms));
@@ -380,7 +384,7 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
   // A CTA with one tile takes no more stages than that has: what it leaves of the
   // SM lets the next kernel of the stream set itself up meanwhile (one token,
   // 2048 x 2048: 12.3 -> 6.5 us).
-  pl.stages = wave::linear_max_stages(l.tile_n, l.out_f32);
+  pl.stages = wave::linear_max_stages(l.tile_n, l.out_f32, ragged_of(kind, s), s.matrices);
   if (kind != Product::kWeightGrad || !s.grouped) {
     const long long k_ext = kind == Product::kForward ? e.K : kind == Product::kInputGrad ? e.N : e.M;
     const long long need = ((k_ext + 63) / 64 + pl.splits - 1) / pl.splits;
@@ -424,7 +428,7 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
     p.Q = d.in_features;
     p.K = d.tokens;
   }
-  p.ragged = !s.grouped ? wave::kRaggedNone : kind == Product::kWeightGrad ? wave::kRaggedK : wave::kRaggedRows;
+  p.ragged = ragged_of(kind, s);
   p.groups = s.matrices;
   p.offsets = s.grouped ? offsets : nullptr;
   p.tile_q = pl.tile_q;

@@ -146,7 +146,7 @@ def test_every_plan_can_run(wc, knobs):
                 p = wc.linear_plan_for_sms(d, product, sms)
                 pair = p["tile_rows"] == 256
                 f32 = product != 1 and d.y_type == wc.F32
-                unit = 16 if p["tokens_on_columns"] else 128 if pair and product else 64
+                unit = (128 if pair else 64) if product else (32 if pair else 16)
                 assert p["tile_columns"] % unit == 0 and unit <= p["tile_columns"] <= (128 if f32 else 256), (m, n, k, p)
                 assert 1 <= p["splits"] <= 8 and p["grid"] >= 1 and p["grid"] % p["splits"] == 0
                 assert 3 <= p["stages"] <= 12
