@@ -521,7 +521,7 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
 }
 
 // What an epilogue warp has of its own: its slot and the
-// tensor maps of D and z (their boxes are a slot: 32 rows of 128 bytes).
+// tensor maps of D and z (their boxes are what it takes: 32 rows).
 //
 // Blocks leave the slot by one TMA store where they can: through the load-store
 // unit a block is read from shared memory and written to L1 a second time, which
@@ -529,21 +529,32 @@ __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, 
 // each: 3100 of a tile's 5500 cycles).  The store cuts what lies behind the
 // tensor's last row or column; only a block that ends at an expert's last row has
 // to be written row by row.
+// Blocks of 64 bytes a row (the forward pass in 16 bits: 32 columns, whose
+// arithmetic needs the registers) take the slot's halves in turn, so that one is
+// filled while a store reads the other; rows of 128 bytes take it whole.
 struct EpiWarp {
   uint8_t *slot;
   const CUtensorMap *map_d, *map_z;
   int lane;
+  int other_half = kSlotBytes / 2; // from the half in use to the other
 };
-// The slot may be written: the stores that read it have done so.
-__device__ __forceinline__ void slot_wait(const EpiWarp &e) {
-  if (e.lane == 0)
-    tma_store_wait_read<0>();
+// Takes the slot, or its other half: the stores that read it have done so.
+template <bool kHalves> __device__ __forceinline__ void slot_next(EpiWarp &e) {
+  if constexpr (kHalves) {
+    e.slot += e.other_half;
+    e.other_half = -e.other_half;
+    if (e.lane == 0)
+      tma_store_wait_read<1>();
+  } else {
+    if (e.lane == 0)
+      tma_store_wait_read<0>();
+  }
   __syncwarp();
 }
 template <int kElem, int W>
 __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *map, bool tma, void *base, long long ld, int rows,
                                          int cols, bool vec, int q0, int p0, int group) {
-  if (W * kElem == 128 && tma) {
+  if (W * kElem >= 64 && tma) {
     fence_proxy_async_smem();
     __syncwarp();
     if (e.lane == 0) {
@@ -561,7 +572,8 @@ __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *ma
 // forward pass; the products of the backward pass only store.
 template <bool kF32, int W, bool kFull>
 __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTile &t, int q0, float (&v)[W],
-                                              const Ahead<W> &f, const EpiWarp &e) {
+                                              const Ahead<W> &f, EpiWarp &e) {
+  constexpr bool kHalves = !kF32 && W * 2 == 64;
   const int lane = e.lane;
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
   if (rows <= 0 || cols <= 0)
@@ -578,14 +590,14 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
     }
   }
   if (kFull && p.Z) {
-    slot_wait(e);
+    slot_next<kHalves>(e);
     row_to_slot_16bit<W>(e.slot, v, p.is_bf16, lane);
     slot_out<2, W>(e, e.map_z, p.tma_z && whole, static_cast<uint16_t *>(p.Z) + static_cast<long long>(t.lane0) * p.ldz + q0,
                    p.ldz, rows, cols, p.vec_z != 0, q0, t.lane0, 0);
   }
   if constexpr (kFull)
     apply_act<W>(v, p.act);
-  slot_wait(e);
+  slot_next<kHalves>(e);
   uint8_t *slot = e.slot;
   if (kFull && p.R) {
     using S = Slot<2, W>;

@@ -41,7 +41,6 @@ constexpr int kMaxStages = 6; // five where the experts' table is long
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kThreadsCut = kThreads + 32; // the weight gradient has a warp that cuts
-constexpr int kW = 64; // columns of an epilogue chunk; the two groups of four warps take them in turn
 constexpr int kSlots = kEpiWarps * kSlotBytes;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kSmemFixed = 1024 + 1024 + kSlots; // + the stages, the group table
@@ -87,6 +86,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
                    const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
                    const __grid_constant__ LinearParams p) {
   constexpr bool kFull = !kAMn && !kBMn; // the forward pass
+  constexpr int kW = kFull ? 32 : 64; // columns of an epilogue chunk (see linear_sm100.cu); the two groups of four warps take turns
   constexpr bool kCut = kAMn && kBMn;
   const int num_stages = p.stages;
   extern __shared__ uint8_t smem_raw[];
@@ -354,7 +354,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const int quarter = warp & 3;
     const int col0 = ((warp - 2) >> 2) * kW;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const EpiWarp ew{slots + (warp - 2) * kSlotBytes, &tm_d, &tm_z, lane};
+    EpiWarp ew{slots + (warp - 2) * kSlotBytes, &tm_d, &tm_z, lane};
     const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
     TileWalk<false> walk(p, table, kPairP);
     Tile w;
@@ -406,7 +406,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           uint32_t r[kW];
           const uint32_t at = lane_addr + static_cast<uint32_t>(acc * kTN + col0 + c);
           tmem_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-          tmem_ld_32x32b_x32(at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+          if constexpr (kW == 64)
+            tmem_ld_32x32b_x32(at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < kW; ++j)

@@ -126,10 +126,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   constexpr bool kCut = kAMn && kBMn; // the weight gradient: stages may have to be cut at the last row
   constexpr int kColGroups = C::kEpiWarps / 4;
   constexpr int kMyCols = TN / kColGroups; // columns of an epilogue warp
-  // Columns of a chunk: tokens as rows and 16-bit results take 64, rows of 128
-  // bytes.  (With 32 the fixed cost of a chunk -- fence, store, waits -- and its
-  // latencies came twice as often: 1400 cycles each, which bounded short sums.)
-  constexpr int W = kSwap || kF32 ? (kMyCols < 32 ? kMyCols : 32) : 64;
+  // Columns of a chunk.  What only stores takes 64 (of 16 bits: rows of 128 bytes;
+  // with 32 the fixed cost of a chunk -- fence, store, waits -- and its latencies
+  // come twice as often, 1400 cycles each, which bounded short sums); the forward
+  // pass has no registers for more than 32 (8192 x 8192 x 2048 with everything:
+  // 222 us, 235 with 64).
+  constexpr int W = kSwap || kF32 || kFull ? (kMyCols < 32 ? kMyCols : 32) : 64;
   // The groups of four warps take chunks in turn.
   constexpr int kStride = kF32 || kSwap ? W : W * kColGroups;
   static_assert(!kF32 || kMyCols <= 64, "running sums stay in registers");
@@ -401,7 +403,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     const int quarter = warp & 3; // tensor-memory lanes this warp may read
     const int col0 = ((warp - 2) >> 2) * (kF32 || kSwap ? kMyCols : W);
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const EpiWarp ew = epi_warp;
+    EpiWarp ew = epi_warp;
     TileWalk<kSwap> walk(p, table, kTileP);
     Tile w;
     int acc = 0;
@@ -546,7 +548,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     cluster_wait();
     if (warp >= 2 && warp < 2 + C::kEpiWarps && *abort_flag == 0) {
       const int quarter = warp & 3, half = (warp - 2) >> 2;
-      const EpiWarp ew = epi_warp;
+      EpiWarp ew = epi_warp;
       TileWalk<kSwap> walk(p, table, kTileP);
       Tile w;
       if (walk.get(first_tile, w)) {

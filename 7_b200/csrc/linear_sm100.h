@@ -84,7 +84,7 @@ constexpr int linear_table_bytes(int ragged, int groups) { return ragged == kRag
 int linear_max_stages(int tile_n, int out_f32, int ragged, int groups);
 int linear_pair_stages(int ragged, int groups); // (taken whole)
 struct LinearMaps {
-  CUtensorMap a, b, d, z; // d and z: read where tma_d / tma_z are set, boxes of 128 bytes x 32 rows
+  CUtensorMap a, b, d, z; // d and z: read where tma_d / tma_z are set, boxes of 64 (forward, 16-bit) or 128 bytes x 32 rows
 };
 cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_read_status(int out[4], bool clear);

@@ -164,18 +164,18 @@ int make_tensor_map_16bit(CUtensorMap *map, int is_bf16, const void *base, int r
   return WAVE_OK;
 }
 
-// Rank-3 map for stores out of shared memory rows of 128 bytes (64 columns of a
-// 16-bit type, 32 of f32) with the 128-byte swizzle.
+// Rank-3 map for stores out of shared memory rows of 64 or 128 bytes, swizzled by
+// as much.
 int make_tensor_map_store(CUtensorMap *map, int type, void *base, const uint64_t *dims, const uint64_t *strides_bytes,
-                          uint32_t box_rows) {
+                          uint32_t row_bytes, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn)
     return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]}, gstr[2] = {strides_bytes[0], strides_bytes[1]};
-  const cuuint32_t box[3] = {type == WAVE_F32 ? 32u : 64u, box_rows, 1}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {row_bytes / (type == WAVE_F32 ? 4 : 2), box_rows, 1}, estr[3] = {1, 1, 1};
   const CUresult r = fn(map, type == WAVE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == WAVE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         3, base, gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(WAVE_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (store, dims %llu x %llu x %llu)", static_cast<int>(r),

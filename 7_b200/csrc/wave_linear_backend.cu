@@ -14,7 +14,7 @@
 namespace wave { // wave_cuda_backend.cu
 void set_last_error(const char *message);
 int make_tensor_map_store(CUtensorMap *map, int type, void *base, const uint64_t *dims, const uint64_t *strides_bytes,
-                          uint32_t box_rows);
+                          uint32_t row_bytes, uint32_t box_rows);
 }
 
 namespace {
@@ -473,12 +473,13 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   m.d = m.z = m.a;
   if (!l.swap && pl.splits == 1) {
     const bool per_group = p.ragged == wave::kRaggedK;
+    const uint32_t row_bytes = kind == Product::kForward && !out_f32 ? 64 : 128; // of a chunk of the epilogue
     const uint64_t rows = static_cast<uint64_t>(p.P), cols = static_cast<uint64_t>(p.Q);
     if (p.vec_d && p.Q * o.elem % 16 == 0) {
       const uint64_t dims[3] = {cols, rows, per_group ? static_cast<uint64_t>(s.matrices) : 1};
       const uint64_t row = static_cast<uint64_t>(o.ldd) * o.elem;
       const uint64_t strides[2] = {row, per_group ? static_cast<uint64_t>(o.group_d) * o.elem : row * rows};
-      rc = wave::make_tensor_map_store(&m.d, out_f32 ? WAVE_F32 : d.io_type, o.D, dims, strides, 32);
+      rc = wave::make_tensor_map_store(&m.d, out_f32 ? WAVE_F32 : d.io_type, o.D, dims, strides, row_bytes, 32);
       if (rc != WAVE_OK)
         return rc;
       p.tma_d = 1;
@@ -486,7 +487,7 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
     if (p.Z && p.vec_z && p.Q % 8 == 0) {
       const uint64_t dims[3] = {cols, rows, 1}, row = static_cast<uint64_t>(d.ldz) * 2;
       const uint64_t strides[2] = {row, row * rows};
-      if ((rc = wave::make_tensor_map_store(&m.z, d.io_type, o.Z, dims, strides, 32)) != WAVE_OK)
+      if ((rc = wave::make_tensor_map_store(&m.z, d.io_type, o.Z, dims, strides, 64, 32)) != WAVE_OK)
         return rc;
       p.tma_z = 1;
     }
