@@ -29,27 +29,35 @@ cudaError_t launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, int
 // ------------------------------------------------------------------- packing
 // Eight elements to a thread, neighbouring threads on neighbouring pieces of a
 // row; the source may start at any element, so it is read 2 bytes at a time
-// (a warp still reads 512 consecutive bytes) and written 16.
-__global__ void __launch_bounds__(256)
-pack_rows_kernel(const uint16_t *src, long long ld_src, long long group_src, uint16_t *dst, long long ld_dst,
-                 long long group_dst, int rows, int cols, int pieces) {
+// (a warp still reads 512 consecutive bytes) and written 16.  Up to two operands
+// of a call in one launch: matrices [0, first.groups) of the grid's second
+// dimension are the first's.
+struct PackTwo {
+  PackRows first, second;
+};
+__global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackTwo two) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long total = static_cast<long long>(rows) * pieces;
-  const uint16_t *s = src + blockIdx.y * group_src;
-  uint16_t *d = dst + blockIdx.y * group_dst;
+  const int y = static_cast<int>(blockIdx.y);
+  const bool second = y >= two.first.groups;
+  const PackRows &p = second ? two.second : two.first;
+  const int g = second ? y - two.first.groups : y;
+  const int pieces = (p.cols + 7) / 8;
+  const long long total = static_cast<long long>(p.rows) * pieces;
+  const uint16_t *s = static_cast<const uint16_t *>(p.src) + g * p.group_src;
+  uint16_t *d = static_cast<uint16_t *>(p.dst) + g * p.group_dst;
   for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * blockDim.x) {
     const long long r = i / pieces;
     const int c = static_cast<int>(i - r * pieces) * 8;
-    const uint16_t *row = s + r * ld_src + c;
+    const uint16_t *row = s + r * p.ld_src + c;
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = c + 2 * e < cols ? row[2 * e] : 0u, hi = c + 2 * e + 1 < cols ? row[2 * e + 1] : 0u;
+      const uint32_t lo = c + 2 * e < p.cols ? row[2 * e] : 0u, hi = c + 2 * e + 1 < p.cols ? row[2 * e + 1] : 0u;
       w[e] = lo | (hi << 16);
     }
-    *reinterpret_cast<uint4 *>(d + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4 *>(d + r * p.ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -117,6 +125,62 @@ template <bool kF32> __device__ __forceinline__ Eight values(const Raw<kF32> &r,
   return out;
 }
 
+// Rows r, r + kLanes, ... below r1 of eight columns: dz written, its column sums added to acc.
+template <int kAct, bool kDyF32, bool kVec, int kLanes>
+__device__ __forceinline__ void act_grad_rows(const LinearActGrad &p, int r, int r1, int col, int live, float (&acc)[8]) {
+  for (; r < r1; r += kLanes * kAgUnroll) {
+    Raw<kDyF32> dy_raw[kAgUnroll];
+    Raw<false> z_raw[kAgUnroll];
+#pragma unroll
+    for (int u = 0; u < kAgUnroll; ++u) {
+      const int row = r + u * kLanes;
+      if (row < r1) {
+        load_raw<kDyF32, kVec>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
+        if constexpr (kAct >= 0)
+          load_raw<false, kVec>(z_raw[u], p.Z, static_cast<long long>(row) * p.ldz + col, live);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAgUnroll; ++u) {
+      const int row = r + u * kLanes;
+      if (row >= r1)
+        break;
+      Eight g = values<kDyF32>(dy_raw[u], p.is_bf16);
+      if constexpr (kAct >= 0) {
+        const Eight z = values<false>(z_raw[u], p.is_bf16);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 d = __fmul2_rn(make_float2(g.v[e], g.v[e + 1]), slope_pair<kAct>(make_float2(z.v[e], z.v[e + 1])));
+          g.v[e] = d.x;
+          g.v[e + 1] = d.y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 sum = __fadd2_rn(make_float2(acc[e], acc[e + 1]), make_float2(g.v[e], g.v[e + 1]));
+        acc[e] = sum.x;
+        acc[e + 1] = sum.y;
+      }
+      if (p.dZ) {
+        // rows of dZ are padded to whole 16-byte pieces; columns behind the last are zero (0 * slope(0))
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack_pair(g.v[2 * e], g.v[2 * e + 1], p.is_bf16);
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dZ) + static_cast<long long>(row) * p.lddz + col) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+__device__ __forceinline__ void store_dbias(const LinearActGrad &p, int group, int col, float v) {
+  const long long at = static_cast<long long>(group) * p.cols + col;
+  if (p.dbias_type == 0)
+    static_cast<float *>(p.dbias)[at] = v;
+  else
+    static_cast<uint16_t *>(p.dbias)[at] = to_16bit(v, p.dbias_type == 2);
+}
+
 // One chunk of rows x 256 columns to a block.  A chunk never crosses a group's
 // end, so its column sums go to one group; which rows chunk `blockIdx.y` has
 // comes from the offsets, on the device.
@@ -161,53 +225,8 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
-  if (live > 0) {
-    for (int r = r0 + tr; r < r1; r += kAgLanes * kAgUnroll) {
-      Raw<kDyF32> dy_raw[kAgUnroll];
-      Raw<false> z_raw[kAgUnroll];
-#pragma unroll
-      for (int u = 0; u < kAgUnroll; ++u) {
-        const int row = r + u * kAgLanes;
-        if (row < r1) {
-          load_raw<kDyF32, kVec>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
-          if constexpr (kAct >= 0)
-            load_raw<false, kVec>(z_raw[u], p.Z, static_cast<long long>(row) * p.ldz + col, live);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kAgUnroll; ++u) {
-        const int row = r + u * kAgLanes;
-        if (row >= r1)
-          break;
-        Eight g = values<kDyF32>(dy_raw[u], p.is_bf16);
-        if constexpr (kAct >= 0) {
-          const Eight z = values<false>(z_raw[u], p.is_bf16);
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float2 d = __fmul2_rn(make_float2(g.v[e], g.v[e + 1]), slope_pair<kAct>(make_float2(z.v[e], z.v[e + 1])));
-            g.v[e] = d.x;
-            g.v[e + 1] = d.y;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float2 sum = __fadd2_rn(make_float2(acc[e], acc[e + 1]), make_float2(g.v[e], g.v[e + 1]));
-          acc[e] = sum.x;
-          acc[e + 1] = sum.y;
-        }
-        if (p.dZ) {
-          // rows of dZ are padded to whole 16-byte pieces; columns behind the last are zero
-          uint4 q;
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack_pair(g.v[2 * e], g.v[2 * e + 1], p.is_bf16); // (zeros behind the last column: 0 * slope(0))
-          q = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dZ) + static_cast<long long>(row) * p.lddz + col) = q;
-        }
-      }
-    }
-  }
+  if (live > 0)
+    act_grad_rows<kAct, kDyF32, kVec, kAgLanes>(p, r0 + tr, r1, col, live, acc);
   if (!p.partial)
     return;
 #pragma unroll
@@ -253,27 +272,73 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       total += sums[i][lane];
-    const long long at = static_cast<long long>(blockIdx.y) * p.cols + col;
-    if (p.dbias_type == 0)
-      static_cast<float *>(p.dbias)[at] = total;
-    else
-      static_cast<uint16_t *>(p.dbias)[at] = to_16bit(total, p.dbias_type == 2);
+    store_dbias(p, blockIdx.y, col, total);
+  }
+}
+
+// Short groups: all rows of a group x 32 columns to a block, dz and the finished
+// column sums in one launch, without partial sums in memory.  Four threads to a
+// row, 64 rows side by side.
+constexpr int kShortCols = 32;
+constexpr int kShortLanes = kAgThreads / (kShortCols / 8);
+template <int kAct, bool kDyF32, bool kVec>
+__global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid_constant__ LinearActGrad p) {
+  extern __shared__ int ag_smem[];
+  __shared__ float sums[kAgThreads / 32][kShortCols];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int r0 = 0, r1 = p.rows;
+  if (p.offsets) {
+    GroupTable t{ag_smem, ag_smem + p.groups + 1};
+    build_group_table(t, p.offsets, p.groups, p.rows, 1);
+    r0 = t.begin[blockIdx.y];
+    r1 = t.begin[blockIdx.y + 1];
+  }
+  const int tc = threadIdx.x % (kShortCols / 8), tr = threadIdx.x / (kShortCols / 8);
+  const int col = static_cast<int>(blockIdx.x) * kShortCols + tc * 8;
+  const int live = p.cols - col;
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    acc[e] = 0.0f;
+  if (live > 0)
+    act_grad_rows<kAct, kDyF32, kVec, kShortLanes>(p, r0 + tr, r1, col, live, acc);
+  // the eight rows of a warp, then the warps, in order
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1)
+      acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], d);
+  }
+  if ((threadIdx.x & 31) < kShortCols / 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sums[threadIdx.x / 32][tc * 8 + e] = acc[e];
+  }
+  __syncthreads();
+  const int c = static_cast<int>(blockIdx.x) * kShortCols + static_cast<int>(threadIdx.x);
+  if (p.dbias && threadIdx.x < kShortCols && c < p.cols) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAgThreads / 32; ++i)
+      total += sums[i][threadIdx.x];
+    store_dbias(p, blockIdx.y, c, total);
   }
 }
 
 } // namespace
 
-cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
-                             long long group_dst, int rows, int cols, int groups, int pdl, cudaStream_t stream) {
-  const int pieces = (cols + 7) / 8;
-  const long long blocks = (static_cast<long long>(rows) * pieces + 255) / 256;
-  if (blocks == 0 || groups == 0)
+cudaError_t launch_pack_rows(const PackRows &first, const PackRows &second, int pdl, cudaStream_t stream) {
+  auto blocks_of = [](const PackRows &p) {
+    return p.groups > 0 ? (static_cast<long long>(p.rows) * ((p.cols + 7) / 8) + 255) / 256 : 0;
+  };
+  const long long a = blocks_of(first), b = blocks_of(second), blocks = a > b ? a : b;
+  if (blocks == 0)
     return cudaSuccess;
   // enough blocks to fill the machine; the rest in the kernel's loop
   const unsigned grid = static_cast<unsigned>(blocks < 4096 ? blocks : 4096);
-  return launch(dim3(grid, static_cast<unsigned>(groups)), 256, 0, stream, pdl, pack_rows_kernel,
-                static_cast<const uint16_t *>(src), ld_src, group_src, static_cast<uint16_t *>(dst), ld_dst, group_dst, rows,
-                cols, pieces);
+  return launch(dim3(grid, static_cast<unsigned>(first.groups + second.groups)), 256, 0, stream, pdl, pack_rows_kernel,
+                PackTwo{first, second});
 }
 
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows) {
@@ -281,33 +346,44 @@ int linear_act_grad_chunks(int rows, int groups, int chunk_rows) {
   return groups > 0 ? rows / chunk_rows + (groups < rows ? groups : rows) : whole;
 }
 
+namespace {
+// The instantiation for the call's activation, type of dy and alignment.
+template <typename Go> void pick_act_grad(const LinearActGrad &p, Go go) {
+  auto with = [&](auto f32, auto vec) {
+    constexpr bool kF32 = decltype(f32)::value, kVec = decltype(vec)::value;
+    switch (p.Z ? p.act : kActNone) {
+    case kActRelu: go(act_grad_kernel<kActRelu, kF32, kVec>, act_grad_short_kernel<kActRelu, kF32, kVec>); break;
+    case kActGelu: go(act_grad_kernel<kActGelu, kF32, kVec>, act_grad_short_kernel<kActGelu, kF32, kVec>); break;
+    case kActGeluTanh: go(act_grad_kernel<kActGeluTanh, kF32, kVec>, act_grad_short_kernel<kActGeluTanh, kF32, kVec>); break;
+    case kActSilu: go(act_grad_kernel<kActSilu, kF32, kVec>, act_grad_short_kernel<kActSilu, kF32, kVec>); break;
+    default: go(act_grad_kernel<-1, kF32, kVec>, act_grad_short_kernel<-1, kF32, kVec>); break;
+    }
+  };
+  const bool vec = p.vec_dy && (!p.Z || p.vec_z) && p.cols % 8 == 0;
+  if (p.dy_f32)
+    vec ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
+  else
+    vec ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
+}
+} // namespace
+
 cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
-  const int chunks = linear_act_grad_chunks(p.rows, p.offsets ? p.groups : 0, p.chunk_rows);
   const size_t table = p.offsets ? 2 * sizeof(int) * (static_cast<size_t>(p.groups) + 1) : 0;
+  const unsigned groups = static_cast<unsigned>(p.offsets ? p.groups : 1);
   cudaError_t err = cudaSuccess;
+  if (p.short_groups) {
+    const dim3 grid(static_cast<unsigned>((p.cols + kShortCols - 1) / kShortCols), groups);
+    pick_act_grad(p, [&](auto, auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
+    return err;
+  }
+  const int chunks = linear_act_grad_chunks(p.rows, p.offsets ? p.groups : 0, p.chunk_rows);
   if (chunks > 0) {
     const dim3 grid(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks));
-    auto go = [&](auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); };
-    auto pick = [&](auto f32, auto vec) {
-      constexpr bool kF32 = decltype(f32)::value, kVec = decltype(vec)::value;
-      switch (p.Z ? p.act : kActNone) {
-      case kActRelu: go(act_grad_kernel<kActRelu, kF32, kVec>); break;
-      case kActGelu: go(act_grad_kernel<kActGelu, kF32, kVec>); break;
-      case kActGeluTanh: go(act_grad_kernel<kActGeluTanh, kF32, kVec>); break;
-      case kActSilu: go(act_grad_kernel<kActSilu, kF32, kVec>); break;
-      default: go(act_grad_kernel<-1, kF32, kVec>); break;
-      }
-    };
-    const bool vec = p.vec_dy && (!p.Z || p.vec_z) && p.cols % 8 == 0;
-    if (p.dy_f32)
-      vec ? pick(std::true_type{}, std::true_type{}) : pick(std::true_type{}, std::false_type{});
-    else
-      vec ? pick(std::false_type{}, std::true_type{}) : pick(std::false_type{}, std::false_type{});
+    pick_act_grad(p, [&](auto kernel, auto) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
   }
   if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
     return err;
-  return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(p.offsets ? p.groups : 1)), 256, table,
-                stream, p.pdl, column_sum_kernel, p);
+  return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), groups), 256, table, stream, p.pdl, column_sum_kernel, p);
 }
 
 } // namespace wave

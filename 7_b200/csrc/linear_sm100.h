@@ -94,9 +94,15 @@ cudaError_t linear_pair_read_status(int out[4], bool clear);
 
 // ---- helpers around the products (linear_aux_sm100.cu)
 // 16-bit rows with any stride into rows of `ld_dst` elements: what a TMA load
-// needs (16-byte strides) of an operand that does not have it.
-cudaError_t launch_pack_rows(const void *src, long long ld_src, long long group_src, void *dst, long long ld_dst,
-                             long long group_dst, int rows, int cols, int groups, int pdl, cudaStream_t stream);
+// needs (16-byte strides) of an operand that does not have it.  groups = 0: nothing.
+struct PackRows {
+  const void *src;
+  long long ld_src, group_src;
+  void *dst;
+  long long ld_dst, group_dst;
+  int rows, cols, groups;
+};
+cudaError_t launch_pack_rows(const PackRows &first, const PackRows &second, int pdl, cudaStream_t stream);
 
 // dz = dy * act'(z), rounded to the operands' type, and the column sums of the
 // unrounded dz (dbias) of each group in two steps of fixed order.
@@ -115,6 +121,7 @@ struct LinearActGrad {
   void *dbias; // [groups][cols]
   int dbias_type; // 0 f32, 1 f16, 2 bf16
   int vec_dy, vec_z;
+  int short_groups; // all rows of a group to a block: no `partial`, one launch
   int pdl;
 };
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows); // upper bound, sizes `partial`

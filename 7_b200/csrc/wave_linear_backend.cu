@@ -160,22 +160,24 @@ struct Operand {
   }
 };
 
-// Lays the operand out in `to` if its strides are not multiples of 16 bytes.
-int pack(Operand *o, char **to, cudaStream_t stream) {
+// Describes the layout of an operand in `to` whose strides are not multiples of
+// 16 bytes, and points it there; nothing for one that is fine as it is.
+wave::PackRows pack(Operand *o, char **to) {
+  wave::PackRows p{};
   if (!o->packed())
-    return WAVE_OK;
+    return p;
   const long long ld = o->packed_ld(), group = ld * o->rows;
+  p = wave::PackRows{o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices};
   const size_t bytes = o->packed_bytes();
-  cudaError_t err =
-      wave::launch_pack_rows(o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices,
-                             wave::env_knobs().linear_pdl, stream);
-  if (err != cudaSuccess)
-    return cuda_fail(err, "linear: laying out an operand");
   o->ptr = *to;
   o->ld = ld;
   o->group = group;
   *to += bytes;
-  return WAVE_OK;
+  return p;
+}
+int run_packs(const wave::PackRows &first, const wave::PackRows &second, cudaStream_t stream) {
+  const cudaError_t err = wave::launch_pack_rows(first, second, wave::env_knobs().linear_pdl, stream);
+  return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear: laying out an operand");
 }
 
 int operand_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_cols, int box_rows) {
@@ -515,10 +517,21 @@ int chunk_rows(const Shape &s, int sms) {
   return rows;
 }
 
+// Whether a block takes all rows of a group: one launch instead of two, and with
+// experts no search for the group of a chunk in each of many blocks.  Column sums
+// of gelu's gradient, bf16, all rows / chunks in us: 64 x 512 2.1 / 3.8, 128 x
+// 4096 2.7 / 4.1, 500 x 1024 5.2 / 4.1, 1000 x 1024 7.6 / 5.4; 24 experts, 700 x
+// 520 2.8 / 6.1; 32, 3000 x 1032 8.2 / 11.1; 16, 8192 x 4096 37 / 49.
+bool short_groups(const Shape &s) {
+  const long long rows = (s.d.tokens + s.matrices - 1) / s.matrices;
+  return rows <= (s.grouped ? 1024 : 256);
+}
+
 struct BackwardLayout {
   bool make_dz;   // dz has to be written: an activation, an f32 dy, or rows that TMA cannot load
   long long lddz;
   int chunk;
+  bool short_groups;
   size_t dz_bytes, partial_bytes, x_bytes, w_bytes;
 };
 BackwardLayout backward_layout(const Shape &s, int sms) {
@@ -529,7 +542,8 @@ BackwardLayout backward_layout(const Shape &s, int sms) {
   b.chunk = chunk_rows(s, sms);
   b.dz_bytes = b.make_dz ? static_cast<size_t>(round_up(b.lddz * 2 * d.tokens, 256)) : 0;
   const long long chunks = wave::linear_act_grad_chunks(d.tokens, s.grouped ? s.matrices : 0, b.chunk);
-  b.partial_bytes = static_cast<size_t>(round_up(chunks * d.out_features * 4ll, 256));
+  b.short_groups = short_groups(s);
+  b.partial_bytes = b.short_groups ? 0 : static_cast<size_t>(round_up(chunks * d.out_features * 4ll, 256));
   b.x_bytes = tokens_by_in(s, nullptr).packed_bytes();
   b.w_bytes = weights(s, nullptr).packed_bytes();
   return b;
@@ -610,7 +624,8 @@ int wave_cuda_linear_fwd(const wave_linear_desc *d, const void *X, const void *W
                   x.packed_bytes() + w.packed_bytes());
     char *ws = static_cast<char *>(workspace);
     cudaStream_t q = static_cast<cudaStream_t>(stream);
-    if ((rc = pack(&x, &ws, q)) != WAVE_OK || (rc = pack(&w, &ws, q)) != WAVE_OK)
+    const wave::PackRows px = pack(&x, &ws), pw = pack(&w, &ws);
+    if ((rc = run_packs(px, pw, q)) != WAVE_OK)
       return rc;
     const bool f32 = s.d.y_type == WAVE_F32;
     const Outputs o{Y, s.d.ldy, 0, f32 ? 4 : 2, Z, residual, bias};
@@ -662,7 +677,8 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
       g.ldz = s.d.ldz;
       g.dZ = dz_wanted ? ws : nullptr;
       g.lddz = b.lddz;
-      g.partial = dbias ? reinterpret_cast<float *>(ws + b.dz_bytes) : nullptr;
+      g.partial = dbias && !b.short_groups ? reinterpret_cast<float *>(ws + b.dz_bytes) : nullptr;
+      g.short_groups = b.short_groups;
       g.chunk_rows = b.chunk;
       g.dbias = dbias;
       g.dbias_type = s.d.dbias_type == WAVE_F32 ? 0 : is_bf16 ? 2 : 1;
@@ -678,10 +694,13 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
       dz.ld = b.lddz;
     }
     ws += b.dz_bytes + b.partial_bytes;
-    if (dX && s.d.tokens > 0) {
-      Operand w = weights(s, W);
-      if ((rc = pack(&w, &ws, q)) != WAVE_OK)
+    Operand w = weights(s, W), x = tokens_by_in(s, X);
+    if (s.d.tokens > 0) {
+      const wave::PackRows pw = dX ? pack(&w, &ws) : wave::PackRows{}, px = dW ? pack(&x, &ws) : wave::PackRows{};
+      if ((rc = run_packs(pw, px, q)) != WAVE_OK)
         return rc;
+    }
+    if (dX && s.d.tokens > 0) {
       const Outputs o{dX, s.d.lddx, 0, 2, nullptr, nullptr, nullptr};
       if ((rc = run_product(Product::kInputGrad, s, dz, w, offsets, o, false, d->zero_rest, sms, q)) != WAVE_OK)
         return rc;
@@ -697,9 +716,6 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
                                   static_cast<size_t>(s.d.lddw) * o.elem, 0, row, static_cast<size_t>(s.d.out_features), q);
         return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear: clearing the weight gradient");
       }
-      Operand x = tokens_by_in(s, X);
-      if ((rc = pack(&x, &ws, q)) != WAVE_OK)
-        return rc;
       return run_product(Product::kWeightGrad, s, dz, x, offsets, o, f32, 0, sms, q);
     }
     return WAVE_OK;

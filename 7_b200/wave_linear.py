@@ -234,8 +234,10 @@ def _backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype,
         return _backward(_aligned(dy), _aligned(x), _aligned(weight), offsets, activation, pre_activation, dweight_dtype,
                          dbias_dtype, need_dx, need_dweight, need_dbias)
     torch, _ = _types()
-    dx, dw, db = (torch.empty(shape, dtype=t, device=plan.device) if need else None
-                  for need, (shape, t) in zip((need_dx, need_dweight, need_dbias), plan.outs))
+    (dx_shape, _), (dw_shape, dw_t), (db_shape, db_t) = plan.outs
+    dx = x.new_empty(dx_shape) if need_dx else None
+    dw = (x.new_empty(dw_shape) if dw_t == x.dtype else torch.empty(dw_shape, dtype=dw_t, device=plan.device)) if need_dweight else None
+    db = torch.empty(db_shape, dtype=db_t, device=plan.device) if need_dbias else None
     z = _ptr(pre_activation) if plan.desc.activation else None
     _launch(plan, lambda ws, stream: wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw),
                                                                    _ptr(db), ws, stream))
