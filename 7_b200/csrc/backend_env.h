@@ -20,6 +20,7 @@ struct EnvKnobs {
   int fa_poly = -1;              // WAVE_CUDA_FA_POLY: eighths of the exponentials on the FMA pipe, -1 = each kernel's default
   int fa_stagger = -1;           // WAVE_CUDA_FA_STAGGER: cycles, -1 = the library's default
   int linear_tile = 0;           // WAVE_CUDA_LINEAR_TILE: columns of a linear layer's tile (16, 32, 64, 128, 256), 0 = chosen
+  int linear_columns = 0;        // WAVE_CUDA_LINEAR_COLUMNS: columns of a tile that are used (where the layout allows), 0 = chosen
   int linear_splits = 0;         // WAVE_CUDA_LINEAR_SPLITS: CTAs that share a tile's contraction (1..8), 0 = chosen
   int linear_swap = -1;          // WAVE_CUDA_LINEAR_SWAP: 1 tokens on the tile's columns, 0 on its rows, -1 = chosen
   int linear_pair = -1;          // WAVE_CUDA_LINEAR_PAIR: 1 CTA pairs wherever they can, 0 never, -1 = chosen

@@ -398,39 +398,59 @@ __device__ __forceinline__ void slot_to_global(const uint8_t *slot, void *base, 
       *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(slot + S::at(r0 + i * kRowStep, piece));
     return;
   }
-  const int live = cols - piece * S::kVals; // columns of the piece that exist
+  if (vec) {
+    const int live = cols - piece * S::kVals; // columns of the piece that exist
 #pragma unroll
-  for (int i = 0; i < S::kPieces; ++i, dst += step) {
-    if (r0 + i * kRowStep >= rows || live <= 0)
-      continue;
-    const uint4 v = *reinterpret_cast<const uint4 *>(slot + S::at(r0 + i * kRowStep, piece));
-    if (vec && live >= S::kVals) {
-      *reinterpret_cast<uint4 *>(dst) = v;
-    } else {
-      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < S::kPieces; ++i, dst += step) {
+      if (r0 + i * kRowStep >= rows || live <= 0)
+        continue;
+      const uint4 v = *reinterpret_cast<const uint4 *>(slot + S::at(r0 + i * kRowStep, piece));
+      if (live >= S::kVals) {
+        *reinterpret_cast<uint4 *>(dst) = v;
+      } else {
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < S::kVals; ++e)
-        if (e < live) {
-          if constexpr (kElem == 4)
-            *reinterpret_cast<uint32_t *>(dst + e * 4) = words[e];
-          else
-            *reinterpret_cast<uint16_t *>(dst + e * 2) = static_cast<uint16_t>(words[e >> 1] >> ((e & 1) * 16));
-        }
+        for (int e = 0; e < S::kVals; ++e)
+          if (e < live) {
+            if constexpr (kElem == 4)
+              *reinterpret_cast<uint32_t *>(dst + e * 4) = words[e];
+            else
+              *reinterpret_cast<uint16_t *>(dst + e * 2) = static_cast<uint16_t>(words[e >> 1] >> ((e & 1) * 16));
+          }
+      }
     }
+    return;
+  }
+  // Rows that start anywhere: a row at a time, a value to a lane, so that a store
+  // still covers one piece of memory (a lane's 16 bytes in 2-byte stores scatter
+  // over eight rows each: 4000 x 2500 x 1000 took 72 us).
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    uint8_t *row = static_cast<uint8_t *>(base) + static_cast<long long>(r) * ld * kElem;
+#pragma unroll
+    for (int c = lane; c < W; c += 32)
+      if (c < cols) {
+        const uint8_t *src = slot + S::at(r, c / S::kVals) + c % S::kVals * kElem;
+        if constexpr (kElem == 4)
+          *reinterpret_cast<uint32_t *>(row + c * 4) = *reinterpret_cast<const uint32_t *>(src);
+        else
+          *reinterpret_cast<uint16_t *>(row + c * 2) = *reinterpret_cast<const uint16_t *>(src);
+      }
   }
 }
 
-// A 16-bit block of 32 rows x W columns from memory into registers, in the
-// order of slot_to_global; what lies outside rows x cols is zero.
+// A 16-bit block of 32 rows x W columns whose rows are 16-byte aligned from memory
+// into registers, in the order of slot_to_global; what lies outside rows x cols is
+// zero.
 template <int W>
 __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *base, long long ld, int rows, int cols,
-                                               bool vec, int lane) {
+                                               int lane) {
   using S = Slot<2, W>;
   constexpr int kRowStep = 32 / S::kPieces;
   const int r0 = lane / S::kPieces, piece = lane % S::kPieces;
   const uint16_t *src = static_cast<const uint16_t *>(base) + static_cast<long long>(r0) * ld + piece * 8;
   const long long step = ld * kRowStep;
-  if (vec && rows == 32 && cols == W) {
+  if (rows == 32 && cols == W) {
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i, src += step)
       out[i] = *reinterpret_cast<const uint4 *>(src);
@@ -441,7 +461,7 @@ __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *
   for (int i = 0; i < S::kPieces; ++i, src += step) {
     uint4 v = make_uint4(0, 0, 0, 0);
     if (r0 + i * kRowStep < rows && live > 0) {
-      if (vec && live >= 8) {
+      if (live >= 8) {
         v = *reinterpret_cast<const uint4 *>(src);
       } else {
         uint32_t words[4] = {0, 0, 0, 0};
@@ -453,6 +473,28 @@ __device__ __forceinline__ void global_to_regs(uint4 (&out)[W / 8], const void *
       }
     }
     out[i] = v;
+  }
+}
+// The same into the slot: from those registers, or straight from memory, a row at
+// a time, where the rows start anywhere.
+template <int W>
+__device__ __forceinline__ void residual_to_slot(uint8_t *slot, const uint4 (&regs)[W / 8], const void *base, long long ld,
+                                                 int rows, int cols, bool vec, int lane) {
+  using S = Slot<2, W>;
+  if (vec) {
+    constexpr int kRowStep = 32 / S::kPieces;
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i)
+      *reinterpret_cast<uint4 *>(slot + S::at(lane / S::kPieces + i * kRowStep, lane % S::kPieces)) = regs[i];
+    return;
+  }
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    const uint16_t *row = static_cast<const uint16_t *>(base) + static_cast<long long>(r) * ld;
+#pragma unroll
+    for (int c = lane; c < W; c += 32)
+      if (c < cols)
+        *reinterpret_cast<uint16_t *>(slot + S::at(r, c / 8) + c % 8 * 2) = row[c];
   }
 }
 
@@ -506,9 +548,9 @@ template <int W> struct Ahead {
 template <int W>
 __device__ __forceinline__ void fetch_ahead(Ahead<W> &f, const LinearParams &p, const EpiTile &t, int q0, int lane) {
   const int rows = min(32, t.lane_end - t.lane0), cols = min(W, t.q_end - q0);
-  if (p.R)
+  if (p.R && p.vec_r)
     global_to_regs<W>(f.res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(t.lane0) * p.ldr + q0, p.ldr, rows,
-                      cols, p.vec_r != 0, lane);
+                      cols, lane);
 #pragma unroll
   for (int i = 0; i < (W + 31) / 32; ++i) {
     f.bias[i] = 0.0f;
@@ -600,11 +642,8 @@ __device__ __forceinline__ void epilogue_rows(const LinearParams &p, const EpiTi
   slot_next<kHalves>(e);
   uint8_t *slot = e.slot;
   if (kFull && p.R) {
-    using S = Slot<2, W>;
-    constexpr int kRowStep = 32 / S::kPieces;
-#pragma unroll
-    for (int i = 0; i < S::kPieces; ++i)
-      *reinterpret_cast<uint4 *>(slot + S::at(lane / S::kPieces + i * kRowStep, lane % S::kPieces)) = f.res[i];
+    residual_to_slot<W>(slot, f.res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(t.lane0) * p.ldr + q0, p.ldr,
+                        rows, cols, p.vec_r != 0, lane);
     __syncwarp();
     if (p.is_bf16)
       add_row_from_slot<W, true>(v, slot, lane);
@@ -657,13 +696,11 @@ __device__ __forceinline__ void epilogue_columns(const LinearParams &p, const Ep
     }
     apply_act<W>(v, p.act);
     if (p.R) {
-      using S = Slot<2, 32>;
+      const uint16_t *base = static_cast<const uint16_t *>(p.R) + static_cast<long long>(q0) * p.ldr + t.lane0;
       uint4 res[4];
-      global_to_regs<32>(res, static_cast<const uint16_t *>(p.R) + static_cast<long long>(q0) * p.ldr + t.lane0, p.ldr,
-                         tokens, features, p.vec_r != 0, lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint4 *>(slot + S::at(lane / 4 + i * 8, lane % 4)) = res[i];
+      if (p.vec_r)
+        global_to_regs<32>(res, base, p.ldr, tokens, features, lane);
+      residual_to_slot<32>(slot, res, base, p.ldr, tokens, features, p.vec_r != 0, lane);
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < W; ++j)

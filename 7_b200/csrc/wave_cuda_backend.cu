@@ -104,6 +104,10 @@ EnvKnobs read_env() {
     const int n = atoi(v);
     e.linear_tile = (n == 16 || n == 32 || n == 64 || n == 128 || n == 256) ? n : 0;
   }
+  if (const char *v = getenv("WAVE_CUDA_LINEAR_COLUMNS")) {
+    const int n = atoi(v);
+    e.linear_columns = (n >= 16 && n <= 256) ? n : 0;
+  }
   if (const char *v = getenv("WAVE_CUDA_LINEAR_SPLITS")) {
     const int n = atoi(v);
     e.linear_splits = (n >= 1 && n <= 8) ? n : 0;

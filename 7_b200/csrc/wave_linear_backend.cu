@@ -281,7 +281,8 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
   const long long k_iters = (e.k + 63) / 64;
   const double mine = static_cast<double>((k_iters + c->splits - 1) / c->splits);
   const double bytes = (tile_p + c->tile_q) * 128.0;
-  double stage = t.stage * c->tile_q / tile_n;
+  // (a narrower tile saves less time than columns: its other operand is as wide)
+  double stage = t.stage * (1.0 - (pair ? 0.35 : 0.5) * (1.0 - static_cast<double>(c->tile_q) / tile_n));
   if (stage < 0.18) // the issue of a stage
     stage = 0.18;
   if (stage < bytes * side / kL2BytesPerUs)
@@ -341,23 +342,34 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
       const int knob = env.linear_tile;
       if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
         continue;
-      // columns of no use are left out where the layout allows: tiles of equal width
+      // Columns of no use are left out where the layout allows: tiles of equal
+      // width, as few as there can be or up to three more, which can fill a last
+      // round of tiles.
       const int unit = l.b_mn ? (pair ? 128 : 64) : (pair ? 32 : 16);
-      int tile_q = tile_n;
-      if (!(swap && s.grouped)) {
-        const long long n = (e.q + tile_n - 1) / tile_n;
-        tile_q = static_cast<int>(round_up((e.q + (n > 0 ? n : 1) - 1) / (n > 0 ? n : 1), unit));
-        tile_q = tile_q > tile_n ? tile_n : tile_q < unit ? unit : tile_q;
+      const long long least = (e.q + tile_n - 1) / tile_n;
+      int before = 0;
+      for (int more = 0; more < (l.b_mn || swap ? 1 : 4); ++more) {
+        const long long n = least + more > 0 ? least + more : 1;
+        int tile_q = tile_n;
+        if (!(swap && s.grouped)) {
+          tile_q = static_cast<int>(round_up((e.q + n - 1) / n, unit));
+          tile_q = tile_q > tile_n ? tile_n : tile_q < unit ? unit : tile_q;
+        }
+        if (env.linear_columns && !(swap && s.grouped))
+          tile_q = env.linear_columns / unit * unit < unit ? unit : env.linear_columns > tile_n ? tile_n : env.linear_columns / unit * unit;
+        if (tile_q == before || (more > 0 && tile_q <= tile_n / 2))
+          break;
+        before = tile_q;
+        if (swap && !knob && t.tile > 16 && tile_q <= t.tile / 2)
+          continue; // the next smaller tile does it
+        if (env.linear_splits > 0) {
+          consider(t, swap, pair ? 1 : env.linear_splits, tile_q);
+          continue;
+        }
+        for (int c : {1, 2, 3, 4, 6, 8})
+          if (c == 1 || (!pair && t.tile < 256 && (e.k + 63) / 64 >= 2 * c && (swap || tile_q / 16 >= c)))
+            consider(t, swap, c, tile_q);
       }
-      if (swap && !knob && t.tile > 16 && tile_q <= t.tile / 2)
-        continue; // the next smaller tile does it
-      if (env.linear_splits > 0) {
-        consider(t, swap, pair ? 1 : env.linear_splits, tile_q);
-        continue;
-      }
-      for (int c : {1, 2, 3, 4, 6, 8})
-        if (c == 1 || (!pair && t.tile < 256 && (e.k + 63) / 64 >= 2 * c && (swap || tile_q / 16 >= c)))
-          consider(t, swap, c, tile_q);
     }
   }
   if (best.us < 0.0) { // knobs that exclude one another

@@ -318,8 +318,8 @@ int wave_cuda_flash_attention_fwd_host(const wave_fa_desc *desc, const void *Q_h
  * lays them out in the workspace.  Every other buffer needs its elements'
  * alignment only.  A workspace is used by one call at a time, nothing in it
  * needs clearing, and nothing is kept in it between calls.
- * WAVE_CUDA_LINEAR_TILE=<columns>, WAVE_CUDA_LINEAR_SPLITS=<CTAs to a tile> and
- * WAVE_CUDA_LINEAR_SWAP=0|1 and
+ * WAVE_CUDA_LINEAR_TILE=<columns>, WAVE_CUDA_LINEAR_COLUMNS=<used of them>,
+ * WAVE_CUDA_LINEAR_SPLITS=<CTAs to a tile>, WAVE_CUDA_LINEAR_SWAP=0|1 and
  * WAVE_CUDA_LINEAR_PAIR=0|1 override the choice of tiles, WAVE_CUDA_LINEAR_PDL=0
  * launches without programmatic dependent launch (measurement knobs; with other
  * tiles sums are taken in another order).                                    */
