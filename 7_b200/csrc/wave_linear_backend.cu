@@ -204,22 +204,22 @@ int chunk_map(CUtensorMap *map, const Operand &o, int is_bf16, int box_chunks, i
 
 // ------------------------------------------------------------ tile choice
 // What a launch takes is predicted for every tile and split it could have, and
-// the cheapest is taken.  Times in us, fitted to 140 problems (1 to 8192 tokens,
-// 256 to 16384 features, the three products, inputs in turn out of L2 and DRAM),
-// each timed in every variant: the choice is 0.5 % slower than the best variant
-// on average and 9 % at worst.
-//   base    launch, first loads, the last tile's epilogue
-//   stage   64 of the contraction of one tile with nothing else in the way
-//   epi     a tile's epilogue, which hides behind the next tile's stages
+// the cheapest is taken.  Times in us, fitted to 117 problems (1 to 9000 tokens,
+// 256 to 12000 features, the three products, up to 64 experts, inputs in turn out
+// of L2 and DRAM), each timed in up to 21 variants: the choice is 0.9 % slower than
+// the best variant on average and 14 % at worst.
+//   base    launch, first loads, teardown
+//   stage   64 of the contraction of one whole tile with nothing else in the way
+//   epi     a whole tile's epilogue, which hides behind the next tile's stages
 struct TileCost {
   int tile; // columns; 512: CTA pair, 256 x 256
   double base, stage, epi;
 };
-constexpr TileCost kTileCosts[] = {{16, 3.28, 0.23, 0.35},  {32, 4.02, 0.21, 1.1},   {64, 5.36, 0.19, 0.97},
-                                   {128, 5.79, 0.30, 1.33}, {256, 7.23, 0.52, 1.84}, {512, 8.58, 0.29, 3.4}};
+constexpr TileCost kTileCosts[] = {{16, 2.86, 0.24, 0.36}, {32, 3.08, 0.26, 0.65},  {64, 4.59, 0.19, 0.94},
+                                   {128, 4.50, 0.33, 1.16}, {256, 5.34, 0.47, 1.45}, {512, 5.54, 0.325, 2.19}};
 constexpr int kPairTile = 512;
-constexpr double kL2BytesPerUs = 12.6e6; // all SMs together
-constexpr double kSplitCost = 1.9;       // the cluster's barriers and the sum over its CTAs, + 0.06 for each
+constexpr double kL2BytesPerUs = 12.4e6; // all SMs together
+constexpr double kSplitCost = 2.3;       // the cluster's barriers and the sum over its CTAs, + 0.03 for each
 // CTAs that run side by side in clusters of a size (an SM each): clusters do not
 // straddle the GPCs, whose SMs are no multiple of every size (measured with
 // cudaOccupancyMaxActiveClusters; 148 SMs).
@@ -276,23 +276,24 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
   }
   const double fit = (pair ? sms / 2 : sms * (kClusterFit[c->splits] / 148.0));
   const double ctas = about * c->splits, side = ctas < fit ? ctas : fit;
-  // (experts' tiles are dealt over the CTAs unevenly enough that half a round is not a whole one)
-  const double rounds = e.grouped && ctas > fit ? ctas / fit + 0.5 : static_cast<double>(static_cast<long long>((ctas + fit - 1e-6) / fit));
+  // (how many tiles the experts' rows make is not known here: two thirds of a last round)
+  const double rounds = e.grouped && ctas > fit ? ctas / fit + 0.65 : static_cast<double>(static_cast<long long>((ctas + fit - 1e-6) / fit));
   const long long k_iters = (e.k + 63) / 64;
   const double mine = static_cast<double>((k_iters + c->splits - 1) / c->splits);
   const double bytes = (tile_p + c->tile_q) * 128.0;
   // (a narrower tile saves less time than columns: its other operand is as wide)
-  double stage = t.stage * (1.0 - (pair ? 0.35 : 0.5) * (1.0 - static_cast<double>(c->tile_q) / tile_n));
-  if (stage < 0.18) // the issue of a stage
-    stage = 0.18;
+  double stage = t.stage * (1.0 - (pair ? 0.38 : 0.54) * (1.0 - static_cast<double>(c->tile_q) / tile_n));
+  if (stage < 0.17) // the issue of a stage
+    stage = 0.17;
   if (stage < bytes * side / kL2BytesPerUs)
     stage = bytes * side / kL2BytesPerUs;
   const double epi = t.epi * c->tile_q / tile_n;
   const double each = mine * stage;
+  const double base = t.base + epi;
   if (c->splits == 1)
-    c->us = t.base + rounds * (each > epi ? each : epi);
+    c->us = base + rounds * (each > epi ? each : epi);
   else
-    c->us = t.base + kSplitCost + 0.06 * c->splits + rounds * each + (rounds - 1.0) * (t.base - 1.0);
+    c->us = base + kSplitCost + 0.03 * c->splits + rounds * each + (rounds - 1.0) * (base - 1.0);
 }
 
 Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
