@@ -28,6 +28,7 @@ struct EnvKnobs {
 };
 
 EnvKnobs env_knobs();
+unsigned env_generation(); // changes when the knobs are read again
 void reload_env_knobs();
 
 } // namespace wave

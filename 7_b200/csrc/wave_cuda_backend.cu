@@ -17,6 +17,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <atomic>
 #include <mutex>
 #include <initializer_list>
 #include <string>
@@ -71,6 +72,7 @@ namespace {
 std::mutex g_env_mu;
 EnvKnobs g_env;
 bool g_env_loaded = false;
+std::atomic<unsigned> g_env_generation{0};
 
 EnvKnobs read_env() {
   EnvKnobs e;
@@ -135,7 +137,9 @@ void reload_env_knobs() {
   std::lock_guard<std::mutex> lock(g_env_mu);
   g_env = read_env();
   g_env_loaded = true;
+  ++g_env_generation;
 }
+unsigned env_generation() { return g_env_generation.load(); }
 
 // Lets the library's other translation units record a failure message.
 void set_last_error(const char *message) { g_last_error = message ? message : ""; }

@@ -296,7 +296,7 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
     c->us = base + kSplitCost + 0.03 * c->splits + rounds * each + (rounds - 1.0) * (base - 1.0);
 }
 
-Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
+Plan make_plan(Product kind, const Shape &s, bool out_f32, int sms) {
   const wave::EnvKnobs env = wave::env_knobs();
   const wave_linear_desc &d = s.d;
   Plan pl{};
@@ -407,6 +407,37 @@ Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
       pl.stages = need < 3 ? 3 : static_cast<int>(need);
   }
   return pl;
+}
+
+// make_plan, with the thread's last choices at hand: a layer is called with the
+// same descriptor again and again, and the predictions cost a microsecond.
+Plan plan_product(Product kind, const Shape &s, bool out_f32, int sms) {
+  struct Entry {
+    wave_linear_desc d;
+    Product kind;
+    int sms;
+    unsigned generation;
+    bool out_f32, valid;
+    Plan plan;
+  };
+  constexpr int kEntries = 16;
+  static thread_local Entry entries[kEntries];
+  static thread_local int next = 0;
+  const unsigned generation = wave::env_generation();
+  for (const Entry &e : entries)
+    if (e.valid && e.kind == kind && e.out_f32 == out_f32 && e.sms == sms && e.generation == generation &&
+        memcmp(&e.d, &s.d, sizeof s.d) == 0)
+      return e.plan;
+  Entry &e = entries[next];
+  next = (next + 1) % kEntries;
+  e.d = s.d;
+  e.kind = kind;
+  e.out_f32 = out_f32;
+  e.sms = sms;
+  e.generation = generation;
+  e.plan = make_plan(kind, s, out_f32, sms);
+  e.valid = true;
+  return e.plan;
 }
 
 struct Outputs {

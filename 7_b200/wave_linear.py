@@ -16,17 +16,13 @@ implementation.
 from __future__ import annotations
 
 import ctypes as C
-import functools
+
+import torch
 
 from . import wave_cuda as wc
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-
-
-@functools.lru_cache(maxsize=None)
-def _types():
-    import torch
-    return torch, {torch.bfloat16: wc.BF16, torch.float16: wc.F16, torch.float32: wc.F32}
+_TYPES = {torch.bfloat16: wc.BF16, torch.float16: wc.F16, torch.float32: wc.F32}
 
 
 class _Plan:
@@ -40,7 +36,7 @@ class _Plan:
         self.desc = wc.LinearDesc(*fields)
         self.ref = C.byref(self.desc)
         self.device, self.index, self.outs = device, device.index, outs
-        with _types()[0].cuda.device(device):  # the workspace goes by the device's SMs
+        with torch.cuda.device(device):  # the workspace goes by the device's SMs
             try:
                 wc.linear_validate(self.desc)
                 self.need = wc.linear_workspace_bytes(self.desc, backward)
@@ -92,7 +88,6 @@ def _row_stride(t, name: str, rows: int, cols: int, dim: int) -> int:
 
 def _layer(x, weight, offsets):
     """Checks x, weight (and offsets); returns sizes and strides."""
-    torch, types = _types()
     if not x.is_cuda:
         raise ValueError("the tensors must be CUDA tensors: this backend has no CPU path")
     device = x.device
@@ -122,7 +117,7 @@ def _layer(x, weight, offsets):
             stride_w = weight.stride(0)
             if stride_w < (ldw or k) * (n - 1) + k:
                 raise ValueError("the experts' weights must not overlap")
-    return torch, types, device, tokens, n, k, experts, ldx, ldw, stride_w
+    return device, tokens, n, k, experts, ldx, ldw, stride_w
 
 
 def _act(activation: str) -> int:
@@ -136,23 +131,21 @@ def _aligned(t):
     """TMA loads start on 16-byte boundaries: a view that does not is copied."""
     if t.data_ptr() % 16 == 0:
         return t
-    torch, _ = _types()
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-def _launch(plan, call):
-    """Runs `call(workspace, stream)` with the tensors' device current (the
-    library launches on the current device) on its current stream."""
-    torch, _ = _types()
-    if torch.cuda.current_device() != plan.index:
-        with torch.cuda.device(plan.device):
-            return _launch(plan, call)
-    ws = torch.empty(plan.need, dtype=torch.uint8, device=plan.device) if plan.need else None
-    wc.check(call(_ptr(ws), torch._C._cuda_getCurrentRawStream(plan.index)))
+def _on_its_device(call, plan, *args):
+    """`call` with the tensors' device current: the library launches on the current device."""
+    with torch.cuda.device(plan.device):
+        return call(*args)
+
+
+def _workspace(plan):
+    return torch.empty(plan.need, dtype=torch.uint8, device=plan.device) if plan.need else None
 
 
 def _plan_forward(x, weight, offsets, bias, residual, activation, out, out_dtype):
-    torch, types, device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
+    device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
     io = x.dtype
     bias_type = io
     if bias is not None:
@@ -175,7 +168,7 @@ def _plan_forward(x, weight, offsets, bias, residual, activation, out, out_dtype
         if out_dtype is not None and out_dtype != y_type:
             raise ValueError(f"out has dtype {y_type}, out_dtype says {out_dtype}")
         ldy = _matrix(out, "out", tokens, n, (io, torch.float32), device)
-    fields = (tokens, n, k, experts, types[io], types[y_type], types[bias_type], types[io], wc.F32, _act(activation), zero_rest, 0,
+    fields = (tokens, n, k, experts, _TYPES[io], _TYPES[y_type], _TYPES[bias_type], _TYPES[io], wc.F32, _act(activation), zero_rest, 0,
               ldx, ldw, ldy, ldr, 0, 0, 0, stride_w, 0)
     return _Plan(device, False, fields, ((tokens, n), y_type))
 
@@ -186,24 +179,26 @@ def _forward(x, weight, offsets, bias, residual, activation, out, out_dtype, sav
     plan = _plans.get(key)
     if plan is None:
         plan = _remember(key, _plan_forward(x, weight, offsets, bias, residual, activation, out, out_dtype))
+    if torch.cuda.current_device() != plan.index:
+        return _on_its_device(_forward, plan, x, weight, offsets, bias, residual, activation, out, out_dtype, save)
     px, pw = x.data_ptr(), weight.data_ptr()
     if (px | pw) & 15:
         return _forward(_aligned(x), _aligned(weight), offsets, bias, residual, activation, out, out_dtype, save)
-    torch, _ = _types()
     shape, y_type = plan.outs
     y = out
     if y is None:
-        y = x.new_empty(shape) if y_type == x.dtype else torch.empty(shape, dtype=y_type, device=plan.device)
+        y = x.new_empty(shape) if y_type is x.dtype else torch.empty(shape, dtype=y_type, device=plan.device)
     z = None
     if save:  # rows that belong to no expert are left alone with `out`
         z = x.new_zeros(shape) if offsets is not None and out is not None else x.new_empty(shape)
-    _launch(plan, lambda ws, stream: wc.lib().wave_cuda_linear_fwd(
-        plan.ref, px, pw, _ptr(bias), _ptr(residual), _ptr(offsets), y.data_ptr(), _ptr(z), ws, stream))
+    ws = _workspace(plan)
+    wc.check(wc.lib().wave_cuda_linear_fwd(plan.ref, px, pw, _ptr(bias), _ptr(residual), _ptr(offsets), y.data_ptr(), _ptr(z),
+                                           _ptr(ws), torch._C._cuda_getCurrentRawStream(plan.index)))
     return (y, z) if save else y
 
 
 def _plan_backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype):
-    torch, types, device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
+    device, tokens, n, k, experts, ldx, ldw, stride_w = _layer(x, weight, offsets)
     io = x.dtype
     act = _act(activation)
     ldy = _matrix(dy, "dy", tokens, n, (io, torch.float32), device)
@@ -218,7 +213,7 @@ def _plan_backward(dy, x, weight, offsets, activation, pre_activation, dweight_d
         if t not in (io, torch.float32):
             raise ValueError(f"{name} must be {io} or f32; got {t}")
     lead = (experts,) if offsets is not None else ()
-    fields = (tokens, n, k, experts, types[io], types[dy.dtype], types[io], types[dweight_dtype], types[dbias_dtype], act,
+    fields = (tokens, n, k, experts, _TYPES[io], _TYPES[dy.dtype], _TYPES[io], _TYPES[dweight_dtype], _TYPES[dbias_dtype], act,
               int(offsets is not None), 0, ldx, ldw, ldy, 0, ldz, 0, 0, stride_w, 0)
     return _Plan(device, True, fields, (((tokens, k), io), ((*lead, n, k), dweight_dtype), ((*lead, n), dbias_dtype)))
 
@@ -229,18 +224,23 @@ def _backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype,
     plan = _plans.get(key)
     if plan is None:
         plan = _remember(key, _plan_backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype))
+    if torch.cuda.current_device() != plan.index:
+        return _on_its_device(_backward, plan, dy, x, weight, offsets, activation, pre_activation, dweight_dtype, dbias_dtype,
+                              need_dx, need_dweight, need_dbias)
     pdy, px, pw = dy.data_ptr(), x.data_ptr(), weight.data_ptr()
     if (pdy | px | pw) & 15:
         return _backward(_aligned(dy), _aligned(x), _aligned(weight), offsets, activation, pre_activation, dweight_dtype,
                          dbias_dtype, need_dx, need_dweight, need_dbias)
-    torch, _ = _types()
-    (dx_shape, _), (dw_shape, dw_t), (db_shape, db_t) = plan.outs
+    (dx_shape, io), (dw_shape, dw_type), (db_shape, db_type) = plan.outs
     dx = x.new_empty(dx_shape) if need_dx else None
-    dw = (x.new_empty(dw_shape) if dw_t == x.dtype else torch.empty(dw_shape, dtype=dw_t, device=plan.device)) if need_dweight else None
-    db = torch.empty(db_shape, dtype=db_t, device=plan.device) if need_dbias else None
+    dw = None
+    if need_dweight:
+        dw = x.new_empty(dw_shape) if dw_type is io else torch.empty(dw_shape, dtype=dw_type, device=plan.device)
+    db = torch.empty(db_shape, dtype=db_type, device=plan.device) if need_dbias else None
+    ws = _workspace(plan)
     z = _ptr(pre_activation) if plan.desc.activation else None
-    _launch(plan, lambda ws, stream: wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw),
-                                                                   _ptr(db), ws, stream))
+    wc.check(wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+                                           torch._C._cuda_getCurrentRawStream(plan.index)))
     return dx, dw, db
 
 
