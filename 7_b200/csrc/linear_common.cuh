@@ -300,18 +300,22 @@ template <int kAct> __device__ __forceinline__ float2 slope_pair(float2 z) {
     const float2 zc = make_float2(z.x < 0.0f ? -a.x : (z.x >= 0.0f ? a.x : z.x), z.y < 0.0f ? -a.y : (z.y >= 0.0f ? a.y : z.y));
     return __ffma2_rn(__fmul2_rn(zc, both(0.3989422804014327f)), gauss, phi);
   } else if constexpr (kAct == kActGeluTanh || kAct == kActSilu) {
-    // z s with s = sigmoid(r z), r = 1 or 2c (1 + a z^2): s + z s (1 - s) (r z)' = s (1 + (1 - s) z (r z)')
+    // z s with s = sigmoid(r z), r = 1 or 2c (1 + a z^2): s + z s (1 - s) (r z)' = s (1 + (1 - s) z (r z)').
+    // Beyond +-64 (+-16) that is 1 or 0 in f32; cut there, lest (1 - s) z becomes 0 * infinity.
+    constexpr float kCutAt = kAct == kActSilu ? 64.0f : 16.0f;
+    const float2 c = make_float2(fminf(fmaxf(z.x, -kCutAt), kCutAt), fminf(fmaxf(z.y, -kCutAt), kCutAt));
     float2 s, w;
     if constexpr (kAct == kActSilu) {
-      s = sigmoid_of_minus(__fmul2_rn(z, both(-kLog2e)));
-      w = z;
+      s = sigmoid_of_minus(__fmul2_rn(c, both(-kLog2e)));
+      w = c;
     } else {
-      const float2 z2 = __fmul2_rn(z, z);
-      s = sigmoid_of_minus(__fmul2_rn(z, __ffma2_rn(z2, both(-2.0f * kLog2e * kGeluC * kGeluA), both(-2.0f * kLog2e * kGeluC))));
-      w = __fmul2_rn(z, __ffma2_rn(z2, both(6.0f * kGeluC * kGeluA), both(2.0f * kGeluC)));
+      const float2 z2 = __fmul2_rn(c, c);
+      s = sigmoid_of_minus(__fmul2_rn(c, __ffma2_rn(z2, both(-2.0f * kLog2e * kGeluC * kGeluA), both(-2.0f * kLog2e * kGeluC))));
+      w = __fmul2_rn(c, __ffma2_rn(z2, both(6.0f * kGeluC * kGeluA), both(2.0f * kGeluC)));
     }
     const float2 rest = __ffma2_rn(s, both(-1.0f), both(1.0f));
-    return __fmul2_rn(s, __ffma2_rn(rest, w, both(1.0f)));
+    const float2 y = __fmul2_rn(s, __ffma2_rn(rest, w, both(1.0f)));
+    return make_float2(z.x == z.x ? y.x : z.x, z.y == z.y ? y.y : z.y); // a NaN stays one
   } else {
     return both(1.0f);
   }

@@ -100,6 +100,9 @@ int validate(const wave_linear_desc *d) {
     return fail(WAVE_E_INVALID, "descriptor is null");
   if (d->tokens < 0)
     return fail(WAVE_E_INVALID, "tokens must be >= 0; got %d", d->tokens);
+  if (d->tokens > 1 << 30 || d->out_features > 1 << 30 || d->in_features > 1 << 30)
+    return fail(WAVE_E_INVALID, "tokens and features must be at most 2^30; got %d, %d and %d", d->tokens, d->out_features,
+                d->in_features);
   if (d->out_features < 1 || d->in_features < 1)
     return fail(WAVE_E_INVALID, "out_features and in_features must be >= 1; got %d and %d", d->out_features,
                 d->in_features);

@@ -401,6 +401,28 @@ def test_special_values(cuda, wc, wl):
         assert bool(big.isinf().all())
 
 
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_far_pre_activations(cuda, wc, wl, act):
+    """Pre-activations of any size in bf16: values and slopes are the limits, a NaN stays one."""
+    torch = cuda
+    far = torch.tensor([3e38, 1e20, 1e6, 300.0, -300.0, -1e6, -1e20, -3e38], device="cuda").to(torch.bfloat16)[None]
+    eye = torch.eye(8, device="cuda", dtype=torch.bfloat16)
+    # (one value to a token: 0 * 3e38 in the other products is 0)
+    z = torch.diag(far[0])
+    y = wl.linear(z, eye, activation=act)
+    assert torch.equal(torch.diag(y), torch.where(far[0] > 0, far[0], torch.zeros_like(far[0])))
+    dy = torch.ones_like(z)
+    dx = wl.linear_backward(dy, z, eye, activation=act, pre_activation=far.expand(8, 8).contiguous(), need_dweight=False,
+                            need_dbias=False)[0]
+    want = (far > 0).to(torch.bfloat16).expand(8, 8)
+    assert bool(((dx - want).abs() <= 1e-20).all())
+    nan = torch.full_like(z, float("nan"))
+    assert bool(wl.linear_backward(dy, z, eye, activation=act, pre_activation=nan, need_dweight=False)[2].isnan().all())
+    inf = torch.full_like(z, float("inf"))
+    assert bool((wl.linear_backward(dy, z, eye, activation=act, pre_activation=inf, need_dweight=False)[2] == 8).all())
+    assert bool((wl.linear_backward(dy, z, eye, activation=act, pre_activation=-inf, need_dweight=False)[2].abs() <= 1e-20).all())
+
+
 def test_no_tokens(cuda, wc, wl):
     torch = cuda
     w, wg = (torch.ones(*s, 16, 24, dtype=torch.bfloat16, device="cuda") for s in ((), (3,)))

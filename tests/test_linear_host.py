@@ -48,7 +48,9 @@ def test_desc_init(wc):
     (dict(lddw=2), "E_INVALID", "lddw must be 0 or between 64"),
     (dict(experts=2, expert_stride_w=32 * 64 - 1), "E_INVALID", "expert_stride_w must be 0 or hold a whole matrix"),
     (dict(experts=2, lddw=72, expert_stride_dw=32 * 64), "E_INVALID", "expert_stride_dw must be 0 or hold a whole matrix"),
-    (dict(tokens=2**31 - 1, out_features=2**20), "E_INVALID", "too many output tiles"),
+    (dict(tokens=2**30, out_features=2**20), "E_INVALID", "too many output tiles"),
+    (dict(tokens=2**30 + 1), "E_INVALID", "tokens and features must be at most 2^30"),
+    (dict(in_features=2**31 - 1), "E_INVALID", "tokens and features must be at most 2^30"),
 ])
 def test_descriptor_refusals(wc, fields, code, message):
     with pytest.raises(wc.WaveCudaError) as err:
