@@ -9,6 +9,25 @@
 namespace wave {
 namespace linear_detail {
 
+// The order of launches on the stream.  A kernel waits until the one before it is
+// complete, and lets the one after it start as soon as SMs are free.  With
+// `beside` it needs nothing that the launch before it writes (that one is of the
+// same call and started after everything both of them need was complete): it
+// waits only at its end, so that whoever waits for it has waited for both.  So
+// the weight gradient's CTAs take the SMs that the input gradient's last round
+// leaves idle, and small products run side by side (with it / one after the other,
+// in us: 8192 x 8192 x 2048 462 / 482, 515 x 1032 x 776 18.6 / 20.1, 24 experts,
+// 700 x 520 x 1288 34.5 / 37.5).
+__device__ __forceinline__ void start_after_previous(int beside) {
+  if (!beside)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void end_after_previous(int beside) {
+  if (beside)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ------------------------------------------------------------- row ranges
 // The experts' row ranges in shared memory: begin[g] .. begin[g + 1] are group
 // g's rows, blocks[g] the number of row blocks of the groups before it.  What

@@ -130,8 +130,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   cluster_wait();
   tc_fence_after_sync();
   const uint32_t tmem_base = sh->tmem_base;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  start_after_previous(p.beside);
   if (p.ragged != kRaggedNone)
     build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : p.P, kPairP);
 
@@ -435,6 +434,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     }
   }
 
+  end_after_previous(p.beside);
   // Neither CTA may leave, or free tensor memory, while its partner can still
   // read its shared memory, signal its barriers or write its accumulator.
   tc_fence_before_sync();

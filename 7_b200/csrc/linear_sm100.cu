@@ -178,8 +178,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const uint32_t tmem_base = sh->tmem_base;
   // Up to here only this CTA's own state was touched: it may run while the kernel
   // before this one on the stream is finishing.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  start_after_previous(p.beside);
   if (p.ragged != kRaggedNone)
     build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : (kSwap ? p.Q : p.P),
                       kSwap ? p.tile_q : kTileP);
@@ -615,6 +614,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     cluster_wait();
   }
 
+  end_after_previous(p.beside);
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {

@@ -66,6 +66,7 @@ struct LinearParams {
   int vec_d, vec_z, vec_r; // 16-byte accesses are aligned in D / Z / R
   int tma_d, tma_z;  // whole blocks of D / Z leave by TMA stores (tokens as rows, the maps are there)
   int zero_rest;     // rows of D and Z that belong to no group are set to zero
+  int beside;        // runs beside the launch before it (see start_after_previous)
 };
 
 struct LinearLaunch {

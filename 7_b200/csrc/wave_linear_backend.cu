@@ -452,7 +452,7 @@ struct Outputs {
 };
 
 int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operand &b_op, const int *offsets, const Outputs &o,
-                bool out_f32, int zero_rest, int sms, cudaStream_t stream) {
+                bool out_f32, int zero_rest, bool beside, int sms, cudaStream_t stream) {
   const wave_linear_desc &d = s.d;
   const Plan pl = plan_product(kind, s, out_f32, sms);
   const LinearLaunch &l = pl.launch;
@@ -506,6 +506,7 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
   p.vec_z = aligned16(o.Z) && d.ldz % 8 == 0;
   p.vec_r = aligned16(o.R) && d.ldr % 8 == 0;
   p.zero_rest = zero_rest;
+  p.beside = beside && l.pdl;
   wave::LinearMaps m;
   const int b_cols = l.pair ? pl.tile_q / 2 : pl.tile_q; // of one CTA
   p.chunks_a = l.a_mn && chunked(a);
@@ -676,7 +677,7 @@ int wave_cuda_linear_fwd(const wave_linear_desc *d, const void *X, const void *W
       return rc;
     const bool f32 = s.d.y_type == WAVE_F32;
     const Outputs o{Y, s.d.ldy, 0, f32 ? 4 : 2, Z, residual, bias};
-    return run_product(Product::kForward, s, x, w, offsets, o, f32, d->zero_rest, sms, q);
+    return run_product(Product::kForward, s, x, w, offsets, o, f32, d->zero_rest, false, sms, q);
   });
 }
 
@@ -742,15 +743,20 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
     }
     ws += b.dz_bytes + b.partial_bytes;
     Operand w = weights(s, W), x = tokens_by_in(s, X);
+    // The products need nothing of the column sums, nor the second product of the first.
+    bool beside = dbias && !(dz_wanted && b.short_groups);
     if (s.d.tokens > 0) {
       const wave::PackRows pw = dX ? pack(&w, &ws) : wave::PackRows{}, px = dW ? pack(&x, &ws) : wave::PackRows{};
       if ((rc = run_packs(pw, px, q)) != WAVE_OK)
         return rc;
+      if (pw.groups + px.groups > 0)
+        beside = false;
     }
     if (dX && s.d.tokens > 0) {
       const Outputs o{dX, s.d.lddx, 0, 2, nullptr, nullptr, nullptr};
-      if ((rc = run_product(Product::kInputGrad, s, dz, w, offsets, o, false, d->zero_rest, sms, q)) != WAVE_OK)
+      if ((rc = run_product(Product::kInputGrad, s, dz, w, offsets, o, false, d->zero_rest, beside, sms, q)) != WAVE_OK)
         return rc;
+      beside = true;
     }
     if (dW) {
       const bool f32 = s.d.dweight_type == WAVE_F32;
@@ -763,7 +769,7 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
                                   static_cast<size_t>(s.d.lddw) * o.elem, 0, row, static_cast<size_t>(s.d.out_features), q);
         return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear: clearing the weight gradient");
       }
-      return run_product(Product::kWeightGrad, s, dz, x, offsets, o, f32, 0, sms, q);
+      return run_product(Product::kWeightGrad, s, dz, x, offsets, o, f32, 0, beside, sms, q);
     }
     return WAVE_OK;
   });
