@@ -90,6 +90,7 @@ struct Tile {
   int group = 0;
   int p0 = 0, p_end = 0; // first row on the P side, end of the live rows
   int q0 = 0, q_end = 0; // first column on the Q side, end of the live columns
+  int n = 0;             // columns of the tile (kEven only)
   int k_begin = 0, k_len = 0; // contraction: first index (rows of the group when ragged) and length
 };
 
@@ -122,11 +123,14 @@ __device__ __forceinline__ void raster_coords(int id, int num_r, const LinearPar
   r = first + in - c * rows;
 }
 
-template <bool kSwap> struct TileWalk {
+// kEven: an expert's tokens are shared out evenly over as few blocks as tile_q
+// allows, in steps of 32 columns.
+template <bool kSwap, bool kEven = false> struct TileWalk {
   const LinearParams &p;
   const GroupTable t;
   int g;
   int tile_p;
+  int even_of = -1, even = 0; // the group whose blocks' width `even` is
   __device__ TileWalk(const LinearParams &params, const GroupTable &table, int rows_of_tile)
       : p(params), t(table), g(0), tile_p(rows_of_tile) {}
   // get() by a whole warp, the answer in uniform registers.
@@ -137,6 +141,8 @@ template <bool kSwap> struct TileWalk {
     w.q0 = warp_uniform(w.q0);
     w.k_begin = warp_uniform(w.k_begin);
     w.k_len = warp_uniform(w.k_len);
+    if (kEven)
+      w.n = warp_uniform(w.n);
     return __all_sync(0xffffffffu, got) != 0;
   }
   // Tiles are asked for in increasing order.  False: there is no such tile.
@@ -154,8 +160,17 @@ template <bool kSwap> struct TileWalk {
       if (kSwap) {
         w.p0 = fb * tile_p;
         w.p_end = p.P;
-        w.q0 = t.begin[g] + rb * p.tile_q;
         w.q_end = t.begin[g + 1];
+        if (kEven) {
+          if (even_of != g) {
+            even_of = g;
+            even = (small_div(w.q_end - t.begin[g] + blocks - 1, blocks) + 31) & ~31;
+          }
+          w.n = even;
+          w.q0 = t.begin[g] + rb * even;
+        } else {
+          w.q0 = t.begin[g] + rb * p.tile_q;
+        }
       } else {
         w.p0 = t.begin[g] + rb * tile_p;
         w.p_end = t.begin[g + 1];

@@ -6,6 +6,16 @@
 // for the same outputs: a deeper ring and a third less shared-memory traffic.
 // Operand layouts, experts and the epilogue are those of linear_sm100.cu.
 //
+// With experts the sides may change (kSwap): 256 features are the tile's rows, and
+// its columns the tokens, so a tile is as wide as it has tokens for (an expert's
+// are shared out evenly, in steps of 32), where rows come in whole 256s.  A step's
+// time does not fall with the columns alone: what it loads and reads of shared
+// memory, 128 rows of A and up to as much of B a CTA, keeps the memory as busy as
+// 256 columns keep the tensor cores; so the host also picks the columns that are
+// loaded (tile_q).  Rows / columns in us, bf16: 3001 tokens, 1032 x 1544, 32 experts
+// 42 / 36; 8192, 4096 x 2048, 16 130 / 122; 16384, 2048 x 1024, 64 96 / 87; with
+// whole blocks (16384, 8192 x 4096, 8) 771 / 772.
+//
 // Barriers across the pair:
 //   full[s]    in the leader, armed by its loader with the bytes of both CTAs'
 //              loads (an arrival of the other CTA's loader for each stage was
@@ -80,13 +90,13 @@ __device__ __forceinline__ void tma_load_chunks_pair(void *dst, const CUtensorMa
                : "memory");
 }
 
-template <bool kAMn, bool kBMn>
+template <bool kAMn, bool kBMn, bool kSwap>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAMn && kBMn ? kThreadsCut : kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_d, const __grid_constant__ CUtensorMap tm_z,
                    const __grid_constant__ LinearParams p) {
-  constexpr bool kFull = !kAMn && !kBMn; // the forward pass
-  constexpr int kW = kFull ? 32 : 64; // columns of an epilogue chunk (see linear_sm100.cu); the two groups of four warps take turns
+  constexpr bool kFull = !kAMn && !kBMn && !kSwap; // the forward pass, tokens as rows
+  constexpr int kW = kFull || kSwap ? 32 : 64; // columns of an epilogue chunk (see linear_sm100.cu); the two groups of four warps take turns
   constexpr bool kCut = kAMn && kBMn;
   const int num_stages = p.stages;
   extern __shared__ uint8_t smem_raw[];
@@ -132,7 +142,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   const uint32_t tmem_base = sh->tmem_base;
   start_after_previous(p.beside);
   if (p.ragged != kRaggedNone)
-    build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : p.P, kPairP);
+    build_group_table(table, p.offsets, p.groups, p.ragged == kRaggedK ? p.K : (kSwap ? p.Q : p.P), kSwap ? p.tile_q : kPairP);
 
   // Contraction indices of stage kb, and whether rows behind them have to be cut away.
   auto live_of = [](const Tile &w, int kb) { return min(kBK, w.k_len - kb * kBK); };
@@ -140,7 +150,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
-    TileWalk<false> walk(p, table, kPairP);
+    TileWalk<kSwap, kSwap> walk(p, table, kPairP);
     Tile w;
     Ring ring;
     bool ok = true;
@@ -150,7 +160,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     for (int id = first_tile; ok && walk.get_uniform(id, w); id += tile_step) {
       const int kbs = (w.k_len + kBK - 1) / kBK;
       const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
-      const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * half_q;
+      const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * (kSwap ? w.n / 2 : half_q);
       bool seen = false;
       for (int kb = 0; kb < kbs; ++kb) {
         ok = warp_wait(&sh->empty[ring.stage], ring.phase ^ 1, abort_flag, seen);
@@ -217,7 +227,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   } else if (warp == 1) {
     // ------------------------------------------------ UMMA issue (leader)
     if (leader) {
-      const uint32_t idesc = umma_idesc_f16(kPairP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
+      uint32_t idesc = umma_idesc_f16(kPairP, p.tile_q, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
       constexpr uint64_t kStepA = kAMn ? (16 * 128) >> 4 : 2, kStepB = kBMn ? (16 * 128) >> 4 : 2;
       constexpr uint64_t kStep = kStageBytes >> 4;
       const uint32_t a_addr = smem_u32(tiles), b_addr = a_addr + kABytes;
@@ -225,7 +235,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       const uint64_t db0 = kBMn ? umma_desc_mnmajor_sw128(b_addr, kChunkBytes, 1024) : umma_desc_kmajor_sw128(b_addr);
       const uint32_t tmem_d = static_cast<uint32_t>(warp_uniform(static_cast<int>(tmem_base)));
       const bool chosen = elect_one();
-      TileWalk<false> walk(p, table, kPairP);
+      TileWalk<kSwap, kSwap> walk(p, table, kPairP);
       Tile w, next_w;
       Ring ring;
       int acc = 0;
@@ -234,6 +244,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       bool more_tiles = walk.get_uniform(first_tile, next_w);
       for (int id = first_tile; ok && more_tiles;) {
         w = next_w;
+        if constexpr (kSwap)
+          idesc = umma_idesc_f16(kPairP, w.n, p.is_bf16, kAMn ? 1 : 0, kBMn ? 1 : 0);
         id += tile_step;
         bool looked = false; // where the next tile lies: worked out while products are under way
         const int kbs = (w.k_len + kBK - 1) / kBK;
@@ -314,7 +326,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   } else if (kCut && warp == 2 + kEpiWarps) {
     // ------------------------------------- cutting of last stages (both CTAs)
     if constexpr (kCut) {
-      TileWalk<false> walk(p, table, kPairP);
+      TileWalk<kSwap, kSwap> walk(p, table, kPairP);
       Tile w;
       Ring ring;
       uint32_t phases = 0; // of landed: a bit to a stage
@@ -355,7 +367,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     EpiWarp ew{slots + (warp - 2) * kSlotBytes, &tm_d, &tm_z, lane};
     const uint32_t tempty_leader[2] = {map_to_cta(&sh->tempty[0], 0), map_to_cta(&sh->tempty[1], 0)};
-    TileWalk<false> walk(p, table, kPairP);
+    TileWalk<kSwap, kSwap> walk(p, table, kPairP);
     Tile w;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -381,8 +393,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       t.group = w.group;
       t.lane0 = w.p0 + rank * kRows + quarter * 32;
       t.lane_end = w.p_end;
-      t.q_end = min(w.q_end, w.q0 + p.tile_q);
-      const int my_cols = p.tile_q - col0;
+      const int cols = kSwap ? w.n : p.tile_q;
+      t.q_end = min(w.q_end, w.q0 + cols);
+      const int my_cols = cols - col0;
+      float col_bias = 0.0f; // tokens as columns: the bias of the lane's feature
+      if constexpr (kSwap)
+        col_bias = column_bias(p, t, lane);
       Ahead<kW> next;
       if (kFull && my_cols > 0)
         fetch_ahead<kW>(next, p, t, w.q0 + col0, lane);
@@ -414,7 +430,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           if (c + 2 * kW >= my_cols)
             release(); // read out: the tile after the next may use it
         }
-        epilogue_rows<false, kW, kFull>(p, t, w.q0 + col0 + c, v, next, ew);
+        if constexpr (kSwap)
+          epilogue_columns<false, kW>(p, t, w.q0 + col0 + c, v, col_bias, ew.slot, lane);
+        else
+          epilogue_rows<false, kW, kFull>(p, t, w.q0 + col0 + c, v, next, ew);
         if (kFull && c + 2 * kW < my_cols)
           fetch_ahead<kW>(next, p, t, w.q0 + col0 + c + 2 * kW, lane);
       }
@@ -425,11 +444,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       tma_store_wait<0>(); // the slots outlive the stores that read them
     if (p.zero_rest && p.ragged == kRaggedRows) {
       const int wid = static_cast<int>(blockIdx.x) * kEpiWarps + warp - 2, warps = static_cast<int>(gridDim.x) * kEpiWarps;
-      zero_rows(p.D, 2, p.ldd, 0, table.begin[0], p.Q, wid, warps, lane);
-      zero_rows(p.D, 2, p.ldd, table.begin[p.groups], p.P, p.Q, wid, warps, lane);
+      const int rows = kSwap ? p.Q : p.P, cols = kSwap ? p.P : p.Q;
+      zero_rows(p.D, 2, p.ldd, 0, table.begin[0], cols, wid, warps, lane);
+      zero_rows(p.D, 2, p.ldd, table.begin[p.groups], rows, cols, wid, warps, lane);
       if (p.Z) {
-        zero_rows(p.Z, 2, p.ldz, 0, table.begin[0], p.Q, wid, warps, lane);
-        zero_rows(p.Z, 2, p.ldz, table.begin[p.groups], p.P, p.Q, wid, warps, lane);
+        zero_rows(p.Z, 2, p.ldz, 0, table.begin[0], cols, wid, warps, lane);
+        zero_rows(p.Z, 2, p.ldz, table.begin[p.groups], rows, cols, wid, warps, lane);
       }
     }
   }
@@ -448,11 +468,11 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   }
 }
 
-template <bool kAMn, bool kBMn>
+template <bool kAMn, bool kBMn, bool kSwap>
 cudaError_t launch_one(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
   if (p.stages != linear_pair_stages(p.ragged, p.groups))
     return cudaErrorInvalidValue;
-  auto kernel = linear_pair_kernel<kAMn, kBMn>;
+  auto kernel = linear_pair_kernel<kAMn, kBMn, kSwap>;
   cudaError_t err = prepare_kernel(kernel, kSmemLimit, nullptr);
   if (err != cudaSuccess)
     return err;
@@ -478,9 +498,14 @@ int linear_pair_stages(int ragged, int groups) {
 }
 
 cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream) {
+  if (l.swap) { // with experts only
+    if (l.b_mn || p.ragged != kRaggedRows)
+      return cudaErrorInvalidValue;
+    return l.a_mn ? launch_one<true, false, true>(m, p, l, stream) : launch_one<false, false, true>(m, p, l, stream);
+  }
   if (!l.a_mn)
-    return l.b_mn ? launch_one<false, true>(m, p, l, stream) : launch_one<false, false>(m, p, l, stream);
-  return l.b_mn ? launch_one<true, true>(m, p, l, stream) : cudaErrorInvalidValue;
+    return l.b_mn ? launch_one<false, true, false>(m, p, l, stream) : launch_one<false, false, false>(m, p, l, stream);
+  return l.b_mn ? launch_one<true, true, false>(m, p, l, stream) : cudaErrorInvalidValue;
 }
 
 cudaError_t linear_pair_read_status(int out[4], bool clear) {

@@ -75,7 +75,7 @@ struct LinearLaunch {
   int tile_n;     // kernel instantiation: 16, 32, 64, 128 or 256 columns
   int out_f32;
   int grid;       // CTAs (a multiple of splits)
-  int pair;       // CTA-pair kernel: 256 x tile_q tiles, 16-bit results, tokens as rows
+  int pair;       // CTA-pair kernel: 256 x tile_q tiles, 16-bit results, tokens as rows or (with experts) columns
   int pdl;        // launch with programmatic stream serialization
 };
 
@@ -90,6 +90,7 @@ struct LinearMaps {
 cudaError_t launch_linear(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_read_status(int out[4], bool clear);
 // tile_q a multiple of 32 (of 128 where B is stored [K][Q]) up to 256; grid even.
+// With swap (experts only) tile_q bounds the tokens of a tile.
 cudaError_t launch_linear_pair(const LinearMaps &m, const LinearParams &p, const LinearLaunch &l, cudaStream_t stream);
 cudaError_t linear_pair_read_status(int out[4], bool clear);
 

@@ -266,13 +266,19 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
   const int tile_p = pair ? 256 : 128, tile_n = pair ? 256 : t.tile;
   c->pb = (e.p + tile_p - 1) / tile_p;
   c->qb = (e.q + c->tile_q - 1) / c->tile_q;
-  double about;
+  double about, width = c->tile_q;
   if (e.kind == Product::kWeightGrad) {
     c->tiles = c->pb * c->qb * e.matrices;
     about = static_cast<double>(c->tiles);
   } else if (c->swap) {
     c->tiles = c->pb * row_blocks_most(e, c->tile_q);
-    about = static_cast<double>(c->pb) * row_blocks_about(e, c->tile_q);
+    const double blocks = row_blocks_about(e, c->tile_q);
+    about = static_cast<double>(c->pb) * blocks;
+    if (pair) {
+      width = static_cast<double>(e.M) / blocks + 16.0; // (steps of 32)
+      if (width > c->tile_q)
+        width = c->tile_q;
+    }
   } else {
     c->tiles = c->qb * row_blocks_most(e, tile_p);
     about = static_cast<double>(c->qb) * row_blocks_about(e, tile_p);
@@ -286,11 +292,13 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
   const double bytes = (tile_p + c->tile_q) * 128.0;
   // (a narrower tile saves less time than columns: its other operand is as wide)
   double stage = t.stage * (1.0 - (pair ? 0.38 : 0.54) * (1.0 - static_cast<double>(c->tile_q) / tile_n));
+  if (pair && c->swap)
+    stage = t.stage * (0.5 + 0.25 * (c->tile_q + width) / tile_n);
   if (stage < 0.17) // the issue of a stage
     stage = 0.17;
   if (stage < bytes * side / kL2BytesPerUs)
     stage = bytes * side / kL2BytesPerUs;
-  const double epi = t.epi * c->tile_q / tile_n;
+  const double epi = t.epi * width / tile_n;
   const double each = mine * stage;
   const double base = t.base + epi;
   if (c->splits == 1)
@@ -329,19 +337,23 @@ Plan make_plan(Product kind, const Shape &s, bool out_f32, int sms) {
   // otherwise; beyond two tiles of them the two ways are the same.
   const bool may_swap = kind == Product::kForward && env.linear_swap != 0 && (env.linear_swap == 1 || per_expert <= 256);
   const bool may_rows = kind != Product::kForward || (env.linear_swap != 1 && (env.linear_swap == 0 || per_expert > 16));
-  for (int swap = may_rows ? 0 : 1; swap <= (may_swap ? 1 : 0); ++swap) {
-    e.p = kind == Product::kForward ? (swap ? e.N : e.M) : kind == Product::kInputGrad ? e.M : e.N;
-    e.q = kind == Product::kForward ? (swap ? e.M : e.N) : e.K;
+  // CTA pairs take experts' tokens as columns too: a tile has as many as are there.
+  const bool pairs_swap = s.grouped && kind != Product::kWeightGrad && !out_f32 && env.linear_swap != 0;
+  for (int swap = may_rows ? 0 : 1; swap <= (may_swap || pairs_swap ? 1 : 0); ++swap) {
+    const int features = kind == Product::kInputGrad ? e.K : e.N;
+    e.p = swap ? features : kind == Product::kWeightGrad ? e.N : e.M;
+    e.q = swap ? e.M : kind == Product::kForward ? e.N : e.K;
     e.k = kind == Product::kForward ? e.K : kind == Product::kInputGrad ? e.N : (s.grouped ? per_expert : e.M);
     for (const TileCost &t : kTileCosts) {
       const bool pair = t.tile == kPairTile;
       const int tile_n = pair ? 256 : t.tile;
-      if (swap ? t.tile > 128 : t.tile < 64)
+      if (pair ? swap && !pairs_swap : swap ? !may_swap || t.tile > 128 : t.tile < 64)
         continue;
       if (out_f32 && t.tile > 128)
         continue;
       // the knobs take what they can of their choice
-      if (pair ? env.linear_pair == 0 || env.linear_splits > 1 || swap : env.linear_pair == 1 && !out_f32 && !swap)
+      if (pair ? env.linear_pair == 0 || env.linear_splits > 1 || (pairs_swap && !swap && env.linear_swap == 1)
+               : env.linear_pair == 1 && !out_f32 && (!swap || pairs_swap))
         continue;
       const int knob = env.linear_tile;
       if (!pair && knob && (swap ? knob <= 128 : knob >= 64 && !(out_f32 && knob == 256)) && knob != t.tile)
@@ -352,6 +364,12 @@ Plan make_plan(Product kind, const Shape &s, bool out_f32, int sms) {
       const int unit = l.b_mn ? (pair ? 128 : 64) : (pair ? 32 : 16);
       const long long least = (e.q + tile_n - 1) / tile_n;
       int before = 0;
+      if (pair && swap) { // blocks of up to so many tokens: a stage loads that much of them
+        for (int tile_q = 64; tile_q <= 256; tile_q += 32)
+          if (!env.linear_columns || tile_q == env.linear_columns)
+            consider(t, swap, 1, tile_q);
+        continue;
+      }
       for (int more = 0; more < (l.b_mn || swap ? 1 : 4); ++more) {
         const long long n = least + more > 0 ? least + more : 1;
         int tile_q = tile_n;
@@ -382,6 +400,10 @@ Plan make_plan(Product kind, const Shape &s, bool out_f32, int sms) {
     consider(kTileCosts[3], false, 1, 128);
   }
   l.swap = best.swap;
+  if (l.swap) { // the operands change sides
+    l.a_mn = kind == Product::kInputGrad;
+    l.b_mn = 0;
+  }
   l.pair = best.tile == kPairTile;
   l.tile_n = l.pair ? 256 : best.tile;
   pl.tile_q = best.tile_q;
@@ -469,8 +491,8 @@ int run_product(Product kind, const Shape &s, const Operand &a_tok, const Operan
     p.Q = l.swap ? d.tokens : d.out_features;
     p.K = d.in_features;
   } else if (kind == Product::kInputGrad) {
-    p.P = d.tokens;
-    p.Q = d.in_features;
+    p.P = l.swap ? d.in_features : d.tokens;
+    p.Q = l.swap ? d.tokens : d.in_features;
     p.K = d.out_features;
   } else {
     p.P = d.out_features;

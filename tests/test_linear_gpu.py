@@ -288,6 +288,20 @@ def test_grouped_exact(cuda, wc, wl, m, n, k, sizes, front, io, out):
     wc.check_device_status()
 
 
+@pytest.mark.parametrize("columns,io", [(64, "bf16"), (128, "f16"), (160, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("m,n,k,sizes,front", GROUPS + [
+    (1400, 264, 520, [1, 0, 32, 33, 64, 255, 256, 257, 5], 3), (2900, 1001, 330, [513, 600, 0, 700, 1, 1023], 0),
+    (300, 40, 8, [300], 0), (5200, 2312, 136, [2600, 17, 0, 2300], 21)])
+def test_grouped_pairs_with_tokens_on_columns(cuda, wc, wl, m, n, k, sizes, front, columns, io):
+    """Tiles as wide as the experts have tokens; the last one has more tiles than pairs and more blocks than a band."""
+    with env_knobs(wc, WAVE_CUDA_LINEAR_PAIR=1, WAVE_CUDA_LINEAR_SWAP=1, WAVE_CUDA_LINEAR_COLUMNS=columns):
+        d = wc.LinearDesc(m, n, k, len(sizes), wc.BF16, wc.BF16, wc.BF16, wc.BF16, wc.F32)
+        for product in (0, 1):
+            plan = wc.linear_plan_for_sms(d, product, 148)
+            assert plan["tile_rows"] == 256 and plan["tokens_on_columns"] and plan["tile_columns"] == columns
+        test_grouped_exact(cuda, wc, wl, m, n, k, sizes, front, io, io)
+
+
 @pytest.mark.parametrize("gap", [1, 8])
 def test_grouped_strided(cuda, wc, wl, gap):
     """Gaps between rows and between the experts' matrices."""

@@ -148,12 +148,13 @@ def test_every_plan_can_run(wc, knobs):
                 p = wc.linear_plan_for_sms(d, product, sms)
                 pair = p["tile_rows"] == 256
                 f32 = product != 1 and d.y_type == wc.F32
-                unit = (128 if pair else 64) if product else (32 if pair else 16)
+                unit = (128 if pair else 64) if product and not p["tokens_on_columns"] else (32 if pair else 16)
                 assert p["tile_columns"] % unit == 0 and unit <= p["tile_columns"] <= (128 if f32 else 256), (m, n, k, p)
                 assert 1 <= p["splits"] <= 8 and p["grid"] >= 1 and p["grid"] % p["splits"] == 0
                 assert 3 <= p["stages"] <= 12
-                assert not pair or (p["splits"] == 1 and p["grid"] % 2 == 0 and not p["tokens_on_columns"] and not f32)
-                assert not p["tokens_on_columns"] or (product == 0 and p["tile_columns"] <= 128)
+                assert not pair or (p["splits"] == 1 and p["grid"] % 2 == 0 and not f32)
+                assert not p["tokens_on_columns"] or (product == 0 and p["tile_columns"] <= 128) or (
+                    pair and product < 2 and d.experts > 0)
                 if p["splits"] > 1:  # one cluster to a tile
                     rows, cols = p["tile_rows"], p["tile_columns"]
                     up = lambda a, b: -(-a // b)  # noqa: E731
