@@ -292,13 +292,15 @@ void predict(const Extents &e, const TileCost &t, int sms, Candidate *c) {
   const double bytes = (tile_p + c->tile_q) * 128.0;
   // (a narrower tile saves less time than columns: its other operand is as wide)
   double stage = t.stage * (1.0 - (pair ? 0.38 : 0.54) * (1.0 - static_cast<double>(c->tile_q) / tile_n));
-  if (pair && c->swap)
+  if (pair && c->swap) // what is loaded and what is multiplied, a quarter each (38 more problems: 2.3 % behind the best, 16 % at worst)
     stage = t.stage * (0.5 + 0.25 * (c->tile_q + width) / tile_n);
   if (stage < 0.17) // the issue of a stage
     stage = 0.17;
   if (stage < bytes * side / kL2BytesPerUs)
     stage = bytes * side / kL2BytesPerUs;
-  const double epi = t.epi * width / tile_n;
+  double epi = t.epi * width / tile_n;
+  if (pair && c->swap && epi < 0.8) // two chunks of 32 tokens, however few there are
+    epi = 0.8;
   const double each = mine * stage;
   const double base = t.base + epi;
   if (c->splits == 1)
