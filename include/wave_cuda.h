@@ -354,7 +354,7 @@ int wave_cuda_linear_workspace_bytes(const wave_linear_desc *desc, int backward,
  * GPU of `sm_count` SMs that need not be present.  For planning tools and tests. */
 typedef struct wave_linear_plan {
   int tile_rows, tile_columns; /* of the tensor core's tile; 256 rows: a pair of CTAs */
-  int tokens_on_columns;       /* forward with few tokens: features on the tile's rows */
+  int tokens_on_columns;       /* features on the tile's rows: few tokens, or experts on CTA pairs */
   int splits;                  /* CTAs of a cluster that share a tile's contraction */
   int grid, stages;
 } wave_linear_plan;
