@@ -147,6 +147,11 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   // Contraction indices of stage kb, and whether rows behind them have to be cut away.
   auto live_of = [](const Tile &w, int kb) { return min(kBK, w.k_len - kb * kBK); };
   auto is_cut = [&](int live) { return kCut && p.ragged == kRaggedK && live < kBK; };
+  // The stage that has to be cut is the first of its tile in the ring, and its
+  // products follow those of the next kCutLag, so that the cutting is not waited for
+  // (15 experts of 546 rows, 4096 x 2048: the last in both 141 us; after 1 / 2 / 3
+  // others 127 / 127.5 / 126.5, of 1010 rows 208, 196 / 199 / 196).
+  constexpr int kCutLag = 1;
 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
@@ -162,7 +167,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       const int za = p.group_a ? w.group : 0, zb = p.group_b ? w.group : 0;
       const int pa = w.p0 + rank * kRows, qb = w.q0 + rank * (kSwap ? w.n / 2 : half_q);
       bool seen = false;
-      for (int kb = 0; kb < kbs; ++kb) {
+      const bool cut = is_cut(live_of(w, kbs - 1));
+      for (int i = 0; i < kbs; ++i) {
+        const int kb = !cut ? i : i == 0 ? kbs - 1 : i - 1;
         ok = warp_wait(&sh->empty[ring.stage], ring.phase ^ 1, abort_flag, seen);
         if (!ok) {
           pair_report(kStatusWaitTimeout, 0, ring.stage);
@@ -175,7 +182,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         const int k = w.k_begin + kb * kBK;
         ring.advance(num_stages);
         seen = warp_peek(&sh->empty[ring.stage], ring.phase ^ 1);
-        if (kCut && is_cut(live_of(w, kb))) {
+        if (kCut && cut && i == 0) {
           if (chosen) {
             // this CTA's bytes on its own barrier: the cutting warp takes them over
             mbar_arrive_expect_tx(landed, tx);
@@ -260,55 +267,66 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             pair_report(kStatusWaitTimeout, 1, 100 + acc);
             break;
           }
-          bool seen = false;
-          for (int i = 0; i < whole; ++i) {
-            ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, seen);
-            if (!ok) {
-              pair_report(kStatusWaitTimeout, 1, ring.stage);
-              break;
-            }
-            tc_fence_after_sync();
-            const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
-            uint64_t *done = &sh->empty[ring.stage];
+          const int cut_stage = ring.stage;
+          if (cut)
             ring.advance(num_stages);
-            seen = warp_peek(&sh->full[ring.stage], ring.phase);
-            if (chosen) {
-              umma_ss_pair(d, da, db, idesc, more);
+          auto issue = [&](int stages) {
+            bool seen = false;
+            for (int i = 0; i < stages; ++i) {
+              ok = warp_wait(&sh->full[ring.stage], ring.phase, abort_flag, seen);
+              if (!ok) {
+                pair_report(kStatusWaitTimeout, 1, ring.stage);
+                break;
+              }
+              tc_fence_after_sync();
+              const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
+              uint64_t *done = &sh->empty[ring.stage];
+              ring.advance(num_stages);
+              seen = warp_peek(&sh->full[ring.stage], ring.phase);
+              if (chosen) {
+                umma_ss_pair(d, da, db, idesc, more);
 #pragma unroll
-              for (int k = 1; k < kBK / 16; ++k)
-                umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
-              umma_commit_pair(done, 3); // frees the stage in both CTAs
+                for (int k = 1; k < kBK / 16; ++k)
+                  umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+                umma_commit_pair(done, 3); // frees the stage in both CTAs
+              }
+              __syncwarp();
+              more = 1;
+              if (!looked) {
+                more_tiles = walk.get_uniform(id, next_w);
+                looked = true;
+              }
             }
-            __syncwarp();
-            more = 1;
-            if (!looked) {
-              more_tiles = walk.get_uniform(id, next_w);
-              looked = true;
-            }
-          }
+          };
+          const int before = cut ? min(whole, kCutLag) : whole;
+          issue(before);
           if (!ok)
             break;
           if constexpr (kCut) {
             if (cut) {
-              const uint32_t parity = (cut_phases >> ring.stage) & 1u;
-              cut_phases ^= 1u << ring.stage;
-              ok = warp_wait_cluster(&sh->cut[ring.stage], parity, abort_flag);
+              const uint32_t parity = (cut_phases >> cut_stage) & 1u;
+              cut_phases ^= 1u << cut_stage;
+              ok = warp_wait_cluster(&sh->cut[cut_stage], parity, abort_flag);
               if (!ok) {
-                pair_report(kStatusWaitTimeout, 1, 70 + ring.stage);
+                pair_report(kStatusWaitTimeout, 1, 70 + cut_stage);
                 break;
               }
               fence_proxy_async_smem();
               tc_fence_after_sync();
               const int steps = (live + 15) / 16;
               if (chosen) {
-                mbar_arrive(&sh->full[ring.stage]); // the stage's turn of this barrier
-                const uint64_t da = da0 + static_cast<uint64_t>(ring.stage) * kStep, db = db0 + static_cast<uint64_t>(ring.stage) * kStep;
-                for (int k = 0; k < steps; ++k, more = 1)
-                  umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, more);
-                umma_commit_pair(&sh->empty[ring.stage], 3);
+                mbar_arrive(&sh->full[cut_stage]); // the stage's turn of this barrier
+                const uint64_t da = da0 + static_cast<uint64_t>(cut_stage) * kStep, db = db0 + static_cast<uint64_t>(cut_stage) * kStep;
+                umma_ss_pair(d, da, db, idesc, more);
+                for (int k = 1; k < steps; ++k)
+                  umma_ss_pair(d, da + k * kStepA, db + k * kStepB, idesc, 1u);
+                umma_commit_pair(&sh->empty[cut_stage], 3);
               }
               __syncwarp();
-              ring.advance(num_stages);
+              more = 1;
+              issue(whole - before);
+              if (!ok)
+                break;
             }
           }
           if (chosen)
@@ -336,16 +354,17 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           continue;
         const int live = live_of(w, kbs - 1);
         const bool cut = is_cut(live);
-        ring.stage = (ring.stage + kbs - (cut ? 1 : 0)) % num_stages;
+        const int stage = ring.stage;
+        ring.stage = (ring.stage + kbs) % num_stages;
         if (!cut)
           continue;
-        const uint32_t parity = (phases >> ring.stage) & 1u;
-        phases ^= 1u << ring.stage;
-        if (!warp_wait(&sh->landed[ring.stage], parity, abort_flag, false)) {
-          pair_report(kStatusWaitTimeout, 3, ring.stage);
+        const uint32_t parity = (phases >> stage) & 1u;
+        phases ^= 1u << stage;
+        if (!warp_wait(&sh->landed[stage], parity, abort_flag, false)) {
+          pair_report(kStatusWaitTimeout, 3, stage);
           break;
         }
-        uint8_t *a_tile = tiles + ring.stage * kStageBytes;
+        uint8_t *a_tile = tiles + stage * kStageBytes;
         const int steps = (live + 15) / 16;
         const int vecs = (steps * 16 - live) * 8; // 16-byte pieces in a chunk
         const int chunks = kRows / 64 + p.tile_q / 128;
@@ -355,9 +374,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0)
-          mbar_arrive_cluster(map_to_cta(&sh->cut[ring.stage], 0));
+          mbar_arrive_cluster(map_to_cta(&sh->cut[stage], 0));
         __syncwarp();
-        ring.stage = (ring.stage + 1) % num_stages;
       }
     }
   } else {
