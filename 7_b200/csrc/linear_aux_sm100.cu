@@ -65,7 +65,10 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
 constexpr int kAgThreads = 256;
 constexpr int kAgCols = 256;                   // columns of a block, eight to a thread
 constexpr int kAgLanes = kAgThreads / (kAgCols / 8); // rows side by side
-constexpr int kAgUnroll = 4;                   // rows in flight for each thread
+// Rows in flight for each thread, where the registers of four blocks to an SM are
+// to hold them without spilling (8192 x 8192 bf16, gelu_tanh: 2 rows in 80 us, 3 in
+// 83, 4 in 110), and elsewhere.
+constexpr int kAgUnrollVec = 2, kAgUnroll = 4;
 
 struct Eight {
   float v[8];
@@ -126,13 +129,13 @@ template <bool kF32> __device__ __forceinline__ Eight values(const Raw<kF32> &r,
 }
 
 // Rows r, r + kLanes, ... below r1 of eight columns: dz written, its column sums added to acc.
-template <int kAct, bool kDyF32, bool kVec, int kLanes>
+template <int kAct, bool kDyF32, bool kVec, int kLanes, int kUnroll>
 __device__ __forceinline__ void act_grad_rows(const LinearActGrad &p, int r, int r1, int col, int live, float (&acc)[8]) {
-  for (; r < r1; r += kLanes * kAgUnroll) {
-    Raw<kDyF32> dy_raw[kAgUnroll];
-    Raw<false> z_raw[kAgUnroll];
+  for (; r < r1; r += kLanes * kUnroll) {
+    Raw<kDyF32> dy_raw[kUnroll];
+    Raw<false> z_raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kAgUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
       const int row = r + u * kLanes;
       if (row < r1) {
         load_raw<kDyF32, kVec>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
@@ -141,7 +144,7 @@ __device__ __forceinline__ void act_grad_rows(const LinearActGrad &p, int r, int
       }
     }
 #pragma unroll
-    for (int u = 0; u < kAgUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
       const int row = r + u * kLanes;
       if (row >= r1)
         break;
@@ -226,7 +229,7 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
   if (live > 0)
-    act_grad_rows<kAct, kDyF32, kVec, kAgLanes>(p, r0 + tr, r1, col, live, acc);
+    act_grad_rows<kAct, kDyF32, kVec, kAgLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
   if (!p.partial)
     return;
 #pragma unroll
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
   if (live > 0)
-    act_grad_rows<kAct, kDyF32, kVec, kShortLanes>(p, r0 + tr, r1, col, live, acc);
+    act_grad_rows<kAct, kDyF32, kVec, kShortLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
   // the eight rows of a warp, then the warps, in order
 #pragma unroll
   for (int e = 0; e < 8; ++e) {

@@ -590,13 +590,14 @@ int chunk_rows(const Shape &s, int sms) {
 }
 
 // Whether a block takes all rows of a group: one launch instead of two, and with
-// experts no search for the group of a chunk in each of many blocks.  Column sums
-// of gelu's gradient, bf16, all rows / chunks in us: 64 x 512 2.1 / 3.8, 128 x
-// 4096 2.7 / 4.1, 500 x 1024 5.2 / 4.1, 1000 x 1024 7.6 / 5.4; 24 experts, 700 x
-// 520 2.8 / 6.1; 32, 3000 x 1032 8.2 / 11.1; 16, 8192 x 4096 37 / 49.
+// experts no search for the group of a chunk in each of many blocks.  What the
+// gradient of gelu or silu and the column sums add to dx, bf16, all rows / chunks
+// in us: 64 x 512 2.4 / 3.7, 128 x 4096 3.0 / 4.4, 250 x 1024 3.6 / 4.0, 500 x 1024
+// 5.4 / 4.2; 24 experts, 700 x 520 2.5 / 4.8; 32, 3000 x 1032 7.0 / 10; 15, 8190 x
+// 4096 41 / 44; 64, 16384 x 1024 31 / 27; 8, 8000 x 2048 30 / 24.
 bool short_groups(const Shape &s) {
   const long long rows = (s.d.tokens + s.matrices - 1) / s.matrices;
-  return rows <= (s.grouped ? 1024 : 256);
+  return rows <= (s.grouped ? 640 : 256);
 }
 
 struct BackwardLayout {
