@@ -16,8 +16,8 @@ namespace linear_detail {
 // waits only at its end, so that whoever waits for it has waited for both.  So
 // the weight gradient's CTAs take the SMs that the input gradient's last round
 // leaves idle, and small products run side by side (with it / one after the other,
-// in us: 8192 x 8192 x 2048 462 / 482, 515 x 1032 x 776 18.6 / 20.1, 24 experts,
-// 700 x 520 x 1288 34.5 / 37.5).
+// in us: 8192 x 8192 x 2048 446 / 466, 515 x 1032 x 776 18.3 / 19.8, 24 experts,
+// 700 x 520 x 1288 34.5 / 37.8).
 __device__ __forceinline__ void start_after_previous(int beside) {
   if (!beside)
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -207,7 +207,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     // Like the issuing warp below, the whole warp walks and waits and one elected
     // lane acts: with the loop in one lane's branch the compiler cannot keep the
     // operands of the copies and products in uniform registers, and a stage takes
-    // 0.28 us to issue whatever the size of its tile (now 0.11).
+    // 0.28 us to issue whatever the size of its tile (now 0.18).
     TileWalk<kSwap> walk(p, table, kTileP);
     Tile w;
     Ring ring;
