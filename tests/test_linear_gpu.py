@@ -570,6 +570,57 @@ def test_graph_capture_and_replay(cuda, wc, wl):
     wc.check_device_status()
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("m,n,k,experts", [(515, 1032, 776, 0), (300, 136, 4096, 0), (2304, 2048, 1024, 0), (700, 520, 1288, 6), (4096, 72, 2568, 3)])
+def test_launches_side_by_side(cuda, wc, wl, m, n, k, experts, captured):
+    """The backward pass' products overlap: what follows on the stream (another layer, the inputs written anew) sees all of
+    them finished, and the next call does not disturb them."""
+    torch, gen = cuda, make_gen(cuda, m)
+    lead = (experts,) if experts else ()
+    x, w, dy, z = (torch.randn(s, generator=gen, device="cuda").to(torch.bfloat16) for s in ((m, k), (*lead, n, k), (m, n), (m, n)))
+    v = torch.randn(64, k, generator=gen, device="cuda").to(torch.bfloat16)
+    off = offsets_of(torch, [m // experts] * (experts - 1) + [m - m // experts * (experts - 1)]) if experts else None
+
+    def backward(dy, x, z, **need):
+        if experts:
+            return wl.grouped_linear_backward(dy, x, w, off, activation="silu", pre_activation=z, **need)
+        return wl.linear_backward(dy, x, w, activation="silu", pre_activation=z, **need)
+
+    alone = []
+    for i, name in enumerate(("need_dx", "need_dweight", "need_dbias")):
+        alone.append(backward(dy, x, z, **{o: o == name for o in ("need_dx", "need_dweight", "need_dbias")})[i])
+        torch.cuda.synchronize()
+    alone.append(wl.linear(alone[0], v))
+    torch.cuda.synchronize()
+    dy1, x1, z1 = (torch.empty_like(t) for t in (dy, x, z))
+
+    def step():
+        for to, t in ((dy1, dy), (x1, x), (z1, z)):
+            to.copy_(t)
+        dx, dw, db = backward(dy1, x1, z1)
+        y = wl.linear(dx, v)  # another layer reads dx at once
+        for t in (dy1, x1, z1):
+            t.fill_(float("nan"))
+        again = backward(dy, x, z)
+        return [dx, dw, db, y, *again]
+
+    if captured:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+    for _ in range(5):
+        if captured:
+            graph.replay()
+        else:
+            got = step()
+        torch.cuda.synchronize()
+        for g, e in zip(got, alone + alone[:3]):
+            assert torch.equal(g, e)
+    wc.check_device_status()
+
+
 def test_same_call_same_bits(cuda, wc, wl):
     torch, gen = cuda, make_gen(cuda, 15)
     for m, n, k in ((3, 2048, 2048), (200, 520, 1000)):
