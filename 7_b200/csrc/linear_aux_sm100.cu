@@ -80,7 +80,8 @@ template <bool kF32> struct Raw {
 };
 
 // kVec: all eight exist and are aligned; else `live` of them exist and the others are zero.
-template <bool kF32, bool kVec>
+// kOnce: nobody reads them again, they may leave L2 first.
+template <bool kF32, bool kVec, bool kOnce>
 __device__ __forceinline__ void load_raw(Raw<kF32> &out, const void *base, long long at, int live) {
   if constexpr (kF32) {
     const uint32_t *src = static_cast<const uint32_t *>(base) + at;
@@ -98,7 +99,7 @@ __device__ __forceinline__ void load_raw(Raw<kF32> &out, const void *base, long 
   } else {
     const uint16_t *src = static_cast<const uint16_t *>(base) + at;
     if constexpr (kVec) {
-      out.w[0] = *reinterpret_cast<const uint4 *>(src);
+      out.w[0] = kOnce ? __ldcs(reinterpret_cast<const uint4 *>(src)) : *reinterpret_cast<const uint4 *>(src);
     } else {
       uint32_t t[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -129,7 +130,7 @@ template <bool kF32> __device__ __forceinline__ Eight values(const Raw<kF32> &r,
 }
 
 // Rows r, r + kLanes, ... below r1 of eight columns: dz written, its column sums added to acc.
-template <int kAct, bool kDyF32, bool kVec, int kLanes, int kUnroll>
+template <int kAct, bool kDyF32, bool kVec, bool kOnce, int kLanes, int kUnroll>
 __device__ __forceinline__ void act_grad_rows(const LinearActGrad &p, int r, int r1, int col, int live, float (&acc)[8]) {
   for (; r < r1; r += kLanes * kUnroll) {
     Raw<kDyF32> dy_raw[kUnroll];
@@ -138,9 +139,9 @@ __device__ __forceinline__ void act_grad_rows(const LinearActGrad &p, int r, int
     for (int u = 0; u < kUnroll; ++u) {
       const int row = r + u * kLanes;
       if (row < r1) {
-        load_raw<kDyF32, kVec>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
+        load_raw<kDyF32, kVec, kOnce>(dy_raw[u], p.dY, static_cast<long long>(row) * p.ldy + col, live);
         if constexpr (kAct >= 0)
-          load_raw<false, kVec>(z_raw[u], p.Z, static_cast<long long>(row) * p.ldz + col, live);
+          load_raw<false, kVec, kOnce>(z_raw[u], p.Z, static_cast<long long>(row) * p.ldz + col, live);
       }
     }
 #pragma unroll
@@ -192,7 +193,10 @@ __device__ __forceinline__ void store_dbias(const LinearActGrad &p, int group, i
 // costs more than the arithmetic (8192 x 8192 bf16, gelu_tanh: 243 us).
 // Bound by memory: what counts is bytes in flight, so rows wait in registers as
 // they lie in memory (widened on arrival they took 98 registers and left two
-// blocks to an SM: 177 us).
+// blocks to an SM: 177 us).  dy and z leave L2 first, so that more of dz is there
+// for the products (4096 x 8192, silu, with dx 59.0 -> 55.4 us, 16384 x 2048 56.6 ->
+// 53.0); not where dz is dy itself, nor in the kernel for short groups, whose
+// neighbours share lines (15 experts, backward 301 -> 310).
 template <int kAct, bool kDyF32, bool kVec>
 __global__ void __launch_bounds__(kAgThreads, kVec && !kDyF32 ? 4 : 2)
 act_grad_kernel(const __grid_constant__ LinearActGrad p) {
@@ -229,7 +233,7 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
   if (live > 0)
-    act_grad_rows<kAct, kDyF32, kVec, kAgLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
+    act_grad_rows<kAct, kDyF32, kVec, (kAct >= 0), kAgLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
   if (!p.partial)
     return;
 #pragma unroll
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
   if (live > 0)
-    act_grad_rows<kAct, kDyF32, kVec, kShortLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
+    act_grad_rows<kAct, kDyF32, kVec, false, kShortLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
   // the eight rows of a warp, then the warps, in order
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
