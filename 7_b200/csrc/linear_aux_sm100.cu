@@ -283,15 +283,17 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
   }
 }
 
-// Short groups: all rows of a group x 32 columns to a block, dz and the finished
-// column sums in one launch, without partial sums in memory.  Four threads to a
-// row, 64 rows side by side.
-constexpr int kShortCols = 32;
-constexpr int kShortLanes = kAgThreads / (kShortCols / 8);
-template <int kAct, bool kDyF32, bool kVec>
+// Short groups: all rows of a group x 32 or 64 columns to a block, dz and the
+// finished column sums in one launch, without partial sums in memory.  64 columns
+// are whole lines of 128 bytes, which nobody else reads (they leave L2 first); 32
+// are for few groups, where there would be too few blocks.  With dx, 32 / 64
+// columns in us: 64 groups of 200 rows x 2048 66 / 52, 16 of 300 x 4096 47 / 39, 15
+// of 546 x 4096 73 / 67, 32 of 94 x 1032 17.0 / 16.0; one of 250 x 1024 11.1 / 12.6,
+// one of 250 x 4096 13.5 / 14.9.
+template <int kAct, bool kDyF32, bool kVec, int kCols>
 __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid_constant__ LinearActGrad p) {
   extern __shared__ int ag_smem[];
-  __shared__ float sums[kAgThreads / 32][kShortCols];
+  __shared__ float sums[kAgThreads / 32][kCols];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int r0 = 0, r1 = p.rows;
@@ -301,30 +303,30 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid
     r0 = t.begin[blockIdx.y];
     r1 = t.begin[blockIdx.y + 1];
   }
-  const int tc = threadIdx.x % (kShortCols / 8), tr = threadIdx.x / (kShortCols / 8);
-  const int col = static_cast<int>(blockIdx.x) * kShortCols + tc * 8;
+  const int tc = threadIdx.x % (kCols / 8), tr = threadIdx.x / (kCols / 8);
+  const int col = static_cast<int>(blockIdx.x) * kCols + tc * 8;
   const int live = p.cols - col;
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     acc[e] = 0.0f;
   if (live > 0)
-    act_grad_rows<kAct, kDyF32, kVec, false, kShortLanes, (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
-  // the eight rows of a warp, then the warps, in order
+    act_grad_rows<kAct, kDyF32, kVec, (kAct >= 0 && kCols * 2 >= 128), kAgThreads / (kCols / 8), (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
+  // the rows of a warp, then the warps, in order
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1)
+    for (int d = kCols / 8; d < 32; d <<= 1)
       acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], d);
   }
-  if ((threadIdx.x & 31) < kShortCols / 8) {
+  if ((threadIdx.x & 31) < kCols / 8) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       sums[threadIdx.x / 32][tc * 8 + e] = acc[e];
   }
   __syncthreads();
-  const int c = static_cast<int>(blockIdx.x) * kShortCols + static_cast<int>(threadIdx.x);
-  if (p.dbias && threadIdx.x < kShortCols && c < p.cols) {
+  const int c = static_cast<int>(blockIdx.x) * kCols + static_cast<int>(threadIdx.x);
+  if (p.dbias && threadIdx.x < kCols && c < p.cols) {
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < kAgThreads / 32; ++i)
@@ -355,15 +357,15 @@ int linear_act_grad_chunks(int rows, int groups, int chunk_rows) {
 
 namespace {
 // The instantiation for the call's activation, type of dy and alignment.
-template <typename Go> void pick_act_grad(const LinearActGrad &p, Go go) {
+template <int kCols, typename Go> void pick_act_grad(const LinearActGrad &p, Go go) {
   auto with = [&](auto f32, auto vec) {
     constexpr bool kF32 = decltype(f32)::value, kVec = decltype(vec)::value;
     switch (p.Z ? p.act : kActNone) {
-    case kActRelu: go(act_grad_kernel<kActRelu, kF32, kVec>, act_grad_short_kernel<kActRelu, kF32, kVec>); break;
-    case kActGelu: go(act_grad_kernel<kActGelu, kF32, kVec>, act_grad_short_kernel<kActGelu, kF32, kVec>); break;
-    case kActGeluTanh: go(act_grad_kernel<kActGeluTanh, kF32, kVec>, act_grad_short_kernel<kActGeluTanh, kF32, kVec>); break;
-    case kActSilu: go(act_grad_kernel<kActSilu, kF32, kVec>, act_grad_short_kernel<kActSilu, kF32, kVec>); break;
-    default: go(act_grad_kernel<-1, kF32, kVec>, act_grad_short_kernel<-1, kF32, kVec>); break;
+    case kActRelu: go(act_grad_kernel<kActRelu, kF32, kVec>, act_grad_short_kernel<kActRelu, kF32, kVec, kCols>); break;
+    case kActGelu: go(act_grad_kernel<kActGelu, kF32, kVec>, act_grad_short_kernel<kActGelu, kF32, kVec, kCols>); break;
+    case kActGeluTanh: go(act_grad_kernel<kActGeluTanh, kF32, kVec>, act_grad_short_kernel<kActGeluTanh, kF32, kVec, kCols>); break;
+    case kActSilu: go(act_grad_kernel<kActSilu, kF32, kVec>, act_grad_short_kernel<kActSilu, kF32, kVec, kCols>); break;
+    default: go(act_grad_kernel<-1, kF32, kVec>, act_grad_short_kernel<-1, kF32, kVec, kCols>); break;
     }
   };
   const bool vec = p.vec_dy && (!p.Z || p.vec_z) && p.cols % 8 == 0;
@@ -379,14 +381,15 @@ cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
   const unsigned groups = static_cast<unsigned>(p.offsets ? p.groups : 1);
   cudaError_t err = cudaSuccess;
   if (p.short_groups) {
-    const dim3 grid(static_cast<unsigned>((p.cols + kShortCols - 1) / kShortCols), groups);
-    pick_act_grad(p, [&](auto, auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
+    const dim3 grid(static_cast<unsigned>((p.cols + p.short_cols - 1) / p.short_cols), groups);
+    auto go = [&](auto, auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); };
+    p.short_cols == 64 ? pick_act_grad<64>(p, go) : pick_act_grad<32>(p, go);
     return err;
   }
   const int chunks = linear_act_grad_chunks(p.rows, p.offsets ? p.groups : 0, p.chunk_rows);
   if (chunks > 0) {
     const dim3 grid(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks));
-    pick_act_grad(p, [&](auto kernel, auto) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
+    pick_act_grad<32>(p, [&](auto kernel, auto) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
   }
   if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
     return err;

@@ -124,6 +124,7 @@ struct LinearActGrad {
   int dbias_type; // 0 f32, 1 f16, 2 bf16
   int vec_dy, vec_z;
   int short_groups; // all rows of a group to a block: no `partial`, one launch
+  int short_cols;   // columns of such a block, 32 or 64
   int pdl;
 };
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows); // upper bound, sizes `partial`

@@ -599,8 +599,8 @@ int chunk_rows(const Shape &s, int sms) {
 // experts no search for the group of a chunk in each of many blocks.  What the
 // gradient of gelu or silu and the column sums add to dx, bf16, all rows / chunks
 // in us: 64 x 512 2.4 / 3.7, 128 x 4096 3.0 / 4.4, 250 x 1024 3.6 / 4.0, 500 x 1024
-// 5.4 / 4.2; 24 experts, 700 x 520 2.5 / 4.8; 32, 3000 x 1032 7.0 / 10; 15, 8190 x
-// 4096 41 / 44; 64, 16384 x 1024 31 / 27; 8, 8000 x 2048 30 / 24.
+// 5.4 / 4.2; 24 experts, 700 x 520 2.5 / 4.8; 32, 3000 x 1032 6.0 / 10; 15, 8190 x
+// 4096 35 / 44; 64, 16384 x 1024 21 / 27; 8, 8000 x 2048 30 / 23.
 bool short_groups(const Shape &s) {
   const long long rows = (s.d.tokens + s.matrices - 1) / s.matrices;
   return rows <= (s.grouped ? 640 : 256);
@@ -758,6 +758,7 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
       g.lddz = b.lddz;
       g.partial = dbias && !b.short_groups ? reinterpret_cast<float *>(ws + b.dz_bytes) : nullptr;
       g.short_groups = b.short_groups;
+      g.short_cols = (d->out_features + 63ll) / 64 * s.matrices >= 2ll * sms ? 64 : 32;
       g.chunk_rows = b.chunk;
       g.dbias = dbias;
       g.dbias_type = s.d.dbias_type == WAVE_F32 ? 0 : is_bf16 ? 2 : 1;
