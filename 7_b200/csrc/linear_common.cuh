@@ -2,6 +2,7 @@
 // ranges, the walk over the output tiles, the activations and the epilogue.
 #pragma once
 #include "linear_sm100.h"
+#include "slot_turns.h"
 #include "sm100_ptx.cuh"
 
 #include <math.h>
@@ -618,17 +619,22 @@ struct EpiWarp {
   int lane;
   int other_half = kSlotBytes / 2; // from the half in use to the other
 };
-// Takes the slot, or its other half: the stores that read it have done so.
-template <bool kHalves> __device__ __forceinline__ void slot_next(EpiWarp &e) {
-  if constexpr (kHalves) {
-    e.slot += e.other_half;
-    e.other_half = -e.other_half;
-    if (e.lane == 0)
-      tma_store_wait_read<1>();
-  } else {
-    if (e.lane == 0)
-      tma_store_wait_read<0>();
+// The bulk groups of a warp's stores: lane 0 issues them all.
+struct LaneZeroBulk {
+  int lane;
+  template <int N> __device__ __forceinline__ void wait_read() const {
+    if (lane == 0)
+      tma_store_wait_read<N>();
   }
+  __device__ __forceinline__ void commit() const {
+    if (lane == 0)
+      tma_store_commit();
+  }
+};
+// Takes the slot, or its other half: the stores that read it have done so.  Each
+// slot_next is followed by one slot_out.
+template <bool kHalves> __device__ __forceinline__ void slot_next(EpiWarp &e) {
+  slot_take<kHalves>(e.slot, e.other_half, LaneZeroBulk{e.lane});
   __syncwarp();
 }
 template <int kElem, int W>
@@ -637,15 +643,14 @@ __device__ __forceinline__ void slot_out(const EpiWarp &e, const CUtensorMap *ma
   if (W * kElem >= 64 && tma) {
     fence_proxy_async_smem();
     __syncwarp();
-    if (e.lane == 0) {
+    if (e.lane == 0)
       tma_store_3d(map, e.slot, q0, p0, group);
-      tma_store_commit();
-    }
   } else {
     __syncwarp();
     slot_to_global<kElem, W>(e.slot, base, ld, rows, cols, vec, e.lane);
     __syncwarp();
   }
+  slot_leave(LaneZeroBulk{e.lane});
 }
 
 // Tokens as rows: v holds columns q0 .. q0 + W of the lane's row.  kFull: the
