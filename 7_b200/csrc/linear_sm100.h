@@ -103,8 +103,11 @@ struct PackRows {
   void *dst;
   long long ld_dst, group_dst;
   int rows, cols, groups;
+  const int *offsets; // not null: matrices of groups without any of the `tokens` rows are neither read nor written
+  int tokens;
 };
-cudaError_t launch_pack_rows(const PackRows &first, const PackRows &second, int pdl, cudaStream_t stream);
+// x is one matrix, the weights one or one for each group; either may be nothing.
+cudaError_t launch_pack_rows(const PackRows &x, const PackRows &weights, int pdl, cudaStream_t stream);
 
 // dz = dy * act'(z), rounded to the operands' type, and the column sums of the
 // unrounded dz (dbias) of each group in two steps of fixed order.

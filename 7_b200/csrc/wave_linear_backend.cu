@@ -164,13 +164,15 @@ struct Operand {
 };
 
 // Describes the layout of an operand in `to` whose strides are not multiples of
-// 16 bytes, and points it there; nothing for one that is fine as it is.
-wave::PackRows pack(Operand *o, char **to) {
+// 16 bytes, and points it there; nothing for one that is fine as it is.  With
+// `offsets` (the experts' weights) only of the experts that have rows.
+wave::PackRows pack(Operand *o, char **to, const int *offsets = nullptr, int tokens = 0) {
   wave::PackRows p{};
   if (!o->packed())
     return p;
   const long long ld = o->packed_ld(), group = ld * o->rows;
-  p = wave::PackRows{o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices};
+  p = wave::PackRows{o->ptr, o->ld, o->matrices > 1 ? o->group : 0, *to, ld, group, o->rows, o->cols, o->matrices,
+                     offsets, tokens};
   const size_t bytes = o->packed_bytes();
   o->ptr = *to;
   o->ld = ld;
@@ -178,8 +180,8 @@ wave::PackRows pack(Operand *o, char **to) {
   *to += bytes;
   return p;
 }
-int run_packs(const wave::PackRows &first, const wave::PackRows &second, cudaStream_t stream) {
-  const cudaError_t err = wave::launch_pack_rows(first, second, wave::env_knobs().linear_pdl, stream);
+int run_packs(const wave::PackRows &x, const wave::PackRows &weights, cudaStream_t stream) {
+  const cudaError_t err = wave::launch_pack_rows(x, weights, wave::env_knobs().linear_pdl, stream);
   return err == cudaSuccess ? WAVE_OK : cuda_fail(err, "linear: laying out an operand");
 }
 
@@ -703,7 +705,7 @@ int wave_cuda_linear_fwd(const wave_linear_desc *d, const void *X, const void *W
                   x.packed_bytes() + w.packed_bytes());
     char *ws = static_cast<char *>(workspace);
     cudaStream_t q = static_cast<cudaStream_t>(stream);
-    const wave::PackRows px = pack(&x, &ws), pw = pack(&w, &ws);
+    const wave::PackRows px = pack(&x, &ws), pw = pack(&w, &ws, s.grouped ? offsets : nullptr, d->tokens);
     if ((rc = run_packs(px, pw, q)) != WAVE_OK)
       return rc;
     const bool f32 = s.d.y_type == WAVE_F32;
@@ -778,8 +780,9 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
     // The products need nothing of the column sums, nor the second product of the first.
     bool beside = dbias && !(dz_wanted && b.short_groups);
     if (s.d.tokens > 0) {
-      const wave::PackRows pw = dX ? pack(&w, &ws) : wave::PackRows{}, px = dW ? pack(&x, &ws) : wave::PackRows{};
-      if ((rc = run_packs(pw, px, q)) != WAVE_OK)
+      const wave::PackRows pw = dX ? pack(&w, &ws, s.grouped ? offsets : nullptr, d->tokens) : wave::PackRows{};
+      const wave::PackRows px = dW ? pack(&x, &ws) : wave::PackRows{};
+      if ((rc = run_packs(px, pw, q)) != WAVE_OK)
         return rc;
       if (pw.groups + px.groups > 0)
         beside = false;
