@@ -342,8 +342,8 @@ template <int kAct> __device__ __forceinline__ float2 slope_pair(float2 z) {
     return __ffma2_rn(__fmul2_rn(zc, both(0.3989422804014327f)), gauss, phi);
   } else if constexpr (kAct == kActGeluTanh || kAct == kActSilu) {
     // z s with s = sigmoid(r z), r = 1 or 2c (1 + a z^2): s + z s (1 - s) (r z)' = s (1 + (1 - s) z (r z)').
-    // Beyond +-64 (+-16) that is 1 or 0 in f32; cut there, lest (1 - s) z becomes 0 * infinity.
-    constexpr float kCutAt = kAct == kActSilu ? 64.0f : 16.0f;
+    // Beyond +-128 (+-16) that is 1 or 0 in f32; cut there, lest (1 - s) z becomes 0 * infinity.
+    constexpr float kCutAt = kAct == kActSilu ? 128.0f : 16.0f;
     const float2 c = make_float2(fminf(fmaxf(z.x, -kCutAt), kCutAt), fminf(fmaxf(z.y, -kCutAt), kCutAt));
     float2 s, w;
     if constexpr (kAct == kActSilu) {
