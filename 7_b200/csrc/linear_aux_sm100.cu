@@ -102,6 +102,7 @@ constexpr int kAgLanes = kAgThreads / (kAgCols / 8); // rows side by side
 // to hold them without spilling (8192 x 8192 bf16, gelu_tanh: 2 rows in 80 us, 3 in
 // 83, 4 in 110), and elsewhere.
 constexpr int kAgUnrollVec = 2, kAgUnroll = 4;
+constexpr int kShortRows = 1024; // most rows of a block of the kernel for short groups
 
 struct Eight {
   float v[8];
@@ -218,6 +219,19 @@ __device__ __forceinline__ void store_dbias(const LinearActGrad &p, int group, i
     static_cast<uint16_t *>(p.dbias)[at] = to_16bit(v, p.dbias_type == 2);
 }
 
+// The group with blocks[g] <= block < blocks[g + 1].
+__device__ __forceinline__ int group_of_block(const GroupTable &t, int groups, int block) {
+  int lo = 0, hi = groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.blocks[mid] <= block)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
 // One chunk of rows x 256 columns to a block.  A chunk never crosses a group's
 // end, so its column sums go to one group; which rows chunk `blockIdx.y` has
 // comes from the offsets, on the device.
@@ -244,16 +258,9 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
     const int chunk = blockIdx.y;
     if (chunk >= t.blocks[p.groups])
       return;
-    int lo = 0, hi = p.groups; // the group with blocks[lo] <= chunk < blocks[lo + 1]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (t.blocks[mid] <= chunk)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    r0 = t.begin[lo] + (chunk - t.blocks[lo]) * p.chunk_rows;
-    r1 = min(r0 + p.chunk_rows, t.begin[lo + 1]);
+    const int g = group_of_block(t, p.groups, chunk);
+    r0 = t.begin[g] + (chunk - t.blocks[g]) * p.chunk_rows;
+    r1 = min(r0 + p.chunk_rows, t.begin[g + 1]);
   } else {
     r0 = static_cast<int>(blockIdx.y) * p.chunk_rows;
     r1 = min(r0 + p.chunk_rows, p.rows);
@@ -284,23 +291,40 @@ act_grad_kernel(const __grid_constant__ LinearActGrad p) {
 }
 
 // The chunks' sums of each group added up: 32 columns x 8 strands of chunks to a
-// block, strands joined in order.
+// block, strands joined in order.  Short groups: only a group that took more than
+// one block (see act_grad_short_kernel) has anything left to add, and block y of the
+// second dimension does it for the group whose first further block is y: there are
+// as many of them as further blocks at most, not as many as groups.
 __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ LinearActGrad p) {
   extern __shared__ int ag_smem[];
   __shared__ float sums[8][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  int c0 = 0, c1 = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
+  int g = blockIdx.y, c0 = 0, c1 = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
   if (p.offsets) {
     GroupTable t{ag_smem, ag_smem + p.groups + 1};
-    build_group_table(t, p.offsets, p.groups, p.rows, p.chunk_rows);
-    c0 = t.blocks[blockIdx.y];
-    c1 = t.blocks[blockIdx.y + 1];
+    if (p.short_groups) {
+      build_group_table(t, p.offsets, p.groups, p.rows, kShortRows, kShortRows);
+      const int more = blockIdx.y;
+      if (more >= t.blocks[p.groups])
+        return;
+      g = group_of_block(t, p.groups, more);
+      if (more != t.blocks[g])
+        return;
+      c0 = p.groups + more;
+      c1 = p.groups + t.blocks[g + 1];
+    } else {
+      build_group_table(t, p.offsets, p.groups, p.rows, p.chunk_rows);
+      c0 = t.blocks[g];
+      c1 = t.blocks[g + 1];
+    }
   }
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const int col = static_cast<int>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
   if (col < p.cols) {
+    if (p.short_groups && strand == 0)
+      s = p.partial[static_cast<long long>(g) * p.cols + col];
 #pragma unroll 4
     for (int c = c0 + strand; c < c1; c += 8)
       s += p.partial[static_cast<long long>(c) * p.cols + col];
@@ -312,7 +336,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       total += sums[i][lane];
-    store_dbias(p, blockIdx.y, col, total);
+    store_dbias(p, g, col, total);
   }
 }
 
@@ -323,18 +347,36 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 // columns in us: 64 groups of 200 rows x 2048 66 / 52, 16 of 300 x 4096 47 / 39, 15
 // of 546 x 4096 73 / 67, 32 of 94 x 1032 17.0 / 16.0; one of 250 x 1024 11.1 / 12.6,
 // one of 250 x 4096 13.5 / 14.9.
+// That the groups are short is known of their mean only.  No block walks more than
+// kShortRows rows: blocks of the grid's second dimension behind the groups' own take
+// what is left of a longer group, so many rows each, and its column sums are then
+// partial, one row of `partial` to a block of that dimension
+// (column_sum_kernel).  One expert of 16 with all of 8192 rows x 2048, with dx: 263 us
+// without that limit, 57 with it (44 with 512 rows, 87 with 2048); one of 64 with
+// 40960 rows 1320 and 207; 16 of 300 x 4096 54.7 and 55.5.
 template <int kAct, bool kDyF32, bool kVec, int kCols>
 __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid_constant__ LinearActGrad p) {
   extern __shared__ int ag_smem[];
   __shared__ float sums[kAgThreads / 32][kCols];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int y = blockIdx.y;
   int r0 = 0, r1 = p.rows;
+  bool finished = true; // the group has no other block
   if (p.offsets) {
     GroupTable t{ag_smem, ag_smem + p.groups + 1};
-    build_group_table(t, p.offsets, p.groups, p.rows, 1);
-    r0 = t.begin[blockIdx.y];
-    r1 = t.begin[blockIdx.y + 1];
+    build_group_table(t, p.offsets, p.groups, p.rows, kShortRows, kShortRows);
+    int g = y, before = 0; // blocks of the group before this one
+    if (y >= p.groups) {
+      const int more = y - p.groups;
+      if (more >= t.blocks[p.groups])
+        return;
+      g = group_of_block(t, p.groups, more);
+      before = 1 + more - t.blocks[g];
+    }
+    r0 = t.begin[g] + before * kShortRows;
+    r1 = min(r0 + kShortRows, t.begin[g + 1]);
+    finished = t.blocks[g] == t.blocks[g + 1];
   }
   const int tc = threadIdx.x % (kCols / 8), tr = threadIdx.x / (kCols / 8);
   const int col = static_cast<int>(blockIdx.x) * kCols + tc * 8;
@@ -345,6 +387,8 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid
     acc[e] = 0.0f;
   if (live > 0)
     act_grad_rows<kAct, kDyF32, kVec, (kAct >= 0 && kCols * 2 >= 128), kAgThreads / (kCols / 8), (kVec && !kDyF32 ? kAgUnrollVec : kAgUnroll)>(p, r0 + tr, r1, col, live, acc);
+  if (!p.dbias)
+    return;
   // the rows of a warp, then the warps, in order
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -359,12 +403,15 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_short_kernel(const __grid
   }
   __syncthreads();
   const int c = static_cast<int>(blockIdx.x) * kCols + static_cast<int>(threadIdx.x);
-  if (p.dbias && threadIdx.x < kCols && c < p.cols) {
+  if (threadIdx.x < kCols && c < p.cols) {
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < kAgThreads / 32; ++i)
       total += sums[i][threadIdx.x];
-    store_dbias(p, blockIdx.y, c, total);
+    if (finished)
+      store_dbias(p, y, c, total);
+    else
+      p.partial[static_cast<long long>(y) * p.cols + c] = total;
   }
 }
 
@@ -384,6 +431,9 @@ cudaError_t launch_pack_rows(const PackRows &x, const PackRows &weights, int pdl
   return launch(dim3(static_cast<unsigned>(across), static_cast<unsigned>(x_rows + weights.groups)), kPackThreads, 0, stream, pdl,
                 pack_rows_kernel, PackTwo{x, weights, x_rows});
 }
+
+// (a group's further blocks have whole kShortRows of it in front of them)
+int linear_act_grad_short_more(int rows, int groups) { return groups == 0 ? 0 : rows / kShortRows; }
 
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows) {
   const int whole = (rows + chunk_rows - 1) / chunk_rows;
@@ -416,7 +466,8 @@ cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
   const unsigned groups = static_cast<unsigned>(p.offsets ? p.groups : 1);
   cudaError_t err = cudaSuccess;
   if (p.short_groups) {
-    const dim3 grid(static_cast<unsigned>((p.cols + p.short_cols - 1) / p.short_cols), groups);
+    const unsigned more = static_cast<unsigned>(linear_act_grad_short_more(p.rows, p.offsets ? p.groups : 0));
+    const dim3 grid(static_cast<unsigned>((p.cols + p.short_cols - 1) / p.short_cols), groups + more);
     auto go = [&](auto, auto kernel) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); };
     p.short_cols == 64 ? pick_act_grad<64>(p, go) : pick_act_grad<32>(p, go);
     return err;
@@ -426,9 +477,17 @@ cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>((p.cols + kAgCols - 1) / kAgCols), static_cast<unsigned>(chunks));
     pick_act_grad<32>(p, [&](auto kernel, auto) { err = launch(grid, kAgThreads, table, stream, p.pdl, kernel, p); });
   }
-  if (err != cudaSuccess || !p.dbias) // (without rows there are no partial sums, but a bias gradient of zero)
-    return err;
-  return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), groups), 256, table, stream, p.pdl, column_sum_kernel, p);
+  return err;
+}
+
+cudaError_t launch_column_sums(const LinearActGrad &p, cudaStream_t stream) {
+  const size_t table = p.offsets ? 2 * sizeof(int) * (static_cast<size_t>(p.groups) + 1) : 0;
+  const int y = p.short_groups ? linear_act_grad_short_more(p.rows, p.offsets ? p.groups : 0) : p.offsets ? p.groups : 1;
+  if (y == 0)
+    return cudaSuccess;
+  // (without rows there are no partial sums, but a bias gradient of zero)
+  return launch(dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(y)), 256, table, stream, p.pdl,
+                column_sum_kernel, p);
 }
 
 } // namespace wave

@@ -40,9 +40,10 @@ struct GroupTable {
   int *blocks; // [groups + 1]
 };
 
-// Executed by all threads of the block; ends with a barrier.
+// Executed by all threads of the block; ends with a barrier.  `skip`: so many of a
+// group's first rows are in no block.
 __device__ __forceinline__ void build_group_table(const GroupTable &t, const int *offsets, int groups, int rows,
-                                                  int block_rows) {
+                                                  int block_rows, int skip = 0) {
   for (int i = threadIdx.x; i <= groups; i += blockDim.x)
     t.begin[i] = offsets ? min(max(offsets[i], 0), rows) : (i == 0 ? 0 : rows);
   __syncthreads();
@@ -62,7 +63,7 @@ __device__ __forceinline__ void build_group_table(const GroupTable &t, const int
       int before = __shfl_up_sync(0xffffffffu, v, 1);
       if (lane == 0)
         before = base == 0 ? v : prev_last;
-      int n = i <= groups && i > 0 ? (v - before + block_rows - 1) / block_rows : 0; // row blocks of group i - 1
+      int n = i <= groups && i > 0 ? (max(v - before - skip, 0) + block_rows - 1) / block_rows : 0; // row blocks of group i - 1
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, n, d);

@@ -121,16 +121,20 @@ struct LinearActGrad {
   long long ldz;
   void *dZ; // null: column sums only
   long long lddz;
-  float *partial; // [chunks][cols], null: no column sums
+  float *partial; // [chunks][cols] (short groups: [blocks][cols], unused where one launch does it), null: no column sums
   int chunk_rows;
   void *dbias; // [groups][cols]
   int dbias_type; // 0 f32, 1 f16, 2 bf16
   int vec_dy, vec_z;
-  int short_groups; // all rows of a group to a block: no `partial`, one launch
+  int short_groups; // all rows of a group to a block, up to a limit
   int short_cols;   // columns of such a block, 32 or 64
   int pdl;
 };
 int linear_act_grad_chunks(int rows, int groups, int chunk_rows); // upper bound, sizes `partial`
+// Short groups (groups = 0: one of all rows): how many blocks there can be beside one for each group.  None: no group can
+// exceed a block, and one launch without `partial` does it all.
+int linear_act_grad_short_more(int rows, int groups);
 cudaError_t launch_act_grad(const LinearActGrad &p, cudaStream_t stream);
+cudaError_t launch_column_sums(const LinearActGrad &p, cudaStream_t stream); // what act_grad leaves of dbias
 
 } // namespace wave
