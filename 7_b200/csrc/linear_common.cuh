@@ -19,6 +19,13 @@ namespace linear_detail {
 // leaves idle, and small products run side by side (with it / one after the other,
 // in us: 8192 x 8192 x 2048 446 / 466, 515 x 1032 x 776 18.3 / 19.8, 24 experts,
 // 700 x 520 x 1288 34.5 / 37.8).
+// What a kernel with `beside` reads was written by a grid further back (dz by the
+// pass before the launch before it), and griddepcontrol.wait promises visibility
+// to the grid that waits, which that one was not in front of.  It rests on this
+// instead: the launch before it let it start only behind its own wait (or was
+// itself let start so), and the writing grid was complete and its writes performed,
+// in L2, before this one's first instruction; and this one reads none of it through L1, which might hold
+// something older: operands come by TMA, offsets by loads that go to L2.
 __device__ __forceinline__ void start_after_previous(int beside) {
   if (!beside)
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -41,11 +48,12 @@ struct GroupTable {
 };
 
 // Executed by all threads of the block; ends with a barrier.  `skip`: so many of a
-// group's first rows are in no block.
+// group's first rows are in no block.  (The offsets are read past L1, see
+// start_after_previous.)
 __device__ __forceinline__ void build_group_table(const GroupTable &t, const int *offsets, int groups, int rows,
                                                   int block_rows, int skip = 0) {
   for (int i = threadIdx.x; i <= groups; i += blockDim.x)
-    t.begin[i] = offsets ? min(max(offsets[i], 0), rows) : (i == 0 ? 0 : rows);
+    t.begin[i] = offsets ? min(max(__ldcg(offsets + i), 0), rows) : (i == 0 ? 0 : rows);
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
