@@ -143,6 +143,17 @@ int validate(const wave_linear_desc *d) {
   return WAVE_OK;
 }
 
+// A 16-bit result is summed in one accumulator, whose truncation costs 1.2e-9 of the
+// norm for each product (linear_sm100.cu), and its epilogue waits for the whole sum:
+// 2^26 products, a million stages of up to 0.55 us where every SM reads DRAM, are half
+// of the second after which a wait gives up.  f32 results are summed in pieces.
+constexpr int kLongestSum16 = 1 << 26;
+int check_sum(const char *result, int type, int products) {
+  if (type == WAVE_F32 || products <= kLongestSum16)
+    return WAVE_OK;
+  return fail(WAVE_E_UNSUPPORTED, "%s in 16 bits takes sums of at most 2^26 products; got %d", result, products);
+}
+
 // ------------------------------------------------------------------ products
 enum class Product { kForward, kInputGrad, kWeightGrad };
 
@@ -702,6 +713,8 @@ int wave_cuda_linear_fwd(const wave_linear_desc *d, const void *X, const void *W
       return fail(WAVE_E_INVALID, "X, W and Y must be non-null device pointers");
     if (!aligned16(X) || !aligned16(W))
       return fail(WAVE_E_INVALID, "X and W must be 16-byte aligned");
+    if ((rc = check_sum("y", d->y_type, d->in_features)) != WAVE_OK)
+      return rc;
     int sms = 0;
     if ((rc = sm_count(&sms)) != WAVE_OK)
       return rc;
@@ -736,6 +749,10 @@ int wave_cuda_linear_bwd(const wave_linear_desc *d, const void *dY, const void *
         return fail(WAVE_E_INVALID, "the gradient of an activation needs the pre-activation Z");
       if (!aligned16(dY) || (dW && !aligned16(X)) || (dX && !aligned16(W)))
         return fail(WAVE_E_INVALID, "dY, X and W must be 16-byte aligned");
+      if (dX && (rc = check_sum("dX", d->io_type, d->out_features)) != WAVE_OK)
+        return rc;
+      if (dW && (rc = check_sum("dW", d->dweight_type, d->tokens)) != WAVE_OK)
+        return rc;
     }
     int sms = 0;
     if ((rc = sm_count(&sms)) != WAVE_OK)
