@@ -252,7 +252,7 @@ def linear(x, weight, bias=None, residual=None, *, activation: str = "none", out
     (out,) in that type or f32; residual (tokens, out) in that type.
     `activation`: none, relu, gelu (erf), gelu_tanh or silu.  Returns y (tokens,
     out) in x's type, or f32 with `out_dtype`; `out` is written instead where it
-    is given and may be the residual.  With `save_pre_activation` returns (y, z),
+    is given; it may be the residual and overlaps no other tensor.  With `save_pre_activation` returns (y, z),
     z = x @ weight.T + bias in x's type, which the backward pass wants.  Few
     tokens -- one, in decoding -- read the weights at memory speed."""
     return _forward(x, weight, None, bias, residual, activation, out, out_dtype, save_pre_activation)
@@ -262,8 +262,9 @@ def linear_backward(dy, x, weight, *, activation: str = "none", pre_activation=N
                     need_dx: bool = True, need_dweight: bool = True, need_dbias: bool = True):
     """Gradients of `linear`: (dx, dweight, dbias), None for what is not needed.
     dz = dy * act'(pre_activation) is rounded to x's type for the two matrix
-    products; dx has x's type, dweight that or f32, dbias f32 (default) or that.
-    The residual's gradient is dy."""
+    products; dx has x's type, dweight that or f32 (its sums in 32 bits, of factors
+    in 16), dbias f32 (default) or that, from the unrounded dz.  The residual's
+    gradient is dy."""
     return _backward(dy, x, weight, None, activation, pre_activation, dweight_dtype, dbias_dtype, need_dx, need_dweight,
                      need_dbias)
 
@@ -273,8 +274,8 @@ def grouped_linear(x, weight, offsets, bias=None, *, activation: str = "none", o
     """`linear` with a weight matrix for each expert: rows offsets[g] to
     offsets[g + 1] of x (tokens, in), sorted by expert, go through weight[g] of
     (experts, out, in) and bias[g] of (experts, out).  offsets is an int32 tensor
-    of experts + 1 entries on the GPU; it stays there.  Experts without rows cost
-    nothing.  Rows that belong to no expert are zero in a new y and z and stay as
+    of experts + 1 entries on the GPU; it stays there.  Weights of experts
+    without rows are not read.  Rows that belong to no expert are zero in a new y and z and stay as
     they are in `out`."""
     if offsets is None:
         raise ValueError("offsets must be given")
