@@ -610,11 +610,13 @@ int chunk_rows(const Shape &s, int sms) {
 
 // Whether a block takes all rows of a group (up to a limit, as the mean is all that
 // is known here): one launch instead of two where no group can exceed it, and with
-// experts no search for the group of a chunk in each of many blocks.  What the
-// gradient of gelu or silu and the column sums add to dx, bf16, all rows / chunks
-// in us: 64 x 512 2.4 / 3.7, 128 x 4096 3.0 / 4.4, 250 x 1024 3.6 / 4.0, 500 x 1024
-// 5.4 / 4.2; 24 experts, 700 x 520 2.5 / 4.8; 32, 3000 x 1032 6.0 / 10; 15, 8190 x
-// 4096 35 / 44; 64, 16384 x 1024 21 / 27; 8, 8000 x 2048 30 / 23.
+// experts no search for the group of a chunk in each of many blocks.  All rows /
+// chunks in us, bf16: what the gradient of gelu or silu and the column sums add to
+// dx, 64 x 512 2.4 / 3.7, 128 x 4096 3.0 / 4.4, 250 x 1024 3.6 / 4.0, 500 x 1024 5.4 /
+// 4.2; both alone by expert, 24 with 700 rows x 520 in all 3.3 / 5.7, 32 with 3008 x
+// 1032 7.9 / 10.1, 64 with 16384 x 1024 21.7 / 24.9, 16 with 4800 x 4096 22.7 / 28.0,
+// 16 with 9600 x 4096 38.9 / 43.5 (with dx 105.5 / 105.9: here it ends); one of 16 with
+// all of 8192 x 2048, with dx, 58 / 40, and with the mean above it always chunks.
 bool short_groups(const Shape &s) {
   const long long rows = (s.d.tokens + s.matrices - 1) / s.matrices;
   return rows <= (s.grouped ? 640 : 256);
