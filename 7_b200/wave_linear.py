@@ -41,9 +41,20 @@ class _Plan:
                 wc.linear_validate(self.desc)
                 self.need = wc.linear_workspace_bytes(self.desc, backward)
             except wc.WaveCudaError as err:
-                if err.code in (wc.E_INVALID, wc.E_UNSUPPORTED):
-                    raise ValueError(err.message) from None
-                raise
+                raise _refusal(err) from None
+
+
+def _refusal(err):
+    """What the library refuses is a ValueError, like what is refused here."""
+    return ValueError(err.message) if err.code in (wc.E_INVALID, wc.E_UNSUPPORTED) else err
+
+
+def _check(code: int) -> None:
+    if code != wc.OK:
+        try:
+            wc.check(code)
+        except wc.WaveCudaError as err:
+            raise _refusal(err) from None
 
 
 _plans: dict = {}
@@ -192,8 +203,8 @@ def _forward(x, weight, offsets, bias, residual, activation, out, out_dtype, sav
     if save:  # rows that belong to no expert are left alone with `out`
         z = x.new_zeros(shape) if offsets is not None and out is not None else x.new_empty(shape)
     ws = _workspace(plan)
-    wc.check(wc.lib().wave_cuda_linear_fwd(plan.ref, px, pw, _ptr(bias), _ptr(residual), _ptr(offsets), y.data_ptr(), _ptr(z),
-                                           _ptr(ws), torch._C._cuda_getCurrentRawStream(plan.index)))
+    _check(wc.lib().wave_cuda_linear_fwd(plan.ref, px, pw, _ptr(bias), _ptr(residual), _ptr(offsets), y.data_ptr(), _ptr(z),
+                                         _ptr(ws), torch._C._cuda_getCurrentRawStream(plan.index)))
     return (y, z) if save else y
 
 
@@ -239,8 +250,8 @@ def _backward(dy, x, weight, offsets, activation, pre_activation, dweight_dtype,
     db = torch.empty(db_shape, dtype=db_type, device=plan.device) if need_dbias else None
     ws = _workspace(plan)
     z = _ptr(pre_activation) if plan.desc.activation else None
-    wc.check(wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
-                                           torch._C._cuda_getCurrentRawStream(plan.index)))
+    _check(wc.lib().wave_cuda_linear_bwd(plan.ref, pdy, px, pw, z, _ptr(offsets), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+                                         torch._C._cuda_getCurrentRawStream(plan.index)))
     return dx, dw, db
 
 
@@ -252,9 +263,10 @@ def linear(x, weight, bias=None, residual=None, *, activation: str = "none", out
     (out,) in that type or f32; residual (tokens, out) in that type.
     `activation`: none, relu, gelu (erf), gelu_tanh or silu.  Returns y (tokens,
     out) in x's type, or f32 with `out_dtype`; `out` is written instead where it
-    is given; it may be the residual and overlaps no other tensor.  With `save_pre_activation` returns (y, z),
-    z = x @ weight.T + bias in x's type, which the backward pass wants.  Few
-    tokens -- one, in decoding -- read the weights at memory speed."""
+    is given; it may be the residual and overlaps no other tensor.  With
+    `save_pre_activation` returns (y, z), z = x @ weight.T + bias in x's type, which
+    the backward pass wants.  Few tokens -- one, in decoding -- read the weights at
+    memory speed."""
     return _forward(x, weight, None, bias, residual, activation, out, out_dtype, save_pre_activation)
 
 
@@ -275,8 +287,8 @@ def grouped_linear(x, weight, offsets, bias=None, *, activation: str = "none", o
     offsets[g + 1] of x (tokens, in), sorted by expert, go through weight[g] of
     (experts, out, in) and bias[g] of (experts, out).  offsets is an int32 tensor
     of experts + 1 entries on the GPU; it stays there.  Weights of experts
-    without rows are not read.  Rows that belong to no expert are zero in a new y and z and stay as
-    they are in `out`."""
+    without rows are not read.  Rows that belong to no expert are zero in a new y and
+    z and stay as they are in `out`."""
     if offsets is None:
         raise ValueError("offsets must be given")
     return _forward(x, weight, offsets, bias, None, activation, out, out_dtype, save_pre_activation)

@@ -39,3 +39,19 @@ def test_what_is_not_asked_for_is_not_refused(wc):
                        (desc(wc, tokens=FAR, n=8, k=8), (None, None, Y)), (desc(wc, n=FAR, k=1), (None, Y, None)),
                        (desc(wc, tokens=0, n=FAR, k=1), (Y, None, None))):
         assert wc.lib().wave_cuda_linear_bwd(C.byref(d), Y, X, W, None, None, *results, Y, None) == wc.E_CUDA
+
+
+@pytest.mark.gpu
+def test_python_says_so_as_a_value_error(cuda, wc):
+    import importlib
+    wl = importlib.import_module("7_b200.wave_linear")
+    torch = cuda
+    x = torch.zeros(FAR, 1, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="dW in 16 bits takes sums of at most"):
+        wl.linear_backward(x, x, w)
+    with pytest.raises(ValueError, match="y in 16 bits takes sums of at most"):
+        wl.linear(x.view(1, FAR), x.view(1, FAR))
+    dx, dw, db = wl.linear_backward(x, x, w, need_dweight=False)
+    assert dw is None and not bool(dx.any()) and not bool(db.any())
+    wc.check_device_status()
